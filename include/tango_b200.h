@@ -446,6 +446,93 @@ int tango_enable_peer_access(int peer_device);
 int tango_peer_sync(uint64_t *const *slots /* device */, int rank, int world, uint64_t *round_word, const float *val_in,
                     float *val_out, int *status, int64_t limit_ns, tango_stream_t stream);
 
+/* ---------------------------------------------------------------- 8-bit rows
+ * A row-major matrix [rows, cols] is cut into groups of `group` neighbouring columns (the last one may be shorter).  A group
+ * holds int8 codes and one fp32 scale:
+ *   scale = max|x| / 127,   code = x / scale exactly rounded, ties to even (TANGO_ROUND_NEAREST),   value = code * scale.
+ * A group whose scale is below the normal numbers holds zeros; one with an infinity or a NaN has the scale NaN.  The other
+ * rounding modes truncate x / scale or add the stochastic stream of tango_quantize (element r * cols + c) first.
+ * Codes: group g of row r starts at q + r * tango_rows8_ld(cols, group) + g * tango_rows8_pitch(group); the bytes behind a
+ * group's last code are zero.  Scales: [rows, groups].  Groups have 1 to 1024 columns.  Element types of the matrices: */
+#define TANGO_FP32 0
+#define TANGO_BF16 1
+#define TANGO_FP16 2
+
+int64_t tango_rows8_pitch(int64_t group);
+int64_t tango_rows8_ld(int64_t cols, int64_t group);
+
+/* An 8-bit matrix, and one to be made from x (leading dimension ldx, elements).  Host structs, read before the call returns. */
+typedef struct tango_rows8 {
+    const int8_t *q;
+    const float *scales;
+} tango_rows8;
+typedef struct tango_rows8_job {
+    const void *x;
+    int64_t ldx;
+    int8_t *q;
+    float *scales;
+} tango_rows8_job;
+
+/* Up to four matrices of one shape and type in one launch; job j draws its random numbers with call + j.  Replaces what
+ * the reference keeps per tensor with one scale (ctx.backward_cache, cuda/QLinear.py:28-35). */
+int tango_rows8_pack(const tango_rows8_job *jobs, int n_jobs, int64_t rows, int64_t cols, int64_t group, int type, int mode,
+                     uint64_t seed, uint64_t call, const uint64_t *step, tango_stream_t stream);
+int tango_rows8_unpack(const int8_t *q, const float *scales, int64_t rows, int64_t cols, int64_t group, int type, void *out,
+                       int64_t ldo, tango_stream_t stream);
+
+/* y = f(x) and the 8-bit copy of x in one pass, and dx = dy * f'(copy).  act: 0 ELU (alpha 1), 1 GELU (erf), 2 SiLU; job->q
+ * and job->scales NULL: y alone.  In place of an activation whose input or output stays in fp32 until the backward pass
+ * (F.elu, evaluation/test_gat.py:165). */
+int tango_act8_forward(int act, const tango_rows8_job *job, int64_t rows, int64_t cols, int64_t group, int type, void *y, int64_t ldy,
+                       int mode, uint64_t seed, uint64_t call, const uint64_t *step, tango_stream_t stream);
+int tango_act8_backward(int act, const int8_t *q, const float *scales, int64_t rows, int64_t cols, int64_t group, int type,
+                        const void *dy, int64_t lddy, void *dx, int64_t lddx, tango_stream_t stream);
+
+/* ---------------------------------------------------------------- edge attention on 8-bit rows
+ * q, k, v and the incoming gradient o are 8-bit matrices [nodes, heads * d] with groups of d (a scale per node and head).
+ *   z = scale * <q[v], k[u]>,  p = softmax of z over the edges u -> v of row v,  out[v] = sum p v[u]      (no edges: 0)
+ * Row schedule (host struct; NULL: every row by one warp): rows [0, n_heavy) of row_order are cut into the units
+ * (row, first slot, end slot, unused), those of heavy_rows[i] being units heavy_first[i] .. heavy_first[i + 1]; rows up to
+ * n_long_rows get a warp, the rest a part of one.  Units need a workspace, 16-byte aligned, of
+ * tango_edge_attention_workspace_bytes (pass 0 forward, 1 bwd_dst, 2 bwd_src).  d <= 512.  Rows in one order of sums each.
+ * Replaces sddmm_u_dot_v -> edge_softmax -> spmm_u_mul_e (evaluation/test_HGT.py:58-62) and their backward passes. */
+typedef struct tango_edge_plan {
+    const int32_t *row_order;
+    int64_t n_long_rows;
+    const int32_t *units;
+    int64_t n_units;
+    const int32_t *heavy_rows;
+    const int32_t *heavy_first;
+    int64_t n_heavy;
+} tango_edge_plan;
+int64_t tango_edge_attention_workspace_bytes(int pass, int64_t n_units, int heads, int d);
+
+/* CSC in, out [rows, heads, d] contiguous of `type`; stats (optional) [rows, heads, 2] fp32: largest z * log2(e), 1 / sum. */
+int tango_edge_attention(const int32_t *indptr, const int32_t *indices, int64_t n_rows, const tango_edge_plan *plan, int heads, int d,
+                         const tango_rows8 *q, const tango_rows8 *k, const tango_rows8 *v, float scale, void *out, int type,
+                         float *stats, void *ws, int64_t ws_bytes, tango_stream_t stream);
+/* Gradients, the probabilities computed anew from stats.  bwd_dst walks the CSC and writes dq and record [rows, heads, 4] fp32
+ * (what bwd_src reads of a destination); bwd_src walks the CSR behind it and writes dk and dv. */
+int tango_edge_attention_bwd_dst(const int32_t *indptr, const int32_t *indices, int64_t n_rows, const tango_edge_plan *plan, int heads,
+                                 int d, const tango_rows8 *q, const tango_rows8 *k, const tango_rows8 *v, const tango_rows8 *grad,
+                                 float scale, const float *stats, void *dq, int type, float *record, void *ws, int64_t ws_bytes,
+                                 tango_stream_t stream);
+int tango_edge_attention_bwd_src(const int32_t *indptr, const int32_t *indices, int64_t n_rows, const tango_edge_plan *plan, int heads,
+                                 int d, const tango_rows8 *q, const tango_rows8 *k, const tango_rows8 *v, const tango_rows8 *grad,
+                                 const float *record, void *dk, void *dv, int type, void *ws, int64_t ws_bytes,
+                                 tango_stream_t stream);
+
+/* The same attention of n_rows nodes `rows` (int64, any order, repeats allowed; an id outside [0, n_nodes) gives a row of NaN)
+ * whose queries q [n_rows, heads, d] just arrived in `type` (leading dimension ldq, elements), over keys and values kept as
+ * 8-bit rows.  A row may be cut over `splits` blocks (1: none; tango_edge_attention_rows_splits gives a number for the
+ * longest row of the graph), which needs a workspace of tango_edge_attention_rows_workspace_bytes, 16-byte aligned. */
+int tango_edge_attention_rows_splits(int64_t n_rows, int64_t longest);
+int64_t tango_edge_attention_rows_workspace_bytes(int64_t n_rows, int splits, int heads, int d);
+int tango_edge_attention_rows(const int32_t *indptr, const int32_t *indices, int64_t n_nodes, const int64_t *rows, int64_t n_rows,
+                              int splits, int heads, int d, const void *q, int64_t ldq, int type, const tango_rows8 *k,
+                              const tango_rows8 *v, float scale, void *out, void *ws, int64_t ws_bytes, int mode, uint64_t seed,
+                              uint64_t call, const uint64_t *step, tango_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

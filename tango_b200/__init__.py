@@ -7,6 +7,8 @@ from . import config, graph, kernels, util  # noqa: F401
 from .QLinear import QLinear, Qlinear_func, Qlinear_func_reduce, QgemmNT_func  # noqa: F401
 from .SDDMM import sddmm_u_add_v, sddmm_u_dot_v  # noqa: F401
 from .SPMM import spmm_copy_u, spmm_u_mul_e  # noqa: F401
+from .attention import edge_attention, edge_attention_rows  # noqa: F401
+from .rows8 import Activation8, Packed8, activation8, pack8, unpack8  # noqa: F401
 from .util import graph_preprocess  # noqa: F401
 
 __version__ = "0.2.0"
@@ -23,5 +25,6 @@ def install_as_cuda() -> None:
     import sys
     sys.modules["cuda"] = sys.modules[__name__]
     # looked up by module name: the package attribute `QLinear` is the class, not the module
-    for name in ("kernels", "QLinear", "SPMM", "SDDMM", "util", "config", "graph", "_lib", "_native", "gnn", "dist", "peer"):
+    for name in ("kernels", "QLinear", "SPMM", "SDDMM", "util", "config", "graph", "_lib", "_native", "gnn", "dist", "peer",
+                 "attention", "rows8"):
         sys.modules[f"cuda.{name}"] = importlib.import_module(f"{__name__}.{name}")

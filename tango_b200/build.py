@@ -23,8 +23,9 @@ LIB_DIR = os.path.join(HERE, "lib")
 HEADER = os.path.join(ROOT, "include", "tango_b200.h")
 CUDA_HOME = os.environ.get("CUDA_HOME") or "/usr/local/cuda"
 LIB_PATH = os.path.join(LIB_DIR, "libtango_b200.so")
-SOURCES = ["quantize.cu", "quantize_fused.cu", "spmm.cu", "sddmm.cu", "gat_softmax.cu", "gat_project.cu", "igemm_tcgen05.cu", "peer.cu"]
-HOST_SOURCES = ["torch_ops.cpp", "torch_autograd.cpp", "torch_bind.cpp"]
+SOURCES = ["quantize.cu", "quantize_fused.cu", "spmm.cu", "sddmm.cu", "gat_softmax.cu", "gat_project.cu", "igemm_tcgen05.cu", "peer.cu",
+           "rows8.cu", "edge_attention.cu"]
+HOST_SOURCES = ["torch_ops.cpp", "torch_autograd.cpp", "torch_rows8.cpp", "torch_bind.cpp"]
 HOST_LIB_PATH = os.path.join(LIB_DIR, "_torch_ops.so")
 HOST_TAG_PATH = os.path.join(LIB_DIR, "_torch_ops.tag")     # what the host layer was built for
 # measurement aid of the benchmark, a library of its own (not part of the product ABI)
@@ -67,7 +68,7 @@ def built_tag() -> str:
 
 
 def _host_outdated() -> bool:
-    return built_tag() != host_tag() or _newer(HOST_LIB_PATH, _sources(".cpp", "torch_ops.h", "torch_autograd.h"))
+    return built_tag() != host_tag() or _newer(HOST_LIB_PATH, _sources(".cpp", ".h"))
 
 
 def needs_build() -> bool:

@@ -1,0 +1,783 @@
+// Dot-product attention over the edges of a graph, on 8-bit rows (rows8.cuh) with one scale per node and head.
+//
+//   z = scale * <q[v], k[u]>,  p = softmax of z over the edges u -> v of v,  out[v] = sum p v[u]           (forward)
+//   dp = <o[v], v[u]>,  delta[v] = sum p dp,  dq[v] = scale * sum p (dp - delta[v]) k[u]                    (by destination)
+//   dk[u] = scale * sum p (dp - delta[v]) q[v],  dv[u] = sum p o[v]                                         (by source)
+//
+// where q, k, v, o (the incoming gradient) are codes times scales.  No array of edges exists: the forward pass walks a row
+// once with the running maximum and sum of its softmax and leaves both per row and head; the backward passes compute the
+// probabilities from them again, bit for bit (the products of codes are exact integers and the three roundings behind them
+// are the same ones).  delta is not needed beforehand: dq = scale * (sum p dp k - delta sum p k), so one walk
+// gathers delta and both sums, and what the forward pass has to keep is the 8-bit rows and two floats per row and head.
+//
+// Sums are fp32, in one order per row length and shape (no atomics).  What bounds these kernels is the gather of 2 F bytes
+// per edge through L2 together with the instructions that turn codes into floats and add them up.
+//
+// A lane holds VB neighbouring codes of one head (16, less for narrow heads), P lanes a head, L = P * (heads of a block)
+// lanes an edge; the rest of a team of lanes takes further edges, U of them in flight per lane.  A row of more than 48 edges
+// has a warp, a shorter one a part of a warp; the longest ones are cut into units whose partial results are merged by a
+// second launch.
+#include "rows8.cuh"
+
+namespace tango {
+
+enum { FORWARD = 0, BY_DST = 1, BY_SRC = 2 };
+constexpr int kWarps = 8;
+
+struct AttnArgs {
+    const int32_t *indptr, *indices, *row_order;
+    const int4 *units;
+    int64_t n_units, n_heavy, n_long, n_rows;       // rows: [heavy: by units] [to n_long: a warp] [the rest: a team]
+    int heads, d, pitch, hb, team;                  // hb: heads of a block (a power of two); team: lanes of a short row
+    int64_t ld;                                     // bytes of a row of codes
+    const int8_t *fixed_a, *fixed_b, *gather_a, *gather_b;
+    const float *fixed_sa, *fixed_sb, *gather_sa, *gather_sb;
+    float qscale;                                   // scale * log2(e)
+    float2 *stats;                                  // [rows, heads]: maximum of z * log2(e), 1 / sum
+    float4 *record;                                 // [rows, heads], BY_DST writes and BY_SRC gathers: see there
+    void *out_a, *out_b;
+    int type;
+    float *ws;                                      // partial results of the units
+};
+
+// Results below the normal numbers become 0: a probability that small is lost beside the row's largest, which is 1.
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Two floats that one instruction works on.
+struct Pair { uint64_t v; };
+__device__ __forceinline__ Pair pair(float a, float b) {
+    Pair p;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p.v) : "f"(a), "f"(b));
+    return p;
+}
+__device__ __forceinline__ float2 both(Pair p) {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p.v));
+    return f;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+    Pair o;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(o.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return o;
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+    Pair o;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(o.v) : "l"(a.v), "l"(b.v));
+    return o;
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+    Pair o;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(o.v) : "l"(a.v), "l"(b.v));
+    return o;
+}
+__device__ __forceinline__ Pair shuffle2(Pair a, int lanes) { return {__shfl_xor_sync(0xffffffffu, a.v, lanes)}; }
+
+// VB codes.
+template <int VB> struct Codes { uint32_t w[VB / 4]; };
+template <int VB>
+__device__ __forceinline__ Codes<VB> load_codes(const int8_t *p, bool there) {
+    Codes<VB> c;
+#pragma unroll
+    for (int i = 0; i < VB / 4; ++i) c.w[i] = 0;
+    if (there) {
+        if constexpr (VB == 16) {
+            const uint4 t = __ldg(reinterpret_cast<const uint4 *>(p));
+            c.w[0] = t.x; c.w[1] = t.y; c.w[2] = t.z; c.w[3] = t.w;
+        } else if constexpr (VB == 8) {
+            const uint2 t = __ldg(reinterpret_cast<const uint2 *>(p));
+            c.w[0] = t.x; c.w[1] = t.y;
+        } else {
+            c.w[0] = __ldg(reinterpret_cast<const uint32_t *>(p));
+        }
+    }
+    return c;
+}
+// Exact product of two heads, the same number in all their P lanes.
+template <int VB, int P>
+__device__ __forceinline__ float dot(const Codes<VB> &a, const Codes<VB> &b) {
+    int s = 0;
+#pragma unroll
+    for (int i = 0; i < VB / 4; ++i) s = __dp4a((int)a.w[i], (int)b.w[i], s);
+#pragma unroll
+    for (int o = P / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    // up to 256 codes the sum is below 2^22 and sits in the mantissa of 1.5 * 2^23
+    if constexpr (VB * P <= 256) return __fsub_rn(__int_as_float(0x4B400000 + s), kRoundMagic);
+    else return __int2float_rn(s);
+}
+// acc += by * codes
+template <int VB>
+__device__ __forceinline__ void add_codes(Pair (&acc)[VB / 2], const Codes<VB> &c, Pair by) {
+    const Pair bias = pair(-8388736.f, -8388736.f);
+#pragma unroll
+    for (int i = 0; i < VB / 4; ++i) {
+        const uint32_t w = c.w[i] ^ 0x80808080u;
+        const Pair lo = pair(__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7440)), __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7441)));
+        const Pair hi = pair(__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7442)), __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7443)));
+        acc[2 * i] = fma2(add2(lo, bias), by, acc[2 * i]);
+        acc[2 * i + 1] = fma2(add2(hi, bias), by, acc[2 * i + 1]);
+    }
+}
+// accA += a * codes, accB += b * codes
+template <int VB>
+__device__ __forceinline__ void add_codes_twice(Pair (&accA)[VB / 2], Pair (&accB)[VB / 2], const Codes<VB> &c, Pair a, Pair b) {
+    const Pair bias = pair(-8388736.f, -8388736.f);
+#pragma unroll
+    for (int i = 0; i < VB / 4; ++i) {
+        const uint32_t w = c.w[i] ^ 0x80808080u;
+        const Pair lo = add2(pair(__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7440)), __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7441))), bias);
+        const Pair hi = add2(pair(__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7442)), __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7443))), bias);
+        accA[2 * i] = fma2(lo, a, accA[2 * i]);
+        accA[2 * i + 1] = fma2(hi, a, accA[2 * i + 1]);
+        accB[2 * i] = fma2(lo, b, accB[2 * i]);
+        accB[2 * i + 1] = fma2(hi, b, accB[2 * i + 1]);
+    }
+}
+
+// acc * by as elements e .. e + VB of a row of `out` (those below d).
+template <class T, int VB>
+__device__ __forceinline__ void store_row(T *out, int e, int d, const Pair (&acc)[VB / 2], float by) {
+#pragma unroll
+    for (int i = 0; i < VB; i += 4) {
+        const float2 a = both(acc[i / 2]), b = both(acc[i / 2 + 1]);
+        const float v[4] = {a.x * by, a.y * by, b.x * by, b.y * by};
+        if (d % 4 == 0) {
+            if (e + i < d) store4<T, 4>(out + e + i, 4, v);
+        } else {
+            store4<T, 1>(out + e + i, d - e - i, v);
+        }
+    }
+}
+template <int VB>
+__device__ __forceinline__ void store_typed(void *out, int64_t at, int type, int e, int d, const Pair (&acc)[VB / 2], float by) {
+    if (type == TANGO_FP32) store_row<float, VB>(static_cast<float *>(out) + at, e, d, acc, by);
+    else if (type == TANGO_BF16) store_row<Bf16, VB>(static_cast<Bf16 *>(out) + at, e, d, acc, by);
+    else store_row<Fp16, VB>(static_cast<Fp16 *>(out) + at, e, d, acc, by);
+}
+template <int VB>
+__device__ __forceinline__ void store_partial(float *ws, const Pair (&acc)[VB / 2]) {
+#pragma unroll
+    for (int i = 0; i < VB / 2; ++i) reinterpret_cast<float2 *>(ws)[i] = both(acc[i]);
+}
+
+// Floats of a unit's partial result: per head `PartialHeads` of them, then one or two sums per code.
+__host__ __device__ constexpr int partial_heads(int mode) { return mode == FORWARD ? 2 : mode == BY_DST ? 1 : 0; }
+__host__ __device__ constexpr int partial_sums(int mode) { return mode == FORWARD ? 1 : 2; }
+__host__ __device__ inline int64_t partial_floats(int mode, int heads, int64_t ld) {
+    return (partial_heads(mode) * heads + 3) / 4 * 4 + partial_sums(mode) * ld;
+}
+
+// A softmax that is being added up: running maximum (of z * log2 e), sum, weighted sums of codes.
+template <int VB> struct Running {
+    float m = -INFINITY, l = 0.f;
+    Pair acc[VB / 2];
+    __device__ Running() {
+#pragma unroll
+        for (int i = 0; i < VB / 2; ++i) acc[i] = pair(0.f, 0.f);
+    }
+    __device__ __forceinline__ void scale(float c) {
+        l *= c;
+        const Pair cc = pair(c, c);
+#pragma unroll
+        for (int i = 0; i < VB / 2; ++i) acc[i] = mul2(acc[i], cc);
+    }
+    // with the same place of the lanes at a distance of `lanes`
+    __device__ __forceinline__ void merge(int lanes) {
+        const float mo = __shfl_xor_sync(0xffffffffu, m, lanes), lo = __shfl_xor_sync(0xffffffffu, l, lanes);
+        const float top = fmaxf(m, mo);
+        const float c = m == -INFINITY ? 0.f : exp2_fast(m - top), co = mo == -INFINITY ? 0.f : exp2_fast(mo - top);
+        const Pair cc = pair(c, c), cco = pair(co, co);
+        m = top;
+        l = fmaf(l, c, lo * co);
+#pragma unroll
+        for (int i = 0; i < VB / 2; ++i) acc[i] = fma2(acc[i], cc, mul2(shuffle2(acc[i], lanes), cco));
+    }
+};
+
+// One step of the forward pass: U edges of a lane.  z = -inf marks an edge that is not there.
+template <int VB, int U>
+__device__ __forceinline__ void softmax_step(Running<VB> &r, const float (&z)[U], const float (&sv)[U], const Codes<VB> (&v)[U]) {
+    float top = r.m;
+#pragma unroll
+    for (int u = 0; u < U; ++u) top = fmaxf(top, z[u]);
+    if (__any_sync(0xffffffffu, top > r.m)) {       // seldom after the first edges of a row
+        r.scale(r.m == -INFINITY ? 0.f : exp2_fast(r.m - top));
+        r.m = top;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const float p = z[u] == -INFINITY ? 0.f : exp2_fast(z[u] - r.m);
+        r.l += p;
+        const float w = p * sv[u];
+        add_codes<VB>(r.acc, v[u], pair(w, w));
+    }
+}
+
+template <int MODE> struct InFlight { static constexpr int U = MODE == FORWARD ? 4 : 2; };
+
+template <int MODE, int VB, int P>
+__global__ void __launch_bounds__(kWarps * 32) attn_kernel(const __grid_constant__ AttnArgs a) {
+    constexpr int U = InFlight<MODE>::U;
+    const int lane = threadIdx.x & 31;
+    // ---- what this warp works on
+    int64_t w = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
+    int row = -1, beg = 0, end = 0, team = 32;
+    int64_t unit = -1;
+    if (w < a.n_units) {
+        unit = w;
+        const int4 t = __ldg(a.units + w);
+        row = t.x; beg = t.y; end = t.z;
+    } else {
+        int64_t at = w - a.n_units + a.n_heavy;
+        if (at >= a.n_long) {
+            team = a.team;
+            at = a.n_long + (at - a.n_long) * (32 / team) + lane / team;
+        }
+        if (at < a.n_rows) {
+            row = a.row_order ? __ldg(a.row_order + at) : (int)at;
+            beg = __ldg(a.indptr + row);
+            end = __ldg(a.indptr + row + 1);
+        }
+    }
+    const int L = a.hb * P, slots = team / L;
+    const int slot = (lane & (team - 1)) / L, in_edge = lane & (L - 1);
+    const int head = blockIdx.y * a.hb + in_edge / P, chunk = in_edge & (P - 1);
+    const bool has_head = head < a.heads, live = has_head && chunk * VB < a.pitch;
+    const int64_t off = (int64_t)head * a.pitch + chunk * VB;
+
+    // ---- the row's own operands
+    const bool mine = row >= 0 && live;
+    const int64_t rh = (int64_t)row * a.heads + head;
+    const Codes<VB> fa = load_codes<VB>(a.fixed_a + (int64_t)row * a.ld + off, mine);
+    Codes<VB> fb;
+    if constexpr (MODE != FORWARD) fb = load_codes<VB>(a.fixed_b + (int64_t)row * a.ld + off, mine);
+    float sa = 0.f, sb = 0.f, top = 0.f, inv = 0.f;
+    if (row >= 0 && has_head) {
+        sa = __ldg(a.fixed_sa + rh);
+        if constexpr (MODE != FORWARD) sb = __ldg(a.fixed_sb + rh);
+        if constexpr (MODE == BY_DST) {
+            const float2 st = __ldg(a.stats + rh);
+            top = st.x; inv = st.y;
+        }
+    }
+    if constexpr (MODE != BY_SRC) sa *= a.qscale;
+
+    Running<VB> run;                    // forward: the softmax; else acc = the first sum
+    Pair acc2[VB / 2];
+    float delta = 0.f;
+#pragma unroll
+    for (int i = 0; i < VB / 2; ++i) acc2[i] = pair(0.f, 0.f);
+
+    const int stride = slots * U;
+    const int trips = (int)__reduce_max_sync(0xffffffffu, (unsigned)((end - beg + stride - 1) / stride));
+    int j = beg + slot, next[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) next[u] = j + u * slots < end ? __ldg(a.indices + j + u * slots) : -1;
+    for (int t = 0; t < trips; ++t) {
+        Codes<VB> ga[U], gb[U];
+        float ta[U], tb[U];
+        float4 rec[U];
+        bool there[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            there[u] = next[u] >= 0;
+            const int64_t at = (int64_t)next[u] * a.ld + off;
+            ga[u] = load_codes<VB>(a.gather_a + at, there[u] && live);
+            gb[u] = load_codes<VB>(a.gather_b + at, there[u] && live);
+            ta[u] = tb[u] = 0.f;
+            rec[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (there[u] && has_head) {
+                const int64_t h = (int64_t)next[u] * a.heads + head;
+                if constexpr (MODE == BY_SRC) {
+                    rec[u] = __ldg(a.record + h);
+                } else {
+                    ta[u] = __ldg(a.gather_sa + h);
+                    tb[u] = __ldg(a.gather_sb + h);
+                }
+            }
+        }
+        j += stride;
+#pragma unroll
+        for (int u = 0; u < U; ++u) next[u] = j + u * slots < end ? __ldg(a.indices + j + u * slots) : -1;
+        if constexpr (MODE == FORWARD) {
+            float z[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const float s = dot<VB, P>(fa, ga[u]);
+                z[u] = there[u] ? __fmul_rn(s, __fmul_rn(ta[u], sa)) : -INFINITY;
+            }
+            softmax_step<VB, U>(run, z, tb, gb);
+        } else if constexpr (MODE == BY_DST) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const float s = dot<VB, P>(fa, ga[u]), dp = dot<VB, P>(fb, gb[u]) * tb[u];
+                const float z = __fmul_rn(s, __fmul_rn(ta[u], sa));
+                const float p = there[u] ? exp2_fast(z - top) * inv : 0.f;
+                delta = fmaf(p, dp, delta);
+                const float pk = p * ta[u], pdk = pk * dp;
+                add_codes_twice<VB>(run.acc, acc2, ga[u], pair(pdk, pdk), pair(pk, pk));
+            }
+        } else {
+            // record of a destination: scale * log2(e) * scale of q, maximum, scale of o / sum, delta / scale of o
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const float s = dot<VB, P>(fa, ga[u]), dp = dot<VB, P>(fb, gb[u]) * sb;
+                const float z = __fmul_rn(s, __fmul_rn(sa, rec[u].x));
+                const float p = there[u] ? exp2_fast(z - rec[u].y) * rec[u].z : 0.f;
+                const float ds = p * (dp - rec[u].w) * rec[u].x;
+                add_codes<VB>(run.acc, ga[u], pair(ds, ds));
+                add_codes<VB>(acc2, gb[u], pair(p, p));
+            }
+        }
+    }
+
+    // ---- the slots of a team meet
+    for (int o = L; o < team; o <<= 1) {
+        if constexpr (MODE == FORWARD) {
+            run.merge(o);
+        } else {
+            delta += __shfl_xor_sync(0xffffffffu, delta, o);
+#pragma unroll
+            for (int i = 0; i < VB / 2; ++i) {
+                run.acc[i] = add2(run.acc[i], shuffle2(run.acc[i], o));
+                acc2[i] = add2(acc2[i], shuffle2(acc2[i], o));
+            }
+        }
+    }
+    if (slot != 0 || row < 0 || !live) return;
+    if (unit >= 0) {
+        float *ws = a.ws + unit * partial_floats(MODE, a.heads, a.ld);
+        if (chunk == 0) {
+            if constexpr (MODE == FORWARD) { ws[2 * head] = run.m; ws[2 * head + 1] = run.l; }
+            if constexpr (MODE == BY_DST) ws[head] = delta;
+        }
+        ws += (partial_heads(MODE) * a.heads + 3) / 4 * 4 + off;
+        store_partial<VB>(ws, run.acc);
+        if constexpr (MODE != FORWARD) store_partial<VB>(ws + a.ld, acc2);
+        return;
+    }
+    const int64_t out = rh * a.d;
+    const int e = chunk * VB;
+    if constexpr (MODE == FORWARD) {
+        const float by = run.l == 0.f ? 0.f : __fdiv_rn(1.f, run.l);
+        store_typed<VB>(a.out_a, out, a.type, e, a.d, run.acc, by);
+        if (chunk == 0 && a.stats) a.stats[rh] = make_float2(run.l == 0.f ? 0.f : run.m, by);
+    } else if constexpr (MODE == BY_DST) {
+        const Pair nd = pair(-delta, -delta);
+#pragma unroll
+        for (int i = 0; i < VB / 2; ++i) run.acc[i] = fma2(acc2[i], nd, run.acc[i]);
+        store_typed<VB>(a.out_a, out, a.type, e, a.d, run.acc, a.qscale * 0.69314718055994531f * sb);
+        if (chunk == 0) a.record[rh] = make_float4(sa, top, inv * sb, delta);
+    } else {
+        store_typed<VB>(a.out_a, out, a.type, e, a.d, run.acc, 0.69314718055994531f);
+        store_typed<VB>(a.out_b, out, a.type, e, a.d, acc2, 1.f);
+    }
+}
+
+// One block per heavy row: its units in order.
+struct MergeArgs {
+    const int32_t *heavy_rows, *heavy_first;
+    int heads, d, pitch;
+    int64_t ld;
+    const float *ws;
+    const float *fixed_sa, *fixed_sb;
+    float qscale;
+    float2 *stats;
+    float4 *record;
+    void *out_a, *out_b;
+    int type;
+};
+__device__ __forceinline__ void store_one(void *out, int64_t at, int type, float v) {
+    if (type == TANGO_FP32) static_cast<float *>(out)[at] = v;
+    else if (type == TANGO_BF16) from_float(v, static_cast<Bf16 *>(out)[at]);
+    else from_float(v, static_cast<Fp16 *>(out)[at]);
+}
+template <int MODE>
+__global__ void __launch_bounds__(256) attn_merge_kernel(const __grid_constant__ MergeArgs a) {
+    const int64_t row = __ldg(a.heavy_rows + blockIdx.x);
+    const int first = __ldg(a.heavy_first + blockIdx.x), last = __ldg(a.heavy_first + blockIdx.x + 1);
+    const int64_t step = partial_floats(MODE, a.heads, a.ld);
+    const float *ws = a.ws + (int64_t)first * step;
+    const int n = last - first, per_head = (partial_heads(MODE) * a.heads + 3) / 4 * 4;
+    for (int e = threadIdx.x; e < a.ld; e += blockDim.x) {
+        const int head = e / a.pitch, i = e - head * a.pitch;
+        const int64_t rh = row * a.heads + head, out = rh * a.d + i;
+        if (i >= a.d) continue;
+        if constexpr (MODE == FORWARD) {
+            float m = -INFINITY;
+            for (int u = 0; u < n; ++u) m = fmaxf(m, ws[u * step + 2 * head]);
+            float l = 0.f, s = 0.f;
+            for (int u = 0; u < n; ++u) {
+                const float mu = ws[u * step + 2 * head], c = mu == -INFINITY ? 0.f : exp2_fast(mu - m);
+                l = fmaf(ws[u * step + 2 * head + 1], c, l);
+                s = fmaf(ws[u * step + per_head + e], c, s);
+            }
+            const float by = l == 0.f ? 0.f : __fdiv_rn(1.f, l);
+            store_one(a.out_a, out, a.type, s * by);
+            if (i == 0 && a.stats) a.stats[rh] = make_float2(l == 0.f ? 0.f : m, by);
+        } else {
+            float delta = 0.f, x = 0.f, y = 0.f;
+            for (int u = 0; u < n; ++u) {
+                if constexpr (MODE == BY_DST) delta += ws[u * step + head];
+                x += ws[u * step + per_head + e];
+                y += ws[u * step + per_head + a.ld + e];
+            }
+            if constexpr (MODE == BY_DST) {
+                const float sb = a.fixed_sb[rh];
+                store_one(a.out_a, out, a.type, fmaf(y, -delta, x) * (a.qscale * 0.69314718055994531f * sb));
+                if (i == 0) {
+                    const float2 st = a.stats[rh];
+                    a.record[rh] = make_float4(a.fixed_sa[rh] * a.qscale, st.x, st.y * sb, delta);
+                }
+            } else {
+                store_one(a.out_a, out, a.type, x * 0.69314718055994531f);
+                store_one(a.out_b, out, a.type, y);
+            }
+        }
+    }
+}
+
+// ---- a few rows whose queries just arrived: a whole block a row, long rows over several blocks
+struct RowsArgs {
+    const int32_t *indptr, *indices;
+    const int64_t *rows;
+    int64_t n_nodes;
+    const void *q;
+    int64_t ldq;                  // elements between two queries
+    int heads, d, pitch, hb;
+    int64_t ld;
+    const int8_t *k, *v;
+    const float *sk, *sv;
+    float qscale;
+    int splits;                   // blocks a row may be cut into
+    void *out;
+    int type;
+    float *ws;                    // [rows, splits] partial results
+    int mode;
+    uint64_t seed, call;
+    const unsigned long long *step;
+};
+constexpr int kRowChunk = 1024;   // edges below which a row is not cut
+
+__host__ __device__ inline int row_chunk(int len, int splits) {
+    const int c = (len + splits - 1) / splits;
+    return c < kRowChunk ? kRowChunk : c;
+}
+
+template <int VB, int P, class T>
+__device__ __forceinline__ Codes<VB> encode_query(const RowsArgs &a, int64_t r, int head, int chunk, bool live, float &s) {
+    const int64_t at = r * a.ldq + (int64_t)head * a.d + chunk * VB;
+    float v[VB / 4][4];
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < VB / 4; ++i) {
+        load4<T, 1>(static_cast<const T *>(a.q) + at + 4 * i, live ? min(4, a.d - chunk * VB - 4 * i) : 0, v[i]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) top = max(top, __float_as_uint(v[i][k]) & 0x7fffffffu);
+    }
+#pragma unroll
+    for (int o = P / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    s = group_scale(top);
+    const float inv = group_inverse(s);
+    Codes<VB> c;
+#pragma unroll
+    for (int i = 0; i < VB / 4; ++i)
+        c.w[i] = a.mode == TANGO_ROUND_NEAREST
+                     ? encode4(v[i], s, inv)
+                     : encode4_mode(v[i], s, a.mode, a.seed, effective_call(a.call, a.step),
+                                    (uint64_t)r * a.heads * a.d + head * a.d + chunk * VB + 4 * i);
+    return c;
+}
+
+template <int VB, int P>
+__global__ void __launch_bounds__(kWarps * 32) attn_rows_kernel(const __grid_constant__ RowsArgs a) {
+    constexpr int U = InFlight<FORWARD>::U;
+    __shared__ float s_acc[kWarps][32 * VB];
+    __shared__ float2 s_ml[kWarps][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t r = blockIdx.x;
+    const int64_t row = __ldg(a.rows + r);
+    const bool known = row >= 0 && row < a.n_nodes;
+    const int beg0 = known ? __ldg(a.indptr + row) : 0, end0 = known ? __ldg(a.indptr + row + 1) : 0;
+    const int chunk_len = row_chunk(end0 - beg0, a.splits);
+    const bool whole = end0 - beg0 <= chunk_len;
+    if (blockIdx.y > 0 && (int64_t)blockIdx.y * chunk_len >= end0 - beg0) return;
+    const int beg = beg0 + blockIdx.y * chunk_len, end = end0 - beg < chunk_len ? end0 : beg + chunk_len;
+
+    const int L = a.hb * P, slots = 32 / L;
+    const int slot = lane / L, in_edge = lane & (L - 1);
+    const int head = blockIdx.z * a.hb + in_edge / P, chunk = in_edge & (P - 1);
+    const bool has_head = head < a.heads, live = has_head && chunk * VB < a.pitch;
+    const int64_t off = (int64_t)head * a.pitch + chunk * VB;
+    float sa;
+    const Codes<VB> fa = a.type == TANGO_FP32   ? encode_query<VB, P, float>(a, r, head, chunk, live, sa)
+                         : a.type == TANGO_BF16 ? encode_query<VB, P, Bf16>(a, r, head, chunk, live, sa)
+                                                : encode_query<VB, P, Fp16>(a, r, head, chunk, live, sa);
+    sa *= a.qscale;
+    Running<VB> run;
+    const int stride = slots * U * kWarps;
+    for (int j = beg + warp * slots * U; j < end; j += stride) {
+        Codes<VB> ga[U], gb[U];
+        float z[U], ta[U], tb[U];
+        int at[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int e = j + u * slots + slot;
+            at[u] = e < end ? __ldg(a.indices + e) : -1;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const bool there = at[u] >= 0;
+            ga[u] = load_codes<VB>(a.k + (int64_t)at[u] * a.ld + off, there && live);
+            gb[u] = load_codes<VB>(a.v + (int64_t)at[u] * a.ld + off, there && live);
+            ta[u] = tb[u] = 0.f;
+            if (there && has_head) {
+                ta[u] = __ldg(a.sk + (int64_t)at[u] * a.heads + head);
+                tb[u] = __ldg(a.sv + (int64_t)at[u] * a.heads + head);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const float s = dot<VB, P>(fa, ga[u]);
+            z[u] = at[u] >= 0 ? __fmul_rn(s, __fmul_rn(ta[u], sa)) : -INFINITY;
+        }
+        softmax_step<VB, U>(run, z, tb, gb);
+    }
+    for (int o = L; o < 32; o <<= 1) run.merge(o);
+    if (slot == 0) {
+        s_ml[warp][in_edge] = make_float2(run.m, run.l);
+#pragma unroll
+        for (int i = 0; i < VB / 2; ++i) reinterpret_cast<float2 *>(s_acc[warp])[in_edge * (VB / 2) + i] = both(run.acc[i]);
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < L * VB; e += kWarps * 32) {
+        const int ie = e / VB, hd = blockIdx.z * a.hb + ie / P, i = (ie & (P - 1)) * VB + e % VB;
+        if (hd >= a.heads || i >= a.d) continue;
+        float m = -INFINITY, l = 0.f, s = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) m = fmaxf(m, s_ml[w][ie].x);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            const float2 ml = s_ml[w][ie];
+            const float c = ml.x == -INFINITY ? 0.f : exp2_fast(ml.x - m);
+            l = fmaf(ml.y, c, l);
+            s = fmaf(s_acc[w][e], c, s);
+        }
+        if (whole) {
+            const float by = !known ? __int_as_float(0x7fffffff) : l == 0.f ? 0.f : __fdiv_rn(1.f, l);
+            store_one(a.out, (r * a.heads + hd) * a.d + i, a.type, s * by);
+        } else {
+            float *ws = a.ws + (r * a.splits + blockIdx.y) * partial_floats(FORWARD, a.heads, a.ld);
+            if (i == 0) { ws[2 * hd] = m; ws[2 * hd + 1] = l; }
+            ws[(2 * a.heads + 3) / 4 * 4 + hd * a.pitch + i] = s;
+        }
+    }
+}
+
+__global__ void __launch_bounds__(256) attn_rows_merge_kernel(const __grid_constant__ RowsArgs a) {
+    const int64_t r = blockIdx.x, row = __ldg(a.rows + r);
+    if (row < 0 || row >= a.n_nodes) return;
+    const int len = __ldg(a.indptr + row + 1) - __ldg(a.indptr + row), chunk_len = row_chunk(len, a.splits);
+    if (len <= chunk_len) return;
+    const int n = (len + chunk_len - 1) / chunk_len, per_head = (2 * a.heads + 3) / 4 * 4;
+    const int64_t step = partial_floats(FORWARD, a.heads, a.ld);
+    const float *ws = a.ws + r * a.splits * step;
+    for (int e = threadIdx.x; e < a.ld; e += blockDim.x) {
+        const int head = e / a.pitch, i = e - head * a.pitch;
+        if (i >= a.d) continue;
+        float m = -INFINITY, l = 0.f, s = 0.f;
+        for (int u = 0; u < n; ++u) m = fmaxf(m, ws[u * step + 2 * head]);
+        for (int u = 0; u < n; ++u) {
+            const float mu = ws[u * step + 2 * head], c = mu == -INFINITY ? 0.f : exp2_fast(mu - m);
+            l = fmaf(ws[u * step + 2 * head + 1], c, l);
+            s = fmaf(ws[u * step + per_head + e], c, s);
+        }
+        store_one(a.out, (r * a.heads + head) * a.d + i, a.type, s * (l == 0.f ? 0.f : __fdiv_rn(1.f, l)));
+    }
+}
+
+// ---- host side
+constexpr int kMaxHeadWidth = 512;
+
+// The instantiation of a head width: codes of a lane and lanes of a head.
+template <class F>
+static int with_shape(int d, F f) {
+    if (d <= 4) return f(std::integral_constant<int, 4>{}, std::integral_constant<int, 1>{});
+    if (d <= 8) return f(std::integral_constant<int, 8>{}, std::integral_constant<int, 1>{});
+    const std::integral_constant<int, 16> vb{};
+    if (d <= 16) return f(vb, std::integral_constant<int, 1>{});
+    if (d <= 32) return f(vb, std::integral_constant<int, 2>{});
+    if (d <= 64) return f(vb, std::integral_constant<int, 4>{});
+    if (d <= 128) return f(vb, std::integral_constant<int, 8>{});
+    if (d <= 256) return f(vb, std::integral_constant<int, 16>{});
+    return f(vb, std::integral_constant<int, 32>{});
+}
+static int heads_of_a_block(int heads, int p) {
+    int hb = 1;
+    while (hb < heads && hb * 2 * p <= 32) hb *= 2;
+    return hb;
+}
+static bool known_type(int type) { return type >= TANGO_FP32 && type <= TANGO_FP16; }
+
+static int check_shape(int64_t n_rows, int heads, int d, int type) {
+    if (n_rows < 0 || heads < 1 || d < 1 || !known_type(type)) return TANGO_EINVAL;
+    if (d > kMaxHeadWidth || heads > 65535 || n_rows > 0x7fffffffLL) return TANGO_ESIZE;
+    return TANGO_OK;
+}
+
+template <int MODE>
+static int launch(AttnArgs a, const tango_edge_plan *plan, float *ws, int64_t ws_bytes, cudaStream_t st) {
+    a.n_long = a.n_rows;
+    if (plan) {
+        a.row_order = plan->row_order;
+        a.units = reinterpret_cast<const int4 *>(plan->units);
+        a.n_units = plan->n_units; a.n_heavy = plan->n_heavy;
+        if (plan->row_order) a.n_long = plan->n_long_rows;
+        if (a.n_units < 0 || a.n_heavy < 0 || a.n_long < a.n_heavy || a.n_long > a.n_rows) return TANGO_EINVAL;
+        if (a.n_heavy > 0 && (!plan->units || !plan->row_order || !plan->heavy_rows || !plan->heavy_first || !ws ||
+                              ws_bytes < a.n_units * partial_floats(MODE, a.heads, a.ld) * 4))
+            return TANGO_EINVAL;
+        if (!aligned(plan->units, 16) || !aligned(ws, 16)) return TANGO_EALIGN;
+    }
+    a.ws = ws;
+    const int rc = with_shape(a.d, [&](auto vb, auto p) -> int {
+        constexpr int VB = decltype(vb)::value, P = decltype(p)::value;
+        a.hb = heads_of_a_block(a.heads, P);
+        a.team = a.hb * P > 8 ? a.hb * P : 8;
+        const int64_t warps = a.n_units + (a.n_long - a.n_heavy) + ceil_div(a.n_rows - a.n_long, 32 / a.team);
+        const int64_t blocks = ceil_div(warps, kWarps), by = ceil_div(a.heads, a.hb);
+        if (blocks > 0x7fffffffLL || by > 65535) return TANGO_ESIZE;
+        attn_kernel<MODE, VB, P><<<dim3((unsigned)blocks, (unsigned)by), kWarps * 32, 0, st>>>(a);
+        TANGO_LAUNCH_CHECK();
+        return TANGO_OK;
+    });
+    if (rc != TANGO_OK || a.n_heavy == 0) return rc;
+    MergeArgs m{plan->heavy_rows, plan->heavy_first, a.heads, a.d, a.pitch, a.ld, ws, a.fixed_sa, a.fixed_sb, a.qscale,
+                a.stats, a.record, a.out_a, a.out_b, a.type};
+    attn_merge_kernel<MODE><<<(unsigned)a.n_heavy, 256, 0, st>>>(m);
+    TANGO_LAUNCH_CHECK();
+    return TANGO_OK;
+}
+
+static bool good_codes(const tango_rows8 *r, int d) { return r && r->q && r->scales && aligned(r->q, d > 8 ? 16 : d > 4 ? 8 : 4); }
+
+static AttnArgs attn_args(const int32_t *indptr, const int32_t *indices, int64_t n_rows, int heads, int d, float scale, int type) {
+    AttnArgs a{};
+    a.indptr = indptr; a.indices = indices; a.n_rows = n_rows;
+    a.heads = heads; a.d = d; a.pitch = (int)tango_rows8_pitch(d); a.ld = (int64_t)heads * a.pitch;
+    a.qscale = scale * 1.4426950408889634f;
+    a.type = type;
+    return a;
+}
+
+}  // namespace tango
+
+using namespace tango;
+
+extern "C" int64_t tango_edge_attention_workspace_bytes(int pass, int64_t n_units, int heads, int d) {
+    if (pass < FORWARD || pass > BY_SRC || n_units < 0 || heads < 1 || d < 1) return TANGO_EINVAL;
+    if (d > kMaxHeadWidth || heads > 65535 || n_units > (1LL << 31)) return TANGO_ESIZE;
+    return n_units * partial_floats(pass, heads, heads * tango_rows8_pitch(d)) * 4;
+}
+
+extern "C" int tango_edge_attention(const int32_t *indptr, const int32_t *indices, int64_t n_rows, const tango_edge_plan *plan,
+                                    int heads, int d, const tango_rows8 *q, const tango_rows8 *k, const tango_rows8 *v, float scale,
+                                    void *out, int type, float *stats, void *ws, int64_t ws_bytes, tango_stream_t stream) {
+    const int rc = check_shape(n_rows, heads, d, type);
+    if (rc != TANGO_OK || n_rows == 0) return rc;
+    if (!indptr || !indices || !out) return TANGO_EINVAL;
+    for (const tango_rows8 *r : {q, k, v})
+        if (!good_codes(r, d)) return TANGO_EINVAL;
+    if (!aligned(out, 16) || !aligned(stats, 8)) return TANGO_EALIGN;
+    AttnArgs a = attn_args(indptr, indices, n_rows, heads, d, scale, type);
+    a.fixed_a = q->q; a.fixed_sa = q->scales;
+    a.gather_a = k->q; a.gather_sa = k->scales; a.gather_b = v->q; a.gather_sb = v->scales;
+    a.stats = reinterpret_cast<float2 *>(stats); a.out_a = out;
+    return launch<FORWARD>(a, plan, static_cast<float *>(ws), ws_bytes, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int tango_edge_attention_bwd_dst(const int32_t *indptr, const int32_t *indices, int64_t n_rows, const tango_edge_plan *plan,
+                                            int heads, int d, const tango_rows8 *q, const tango_rows8 *k, const tango_rows8 *v,
+                                            const tango_rows8 *grad, float scale, const float *stats, void *dq, int type, float *record,
+                                            void *ws, int64_t ws_bytes, tango_stream_t stream) {
+    const int rc = check_shape(n_rows, heads, d, type);
+    if (rc != TANGO_OK || n_rows == 0) return rc;
+    if (!indptr || !indices || !dq || !stats || !record) return TANGO_EINVAL;
+    for (const tango_rows8 *r : {q, k, v, grad})
+        if (!good_codes(r, d)) return TANGO_EINVAL;
+    if (!aligned(dq, 16) || !aligned(stats, 8) || !aligned(record, 16)) return TANGO_EALIGN;
+    AttnArgs a = attn_args(indptr, indices, n_rows, heads, d, scale, type);
+    a.fixed_a = q->q; a.fixed_sa = q->scales; a.fixed_b = grad->q; a.fixed_sb = grad->scales;
+    a.gather_a = k->q; a.gather_sa = k->scales; a.gather_b = v->q; a.gather_sb = v->scales;
+    a.stats = reinterpret_cast<float2 *>(const_cast<float *>(stats)); a.record = reinterpret_cast<float4 *>(record); a.out_a = dq;
+    return launch<BY_DST>(a, plan, static_cast<float *>(ws), ws_bytes, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int tango_edge_attention_bwd_src(const int32_t *indptr, const int32_t *indices, int64_t n_rows, const tango_edge_plan *plan,
+                                            int heads, int d, const tango_rows8 *q, const tango_rows8 *k, const tango_rows8 *v,
+                                            const tango_rows8 *grad, const float *record, void *dk, void *dv, int type, void *ws,
+                                            int64_t ws_bytes, tango_stream_t stream) {
+    const int rc = check_shape(n_rows, heads, d, type);
+    if (rc != TANGO_OK || n_rows == 0) return rc;
+    if (!indptr || !indices || !dk || !dv || !record) return TANGO_EINVAL;
+    for (const tango_rows8 *r : {q, k, v, grad})
+        if (!good_codes(r, d)) return TANGO_EINVAL;
+    if (!aligned(dk, 16) || !aligned(dv, 16) || !aligned(record, 16)) return TANGO_EALIGN;
+    AttnArgs a = attn_args(indptr, indices, n_rows, heads, d, 0.f, type);
+    a.fixed_a = k->q; a.fixed_sa = k->scales; a.fixed_b = v->q; a.fixed_sb = v->scales;
+    a.gather_a = q->q; a.gather_sa = q->scales; a.gather_b = grad->q; a.gather_sb = grad->scales;
+    a.record = reinterpret_cast<float4 *>(const_cast<float *>(record)); a.out_a = dk; a.out_b = dv;
+    return launch<BY_SRC>(a, plan, static_cast<float *>(ws), ws_bytes, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int tango_edge_attention_rows_splits(int64_t n_rows, int64_t longest) {
+    if (n_rows < 0 || longest < 0) return TANGO_EINVAL;
+    if (n_rows == 0 || longest <= kRowChunk) return 1;
+    const int64_t most = 64, want = ceil_div(longest, kRowChunk);
+    return (int)(want < most ? want : most);
+}
+
+extern "C" int64_t tango_edge_attention_rows_workspace_bytes(int64_t n_rows, int splits, int heads, int d) {
+    if (n_rows < 0 || splits < 1 || heads < 1 || d < 1) return TANGO_EINVAL;
+    if (d > kMaxHeadWidth || heads > 65535 || splits > 65535 || n_rows > 0x7fffffffLL) return TANGO_ESIZE;
+    return splits == 1 ? 0 : n_rows * splits * partial_floats(FORWARD, heads, heads * tango_rows8_pitch(d)) * 4;
+}
+
+extern "C" int tango_edge_attention_rows(const int32_t *indptr, const int32_t *indices, int64_t n_nodes, const int64_t *rows,
+                                         int64_t n_rows, int splits, int heads, int d, const void *q, int64_t ldq, int type,
+                                         const tango_rows8 *k, const tango_rows8 *v, float scale, void *out, void *ws,
+                                         int64_t ws_bytes, int mode, uint64_t seed, uint64_t call, const uint64_t *step,
+                                         tango_stream_t stream) {
+    const int rc = check_shape(n_rows, heads, d, type);
+    if (rc != TANGO_OK) return rc;
+    if (n_nodes < 0 || splits < 1 || mode < TANGO_ROUND_TRUNC || mode > TANGO_ROUND_STOCHASTIC) return TANGO_EINVAL;
+    if (splits > 65535) return TANGO_ESIZE;
+    if (n_rows == 0) return TANGO_OK;
+    if (!indptr || !indices || !rows || !q || !out || (n_rows > 1 && ldq < (int64_t)heads * d)) return TANGO_EINVAL;
+    if (n_nodes > 0 && (!good_codes(k, d) || !good_codes(v, d))) return TANGO_EINVAL;
+    if (splits > 1 && (!ws || ws_bytes < tango_edge_attention_rows_workspace_bytes(n_rows, splits, heads, d))) return TANGO_EINVAL;
+    if (!aligned(q, type == TANGO_FP32 ? 4 : 2) || !aligned(ws, 16)) return TANGO_EALIGN;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    RowsArgs a{};
+    a.indptr = indptr; a.indices = indices; a.rows = rows; a.n_nodes = n_nodes; a.q = q; a.ldq = ldq;
+    a.heads = heads; a.d = d; a.pitch = (int)tango_rows8_pitch(d); a.ld = (int64_t)heads * a.pitch;
+    if (n_nodes > 0) { a.k = k->q; a.sk = k->scales; a.v = v->q; a.sv = v->scales; }
+    a.qscale = scale * 1.4426950408889634f; a.splits = splits; a.out = out; a.type = type; a.ws = static_cast<float *>(ws);
+    a.mode = mode; a.seed = seed; a.call = call; a.step = reinterpret_cast<const unsigned long long *>(step);
+    const int done = with_shape(d, [&](auto vb, auto p) -> int {
+        constexpr int VB = decltype(vb)::value, P = decltype(p)::value;
+        a.hb = heads_of_a_block(heads, P);
+        const int64_t bz = ceil_div(heads, a.hb);
+        if (bz > 65535) return TANGO_ESIZE;
+        attn_rows_kernel<VB, P><<<dim3((unsigned)n_rows, (unsigned)splits, (unsigned)bz), kWarps * 32, 0, st>>>(a);
+        TANGO_LAUNCH_CHECK();
+        return TANGO_OK;
+    });
+    if (done != TANGO_OK || splits == 1) return done;
+    attn_rows_merge_kernel<<<(unsigned)n_rows, 256, 0, st>>>(a);
+    TANGO_LAUNCH_CHECK();
+    return TANGO_OK;
+}

@@ -1,0 +1,146 @@
+// Device side of the 8-bit rows: a matrix cut into groups of neighbouring columns, each with int8 codes and one fp32 scale.
+#pragma once
+#include "common.cuh"
+
+namespace tango {
+
+constexpr float kSmallestNormal = 1.1754943508222875e-38f;      // 2^-126
+constexpr float kRoundMagic = 12582912.f;                       // 1.5 * 2^23: adding it leaves round-to-even(t) in the low bits
+
+// Scale of a group from the bits of its largest magnitude.  Bits of magnitudes order like the magnitudes, infinity and NaN
+// above all numbers: a group that holds one gets the scale NaN, so that its values come back as NaN, not as something else.
+__device__ __forceinline__ float group_scale(uint32_t top) {
+    if (top >= 0x7f800000u) return __int_as_float(0x7fffffff);
+    const float s = __fdiv_rn(__uint_as_float(top), 127.0f);
+    return s < kSmallestNormal ? 0.f : s;
+}
+// About 1 / s; 0 for the scales 0 and NaN.
+__device__ __forceinline__ float group_inverse(float s) { return s > 0.f ? __fdividef(1.0f, s) : 0.f; }
+
+// Four codes: x / s exactly rounded, ties to even.  x * inv is within 127 * 2^-21 of the quotient, which decides all but the
+// values that close to a border between two codes.  For those x - q * s is exact in one fused operation (a multiple of half
+// an ulp of s, at most about s / 2), and its double is compared with s.
+__device__ __forceinline__ uint32_t encode4(const float (&x)[4], float s, float inv) {
+    float b[4], far = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float t = __fmul_rn(x[i], inv);
+        b[i] = __fadd_rn(t, kRoundMagic);
+        far = fmaxf(far, fabsf(__fsub_rn(t, __fsub_rn(b[i], kRoundMagic))));
+    }
+    if (far > 0.4999f) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float q = __fsub_rn(b[i], kRoundMagic);
+            const float r = fmaf(-q, s, x[i]), twice = 2.f * fabsf(r);
+            if (twice > s || (twice == s && (__float_as_int(b[i]) & 1))) b[i] = __fadd_rn(b[i], r > 0.f ? 1.f : -1.f);
+        }
+    }
+    const uint32_t lo = __byte_perm(__float_as_uint(b[0]), __float_as_uint(b[1]), 0x0040);
+    const uint32_t hi = __byte_perm(__float_as_uint(b[2]), __float_as_uint(b[3]), 0x0040);
+    return inv == 0.f ? 0u : __byte_perm(lo, hi, 0x5410);
+}
+
+// The other rounding modes: truncation, and the seeded stochastic stream keyed by the element's flat index.
+static __device__ __noinline__ uint32_t encode4_mode(const float (&x)[4], float s, int mode, uint64_t seed, uint64_t call, uint64_t flat) {
+    if (!(s > 0.f)) return 0u;
+    const Philox ph{(uint32_t)seed, (uint32_t)(seed >> 32)};
+    uint64_t blk = ~0ull;
+    uint4 rnd = make_uint4(0, 0, 0, 0);
+    uint32_t word = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float u = mode == TANGO_ROUND_STOCHASTIC ? sr_uniform(ph, flat + i, call, blk, rnd) : 0.f;
+        word |= (uint32_t)(uint8_t)round_to_i8(__fdiv_rn(x[i], s), mode, u) << (8 * i);
+    }
+    return word;
+}
+
+// The four codes of a word as floats: the biased code lands in the mantissa of 2^23, exactly.
+__device__ __forceinline__ void decode4(uint32_t word, float (&v)[4]) {
+    const uint32_t w = word ^ 0x80808080u;
+    v[0] = __fsub_rn(__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7440)), 8388736.f);
+    v[1] = __fsub_rn(__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7441)), 8388736.f);
+    v[2] = __fsub_rn(__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7442)), 8388736.f);
+    v[3] = __fsub_rn(__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7443)), 8388736.f);
+}
+
+// Quotients of indices below 2^31 by a fixed divisor: floor(i * m / 2^(32 + shift)), with m rounded up.
+struct FastDiv {
+    uint32_t d, m, shift;
+};
+inline FastDiv fast_div(int64_t d) {
+    FastDiv f{(uint32_t)d, 0, 0};
+    if (d <= 1) return f;
+    while ((1ull << (f.shift + 1)) < (uint64_t)d) ++f.shift;            // 2^shift < d <= 2^(shift + 1)
+    f.m = (uint32_t)(((1ull << (32 + f.shift)) + (uint64_t)d - 1) / (uint64_t)d);
+    return f;
+}
+__device__ __forceinline__ uint32_t quotient(uint32_t i, const FastDiv &f) { return f.d <= 1 ? i : __umulhi(i, f.m) >> f.shift; }
+
+// Element types of the matrices: TANGO_FP32, TANGO_BF16, TANGO_FP16.  bf16 and fp16 results are rounded once, to nearest.
+struct Bf16 { uint16_t bits; };
+struct Fp16 { uint16_t bits; };
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(Bf16 v) { return __uint_as_float((uint32_t)v.bits << 16); }
+__device__ __forceinline__ float to_float(Fp16 v) {
+    float f;
+    asm("cvt.f32.f16 %0, %1;" : "=f"(f) : "h"(v.bits));
+    return f;
+}
+__device__ __forceinline__ void from_float(float v, float &o) { o = v; }
+__device__ __forceinline__ void from_float(float v, Bf16 &o) { asm("cvt.rn.bf16.f32 %0, %1;" : "=h"(o.bits) : "f"(v)); }
+__device__ __forceinline__ void from_float(float v, Fp16 &o) { asm("cvt.rn.f16.f32 %0, %1;" : "=h"(o.bits) : "f"(v)); }
+
+// VL elements at once, p aligned to them.
+template <int BYTES> struct Word;
+template <> struct Word<2> { typedef uint16_t T; };
+template <> struct Word<4> { typedef uint32_t T; };
+template <> struct Word<8> { typedef uint2 T; };
+template <> struct Word<16> { typedef uint4 T; };
+template <class T, int VL> union Pack {
+    T e[VL];
+    typename Word<VL * sizeof(T)>::T w;
+    __device__ Pack() {}
+};
+// Four neighbouring elements, of which the first n exist (the others read as 0).
+template <class T, int VL>
+__device__ __forceinline__ void load4(const T *p, int n, float (&v)[4]) {
+    if (n >= 4) {
+#pragma unroll
+        for (int i = 0; i < 4; i += VL) {
+            Pack<T, VL> k;
+            k.w = __ldg(reinterpret_cast<const typename Word<VL * sizeof(T)>::T *>(p + i));
+#pragma unroll
+            for (int j = 0; j < VL; ++j) v[i + j] = to_float(k.e[j]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[i] = 0.f;
+            if (i < n) {
+                Pack<T, 1> k;
+                k.w = __ldg(reinterpret_cast<const typename Word<sizeof(T)>::T *>(p + i));
+                v[i] = to_float(k.e[0]);
+            }
+        }
+    }
+}
+template <class T, int VL>
+__device__ __forceinline__ void store4(T *p, int n, const float (&v)[4]) {
+    if (n >= 4) {
+#pragma unroll
+        for (int i = 0; i < 4; i += VL) {
+            Pack<T, VL> k;
+#pragma unroll
+            for (int j = 0; j < VL; ++j) from_float(v[i + j], k.e[j]);
+            *reinterpret_cast<typename Word<VL * sizeof(T)>::T *>(p + i) = k.w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i < n) from_float(v[i], p[i]);
+    }
+}
+
+}  // namespace tango

@@ -2,6 +2,7 @@
 #include <torch/csrc/utils/pybind.h>
 
 #include "torch_autograd.h"
+#include "torch_rows8.h"
 
 namespace py = pybind11;
 using namespace tango_host;
@@ -15,6 +16,8 @@ static Schedule schedule(const py::object &s, bool with_hub) {
     out.present = true;
     out.units = tensor_attr(s, "units");
     out.heavy_rows = tensor_attr(s, "heavy_rows");
+    out.heavy_first = tensor_attr(s, "heavy_first");
+    out.longest = s.attr("longest").cast<int64_t>();
     out.row_order = tensor_attr(s, "row_order");
     if (const py::object info = s.attr("row_info"); !info.is_none()) out.row_info = info.cast<Tensor>();
     out.n_over_few = s.attr("n_over_few").cast<int64_t>();
@@ -127,5 +130,19 @@ PYBIND11_MODULE(_torch_ops, m) {
     m.def("gat_layer", [](const GraphPtr &g, const Tensor &ft, const Tensor &al, const Tensor &ar, const py::object &bias,
                           double slope, bool int8_weights) {
         return gat_layer_fn(g, ft, al, ar, optional(bias), slope, int8_weights);
+    });
+
+    m.def("pack8", [](const Tensor &x, int64_t group) {
+        const Rows8 r = pack8(x, group);
+        return py::make_tuple(r.q, r.scale);
+    });
+    m.def("unpack8", [](const Tensor &q, const Tensor &scale, const std::vector<int64_t> &sizes, int64_t group, const Tensor &like) {
+        return unpack8({q, scale}, sizes, group, like.scalar_type());
+    });
+    m.def("activation8", &activation8_fn);
+    m.def("edge_attention", &edge_attention_fn);
+    m.def("edge_attention_rows", [](const GraphPtr &g, const Tensor &rows, const Tensor &q, const Tensor &kq, const Tensor &ks,
+                                    const Tensor &vq, const Tensor &vs, double scale) {
+        return edge_attention_rows(g, rows, q, {kq, ks}, {vq, vs}, scale);
     });
 }

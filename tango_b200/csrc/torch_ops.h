@@ -47,8 +47,8 @@ inline void count(int64_t n) { settings().launches.fetch_add(n, std::memory_orde
 
 // The row schedule of one index bundle (tango_b200.graph.SpmmSchedule) and its dense hub region, if any.
 struct Schedule {
-    Tensor units, heavy_rows, row_order, row_info;
-    int64_t n_units = 0, n_heavy = 0, n_long = 0, n_block_rows = 0, n_skip = 0, n_over_few = 0, n_over_one = 0;
+    Tensor units, heavy_rows, heavy_first, row_order, row_info;
+    int64_t longest = 0, n_units = 0, n_heavy = 0, n_long = 0, n_block_rows = 0, n_skip = 0, n_over_few = 0, n_over_one = 0;
     int threshold = 0, unit = 0;
     bool present = false;
     // hub region (tango_b200.graph.HubBlock)

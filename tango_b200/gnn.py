@@ -15,6 +15,8 @@ from . import _native
 from .QLinear import QLinear, Qlinear_func, Qlinear_func_reduce, linear_group
 from .SDDMM import sddmm_u_add_v, sddmm_u_dot_v
 from .SPMM import spmm_copy_u, spmm_u_mul_e
+from .attention import edge_attention, edge_attention_rows
+from .rows8 import in_8_bits, pack8
 
 
 def _norm(deg: torch.Tensor, both: bool) -> torch.Tensor:
@@ -251,11 +253,16 @@ class QGATConv(nn.Module):
 
 
 class GAT(nn.Module):
-    """evaluation/test_gat.py:172-224."""
+    """evaluation/test_gat.py:172-224.  checkpoint="int8": the activations between the layers keep their input in 8 bits for the
+    backward pass instead of in fp32 (`rows8.activation8`); the outputs are the same."""
 
     def __init__(self, g, num_layers, in_dim, num_hidden, num_classes, heads, activation=F.elu, feat_drop=0.0,
-                 attn_drop=0.0, negative_slope=0.2, residual=False, fused=True):
+                 attn_drop=0.0, negative_slope=0.2, residual=False, fused=True, checkpoint=None):
         super().__init__()
+        if checkpoint not in (None, "int8"):
+            raise ValueError(f'checkpoint={checkpoint!r}: None or "int8"')
+        if checkpoint == "int8" and activation is not None:
+            activation = in_8_bits(activation)
         self.g, self.num_layers = g, num_layers
         self.gat_layers = nn.ModuleList()
         if num_layers > 1:
@@ -281,10 +288,15 @@ class GAT(nn.Module):
 class HGT(nn.Module):
     """Single-relation heterogeneous-graph-transformer layer of evaluation/test_HGT.py:27-67: six QLinear
     projections, int8 per-head dot-product scores (sddmm_u_dot_v), 1/sqrt(d_k), edge softmax over each destination's
-    incoming edges (fp32, as in the reference), int8 attention-weighted aggregation (spmm_u_mul_e)."""
+    incoming edges (fp32, as in the reference), int8 attention-weighted aggregation (spmm_u_mul_e).
 
-    def __init__(self, in_dim, out_dim, n_heads, dropout=0.2, use_norm=False):
+    fused=True: the three in one (`attention.edge_attention`): no per-edge tensors, the probabilities stay in fp32, and q, k
+    and v have a scale per node and head instead of one per tensor.  `keys_values` and `forward_rows` serve such a layer to a
+    few nodes at a time."""
+
+    def __init__(self, in_dim, out_dim, n_heads, dropout=0.2, use_norm=False, fused=False):
         super().__init__()
+        self._fused = fused
         assert out_dim % n_heads == 0, "out_dim must be a multiple of n_heads"
         self.in_dim, self.out_dim, self.n_heads = in_dim, out_dim, n_heads
         self.d_k = out_dim // n_heads
@@ -302,10 +314,26 @@ class HGT(nn.Module):
         k = self.attn_linear(next(shared)).view(-1, self.n_heads, self.d_k)
         v = self.msg_linear(next(shared)).view(-1, self.n_heads, self.d_k)
         q = next(shared).view(-1, self.n_heads, self.d_k)
+        if self._fused:
+            return self.a_linear(edge_attention(g, q, k, v, 1.0 / self.sqrt_dk).view(-1, self.out_dim))
         t = sddmm_u_dot_v.apply(g, k, q)
         attn, s_attn = edge_softmax(g, t, 1.0 / self.sqrt_dk, True)   # the reference divides t by sqrt(d_k) first
         out = spmm_u_mul_e.apply(g, v, attn, s_attn).view(-1, self.out_dim)
         return self.a_linear(out)
+
+    @torch.no_grad()
+    def keys_values(self, h):
+        """Keys and values of all nodes in 8 bits, for `forward_rows`."""
+        k = self.attn_linear(self.k_linear(h)).view(-1, self.n_heads, self.d_k)
+        v = self.msg_linear(self.v_linear(h)).view(-1, self.n_heads, self.d_k)
+        return pack8(k, self.d_k), pack8(v, self.d_k)
+
+    @torch.no_grad()
+    def forward_rows(self, g, rows, h_rows, k8, v8):
+        """The layer's output for the nodes `rows` alone, from their features h_rows and what `keys_values` gave.  As `forward`
+        with fused=True, except that the projections of h_rows find their int8 scales in these rows alone."""
+        q = self.q_linear(h_rows).view(-1, self.n_heads, self.d_k)
+        return self.a_linear(edge_attention_rows(g, rows, q, k8, v8, 1.0 / self.sqrt_dk).view(-1, self.out_dim))
 
 
 # ---------------------------------------------------------------------------------------------------- link prediction

@@ -257,9 +257,11 @@ class SpmmSchedule:
 
     force_heavy (optional, nseg == 1): row ids that are finished through the int32 scratch whatever their length (the
     rows of a dense hub block, in the block's row order); they come first in `heavy_rows`, every heavy row comes
-    first in `row_order`, and `n_skip` = n_heavy tells the row kernels to start after them."""
+    first in `row_order`, and `n_skip` = n_heavy tells the row kernels to start after them.
 
-    LAYOUT = 3      # counts up when the fields or their meaning change: see Graph.__setstate__
+    `heavy_first` [n_heavy * nseg + 1]: the first unit of every heavy segment row; `longest`: slots of the longest row."""
+
+    LAYOUT = 4      # counts up when the fields or their meaning change: see Graph.__setstate__
 
     def __init__(self, indptr: torch.Tensor, nseg: int = 1, threshold: Optional[int] = None,
                  unit: Optional[int] = None, force_heavy: Optional[torch.Tensor] = None):
@@ -315,10 +317,12 @@ class SpmmSchedule:
         # Rows that deserve a whole CTA in row-team kernels.  The line is the same for every graph: the order in which a row's
         # softmax terms are added depends on it.
         self.n_block_rows = int((row_deg > BLOCK_ROW_NNZ).sum())
+        self.longest = int(row_deg.max()) if n_rows else 0
         self.n_heavy = int(heavy.numel())
         self.heavy_rows = heavy.to(torch.int32)
         if self.n_heavy == 0:
             self.units = torch.zeros((0, 4), dtype=torch.int32, device=indptr.device)
+            self.heavy_first = torch.zeros(1, dtype=torch.int32, device=indptr.device)
             self.n_units = 0
             return
         # segment rows of the heavy rows, their scratch slots, and the slices of each
@@ -327,7 +331,9 @@ class SpmmSchedule:
         beg, end = ip[seg_rows], ip[seg_rows + 1]
         n_chunks = (end - beg + unit - 1) // unit
         rep = torch.repeat_interleave(torch.arange(seg_rows.numel(), device=indptr.device), n_chunks)
-        first = torch.cumsum(n_chunks, 0) - n_chunks
+        last = torch.cumsum(n_chunks, 0)
+        first = last - n_chunks
+        self.heavy_first = torch.cat([first[:1], last]).to(torch.int32)
         k = torch.arange(rep.numel(), device=indptr.device) - first[rep]
         ub = beg[rep] + k * unit
         ue = torch.minimum(ub + unit, end[rep])
