@@ -460,8 +460,12 @@ int tango_peer_sync(uint64_t *const *slots /* device */, int rank, int world, ui
 
 int64_t tango_rows8_pitch(int64_t group);
 int64_t tango_rows8_ld(int64_t cols, int64_t group);
+int64_t tango_rows8_run(int64_t group);      /* 16, 8 or 4: what pitches and leading dimensions are multiples of */
 
-/* An 8-bit matrix, and one to be made from x (leading dimension ldx, elements).  Host structs, read before the call returns. */
+/* An 8-bit matrix, and one to be made from x (leading dimension ldx, elements).  Host structs, read before the call returns.
+ * The scale of group i is written to scales[i * scale_stride].  interleaved: this is one of two matrices of which every run of
+ * tango_rows8_run(group) codes of the first is followed by the run of the second (rows and groups then lie twice as far apart;
+ * q of the second is one run behind that of the first).  What reads 8-bit matrices reads plain ones unless it says otherwise. */
 typedef struct tango_rows8 {
     const int8_t *q;
     const float *scales;
@@ -471,6 +475,8 @@ typedef struct tango_rows8_job {
     int64_t ldx;
     int8_t *q;
     float *scales;
+    int64_t scale_stride;
+    int interleaved;
 } tango_rows8_job;
 
 /* Up to four matrices of one shape and type in one launch; job j draws its random numbers with call + j.  Replaces what
@@ -491,36 +497,41 @@ int tango_act8_backward(int act, const int8_t *q, const float *scales, int64_t r
 /* ---------------------------------------------------------------- edge attention on 8-bit rows
  * q, k, v and the incoming gradient o are 8-bit matrices [nodes, heads * d] with groups of d (a scale per node and head).
  *   z = scale * <q[v], k[u]>,  p = softmax of z over the edges u -> v of row v,  out[v] = sum p v[u]      (no edges: 0)
- * Row schedule (host struct; NULL: every row by one warp): rows [0, n_heavy) of row_order are cut into the units
- * (row, first slot, end slot, unused), those of heavy_rows[i] being units heavy_first[i] .. heavy_first[i + 1]; rows up to
- * n_long_rows get a warp, the rest a part of one.  Units need a workspace, 16-byte aligned, of
- * tango_edge_attention_workspace_bytes (pass 0 forward, 1 bwd_dst, 2 bwd_src).  d <= 512.  Rows in one order of sums each.
+ * Row schedule (host struct; NULL: every row by one warp): `rows` = (row, first slot, end slot, unused) of every row; the first
+ * n_heavy of them are cut into the units (row, first slot, end slot, place in the row), those of the i-th being units
+ * heavy_first[i] .. heavy_first[i + 1]; rows up to n_long get a warp, the rest a part of one.  `rows` and `units` 16-byte aligned.
+ * Units need a workspace, 16-byte aligned, of tango_edge_attention_workspace_bytes (pass 0 forward, 1 bwd_dst, 2 bwd_src).
+ * d <= 512.  Every sum has one order, which depends on the row's length and the schedule.
  * Replaces sddmm_u_dot_v -> edge_softmax -> spmm_u_mul_e (evaluation/test_HGT.py:58-62) and their backward passes. */
 typedef struct tango_edge_plan {
-    const int32_t *row_order;
-    int64_t n_long_rows;
+    const int32_t *rows;
+    int64_t n_long;
     const int32_t *units;
     int64_t n_units;
-    const int32_t *heavy_rows;
     const int32_t *heavy_first;
     int64_t n_heavy;
 } tango_edge_plan;
+/* Codes of q and o, those of k and v interleaved, 32-byte aligned; scales of q and o, those of k and v in pairs [nodes, heads, 2];
+ * o and so in the backward pass alone. */
+typedef struct tango_edge_operands {
+    const int8_t *q, *kv, *o;
+    const float *sq, *skv, *so;
+} tango_edge_operands;
 int64_t tango_edge_attention_workspace_bytes(int pass, int64_t n_units, int heads, int d);
 
 /* CSC in, out [rows, heads, d] contiguous of `type`; stats (optional) [rows, heads, 2] fp32: largest z * log2(e), 1 / sum. */
 int tango_edge_attention(const int32_t *indptr, const int32_t *indices, int64_t n_rows, const tango_edge_plan *plan, int heads, int d,
-                         const tango_rows8 *q, const tango_rows8 *k, const tango_rows8 *v, float scale, void *out, int type,
-                         float *stats, void *ws, int64_t ws_bytes, tango_stream_t stream);
-/* Gradients, the probabilities computed anew from stats.  bwd_dst walks the CSC and writes dq and record [rows, heads, 4] fp32
- * (what bwd_src reads of a destination); bwd_src walks the CSR behind it and writes dk and dv. */
+                         const tango_edge_operands *x, float scale, void *out, int type, float *stats, void *ws, int64_t ws_bytes,
+                         tango_stream_t stream);
+/* Gradients, the probabilities computed anew from stats.  bwd_dst walks the CSC and writes dq and, for bwd_src, record
+ * [rows, heads, 4] fp32 and qo, the codes of q and o interleaved (both or neither NULL); bwd_src walks the CSR behind it and
+ * writes dk and dv. */
 int tango_edge_attention_bwd_dst(const int32_t *indptr, const int32_t *indices, int64_t n_rows, const tango_edge_plan *plan, int heads,
-                                 int d, const tango_rows8 *q, const tango_rows8 *k, const tango_rows8 *v, const tango_rows8 *grad,
-                                 float scale, const float *stats, void *dq, int type, float *record, void *ws, int64_t ws_bytes,
-                                 tango_stream_t stream);
+                                 int d, const tango_edge_operands *x, float scale, const float *stats, void *dq, int type,
+                                 float *record, int8_t *qo, void *ws, int64_t ws_bytes, tango_stream_t stream);
 int tango_edge_attention_bwd_src(const int32_t *indptr, const int32_t *indices, int64_t n_rows, const tango_edge_plan *plan, int heads,
-                                 int d, const tango_rows8 *q, const tango_rows8 *k, const tango_rows8 *v, const tango_rows8 *grad,
-                                 const float *record, void *dk, void *dv, int type, void *ws, int64_t ws_bytes,
-                                 tango_stream_t stream);
+                                 int d, const int8_t *kv, const float *skv, const int8_t *qo, const float *record, void *dk, void *dv,
+                                 int type, void *ws, int64_t ws_bytes, tango_stream_t stream);
 
 /* The same attention of n_rows nodes `rows` (int64, any order, repeats allowed; an id outside [0, n_nodes) gives a row of NaN)
  * whose queries q [n_rows, heads, d] just arrived in `type` (leading dimension ldq, elements), over keys and values kept as

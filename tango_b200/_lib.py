@@ -130,14 +130,15 @@ _SIGS = {
     "tango_edge_softmax_bwd": ([P, P, P, c_int64, c_int64, c_int, c_float, P, P, P, P, P], c_int),
     "tango_rows8_pitch": ([c_int64], c_int64),
     "tango_rows8_ld": ([c_int64, c_int64], c_int64),
+    "tango_rows8_run": ([c_int64], c_int64),
     "tango_rows8_pack": ([P, c_int, c_int64, c_int64, c_int64, c_int, c_int, c_uint64, c_uint64, P, P], c_int),
     "tango_rows8_unpack": ([P, P, c_int64, c_int64, c_int64, c_int, P, c_int64, P], c_int),
     "tango_act8_forward": ([c_int, P, c_int64, c_int64, c_int64, c_int, P, c_int64, c_int, c_uint64, c_uint64, P, P], c_int),
     "tango_act8_backward": ([c_int, P, P, c_int64, c_int64, c_int64, c_int, P, c_int64, P, c_int64, P], c_int),
     "tango_edge_attention_workspace_bytes": ([c_int, c_int64, c_int, c_int], c_int64),
-    "tango_edge_attention": ([P, P, c_int64, P, c_int, c_int, P, P, P, c_float, P, c_int, P, P, c_int64, P], c_int),
-    "tango_edge_attention_bwd_dst": ([P, P, c_int64, P, c_int, c_int, P, P, P, P, c_float, P, P, c_int, P, P, c_int64, P], c_int),
-    "tango_edge_attention_bwd_src": ([P, P, c_int64, P, c_int, c_int, P, P, P, P, P, P, P, c_int, P, c_int64, P], c_int),
+    "tango_edge_attention": ([P, P, c_int64, P, c_int, c_int, P, c_float, P, c_int, P, P, c_int64, P], c_int),
+    "tango_edge_attention_bwd_dst": ([P, P, c_int64, P, c_int, c_int, P, c_float, P, P, c_int, P, P, P, c_int64, P], c_int),
+    "tango_edge_attention_bwd_src": ([P, P, c_int64, P, c_int, c_int, P, P, P, P, P, P, c_int, P, c_int64, P], c_int),
     "tango_edge_attention_rows_splits": ([c_int64, c_int64], c_int),
     "tango_edge_attention_rows_workspace_bytes": ([c_int64, c_int, c_int, c_int], c_int64),
     "tango_edge_attention_rows": ([P, P, c_int64, P, c_int64, c_int, c_int, c_int, P, c_int64, c_int, P, P, c_float, P, P, c_int64,

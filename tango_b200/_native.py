@@ -153,3 +153,12 @@ def graph(g):
     except AttributeError:       # an object without room for it: rebuilt on every call
         pass
     return handle
+
+
+def edge_graph(g):
+    """The same with the row schedules of the edge-attention kernels, made at the first call."""
+    handle = graph(g)
+    if not handle.has_edge_schedules():
+        from .graph import EdgeSchedule
+        handle.set_edge_schedules(EdgeSchedule(g.adj_csc[0]), EdgeSchedule(g.adj_csr[0]))
+    return handle

@@ -22,16 +22,18 @@
 namespace tango {
 
 enum { FORWARD = 0, BY_DST = 1, BY_SRC = 2 };
-constexpr int kWarps = 8;
+constexpr int kWarps = 4, kRowWarps = 8;
 
 struct AttnArgs {
-    const int32_t *indptr, *indices, *row_order;
-    const int4 *units;
+    const int32_t *indptr, *indices;
+    const int4 *rows, *units;                       // (row, first slot, end slot, place of a unit in its row)
     int64_t n_units, n_heavy, n_long, n_rows;       // rows: [heavy: by units] [to n_long: a warp] [the rest: a team]
     int heads, d, pitch, hb, team;                  // hb: heads of a block (a power of two); team: lanes of a short row
-    int64_t ld;                                     // bytes of a row of codes
-    const int8_t *fixed_a, *fixed_b, *gather_a, *gather_b;
-    const float *fixed_sa, *fixed_sb, *gather_sa, *gather_sb;
+    int ld;                                         // bytes of a row of codes
+    const int8_t *q, *o, *kv;                       // kv and qo: runs of VB codes of the one and of the other in turn
+    int8_t *qo;
+    const float *sq, *so;                           // scales [rows, heads]
+    const float2 *skv;                              // scales of k and v [rows, heads]
     float qscale;                                   // scale * log2(e)
     float2 *stats;                                  // [rows, heads]: maximum of z * log2(e), 1 / sum
     float4 *record;                                 // [rows, heads], BY_DST writes and BY_SRC gathers: see there
@@ -47,53 +49,55 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return y;
 }
 
-// Two floats that one instruction works on.
-struct Pair { uint64_t v; };
-__device__ __forceinline__ Pair pair(float a, float b) {
-    Pair p;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(p.v) : "f"(a), "f"(b));
-    return p;
-}
-__device__ __forceinline__ float2 both(Pair p) {
-    float2 f;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p.v));
-    return f;
-}
-__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
-    Pair o;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(o.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-    return o;
-}
-__device__ __forceinline__ Pair add2(Pair a, Pair b) {
-    Pair o;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(o.v) : "l"(a.v), "l"(b.v));
-    return o;
-}
-__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
-    Pair o;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(o.v) : "l"(a.v), "l"(b.v));
-    return o;
-}
 __device__ __forceinline__ Pair shuffle2(Pair a, int lanes) { return {__shfl_xor_sync(0xffffffffu, a.v, lanes)}; }
 
 // VB codes.
 template <int VB> struct Codes { uint32_t w[VB / 4]; };
 template <int VB>
-__device__ __forceinline__ Codes<VB> load_codes(const int8_t *p, bool there) {
+__device__ __forceinline__ Codes<VB> load_codes(const int8_t *p) {
+    Codes<VB> c;
+    if constexpr (VB == 16) {
+        const uint4 t = __ldg(reinterpret_cast<const uint4 *>(p));
+        c.w[0] = t.x; c.w[1] = t.y; c.w[2] = t.z; c.w[3] = t.w;
+    } else if constexpr (VB == 8) {
+        const uint2 t = __ldg(reinterpret_cast<const uint2 *>(p));
+        c.w[0] = t.x; c.w[1] = t.y;
+    } else {
+        c.w[0] = __ldg(reinterpret_cast<const uint32_t *>(p));
+    }
+    return c;
+}
+// A run of one matrix and the run of the other behind it, in one access.
+template <int VB>
+__device__ __forceinline__ void load_runs(const int8_t *p, Codes<VB> &a, Codes<VB> &b) {
+    if constexpr (VB == 16) {
+        asm("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+            : "=r"(a.w[0]), "=r"(a.w[1]), "=r"(a.w[2]), "=r"(a.w[3]), "=r"(b.w[0]), "=r"(b.w[1]), "=r"(b.w[2]), "=r"(b.w[3]) : "l"(p));
+    } else if constexpr (VB == 8) {
+        const uint4 t = __ldg(reinterpret_cast<const uint4 *>(p));
+        a.w[0] = t.x; a.w[1] = t.y; b.w[0] = t.z; b.w[1] = t.w;
+    } else {
+        const uint2 t = __ldg(reinterpret_cast<const uint2 *>(p));
+        a.w[0] = t.x; b.w[0] = t.y;
+    }
+}
+template <int VB>
+__device__ __forceinline__ void store_runs(int8_t *p, const Codes<VB> &a, const Codes<VB> &b) {
+    if constexpr (VB == 16) {
+        const uint32_t w[8] = {a.w[0], a.w[1], a.w[2], a.w[3], b.w[0], b.w[1], b.w[2], b.w[3]};
+        store_v8(reinterpret_cast<float *>(p), w);
+    } else if constexpr (VB == 8) {
+        *reinterpret_cast<uint4 *>(p) = make_uint4(a.w[0], a.w[1], b.w[0], b.w[1]);
+    } else {
+        *reinterpret_cast<uint2 *>(p) = make_uint2(a.w[0], b.w[0]);
+    }
+}
+template <int VB>
+__device__ __forceinline__ Codes<VB> codes_if(bool there, const int8_t *p) {
+    if (there) return load_codes<VB>(p);
     Codes<VB> c;
 #pragma unroll
     for (int i = 0; i < VB / 4; ++i) c.w[i] = 0;
-    if (there) {
-        if constexpr (VB == 16) {
-            const uint4 t = __ldg(reinterpret_cast<const uint4 *>(p));
-            c.w[0] = t.x; c.w[1] = t.y; c.w[2] = t.z; c.w[3] = t.w;
-        } else if constexpr (VB == 8) {
-            const uint2 t = __ldg(reinterpret_cast<const uint2 *>(p));
-            c.w[0] = t.x; c.w[1] = t.y;
-        } else {
-            c.w[0] = __ldg(reinterpret_cast<const uint32_t *>(p));
-        }
-    }
     return c;
 }
 // Exact product of two heads, the same number in all their P lanes.
@@ -111,25 +115,21 @@ __device__ __forceinline__ float dot(const Codes<VB> &a, const Codes<VB> &b) {
 // acc += by * codes
 template <int VB>
 __device__ __forceinline__ void add_codes(Pair (&acc)[VB / 2], const Codes<VB> &c, Pair by) {
-    const Pair bias = pair(-8388736.f, -8388736.f);
 #pragma unroll
     for (int i = 0; i < VB / 4; ++i) {
-        const uint32_t w = c.w[i] ^ 0x80808080u;
-        const Pair lo = pair(__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7440)), __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7441)));
-        const Pair hi = pair(__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7442)), __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7443)));
-        acc[2 * i] = fma2(add2(lo, bias), by, acc[2 * i]);
-        acc[2 * i + 1] = fma2(add2(hi, bias), by, acc[2 * i + 1]);
+        Pair lo, hi;
+        decode4(c.w[i], lo, hi);
+        acc[2 * i] = fma2(lo, by, acc[2 * i]);
+        acc[2 * i + 1] = fma2(hi, by, acc[2 * i + 1]);
     }
 }
 // accA += a * codes, accB += b * codes
 template <int VB>
 __device__ __forceinline__ void add_codes_twice(Pair (&accA)[VB / 2], Pair (&accB)[VB / 2], const Codes<VB> &c, Pair a, Pair b) {
-    const Pair bias = pair(-8388736.f, -8388736.f);
 #pragma unroll
     for (int i = 0; i < VB / 4; ++i) {
-        const uint32_t w = c.w[i] ^ 0x80808080u;
-        const Pair lo = add2(pair(__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7440)), __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7441))), bias);
-        const Pair hi = add2(pair(__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7442)), __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7443))), bias);
+        Pair lo, hi;
+        decode4(c.w[i], lo, hi);
         accA[2 * i] = fma2(lo, a, accA[2 * i]);
         accA[2 * i + 1] = fma2(hi, a, accA[2 * i + 1]);
         accB[2 * i] = fma2(lo, b, accB[2 * i]);
@@ -170,9 +170,11 @@ __host__ __device__ inline int64_t partial_floats(int mode, int heads, int64_t l
     return (partial_heads(mode) * heads + 3) / 4 * 4 + partial_sums(mode) * ld;
 }
 
-// A softmax that is being added up: running maximum (of z * log2 e), sum, weighted sums of codes.
+// A softmax that is being added up: running maximum (of z * log2 e), sum, weighted sums of codes.  Before the first edge the
+// maximum is a number below all scores, so that nothing here has to ask for it.
+constexpr float kBelow = -3.0e38f;
 template <int VB> struct Running {
-    float m = -INFINITY, l = 0.f;
+    float m = kBelow, l = 0.f;
     Pair acc[VB / 2];
     __device__ Running() {
 #pragma unroll
@@ -188,7 +190,7 @@ template <int VB> struct Running {
     __device__ __forceinline__ void merge(int lanes) {
         const float mo = __shfl_xor_sync(0xffffffffu, m, lanes), lo = __shfl_xor_sync(0xffffffffu, l, lanes);
         const float top = fmaxf(m, mo);
-        const float c = m == -INFINITY ? 0.f : exp2_fast(m - top), co = mo == -INFINITY ? 0.f : exp2_fast(mo - top);
+        const float c = exp2_fast(m - top), co = exp2_fast(mo - top);
         const Pair cc = pair(c, c), cco = pair(co, co);
         m = top;
         l = fmaf(l, c, lo * co);
@@ -197,39 +199,40 @@ template <int VB> struct Running {
     }
 };
 
-// One step of the forward pass: U edges of a lane.  z = -inf marks an edge that is not there.
+// One step of the forward pass: U edges of a lane; an edge that is not there has z = -inf and so no weight.
 template <int VB, int U>
 __device__ __forceinline__ void softmax_step(Running<VB> &r, const float (&z)[U], const float (&sv)[U], const Codes<VB> (&v)[U]) {
     float top = r.m;
 #pragma unroll
     for (int u = 0; u < U; ++u) top = fmaxf(top, z[u]);
     if (__any_sync(0xffffffffu, top > r.m)) {       // seldom after the first edges of a row
-        r.scale(r.m == -INFINITY ? 0.f : exp2_fast(r.m - top));
+        r.scale(exp2_fast(r.m - top));
         r.m = top;
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        const float p = z[u] == -INFINITY ? 0.f : exp2_fast(z[u] - r.m);
+        const float p = exp2_fast(z[u] - r.m);
         r.l += p;
         const float w = p * sv[u];
         add_codes<VB>(r.acc, v[u], pair(w, w));
     }
 }
 
-template <int MODE> struct InFlight { static constexpr int U = MODE == FORWARD ? 4 : 2; };
+template <int MODE> struct InFlight { static constexpr int U = 2; };
 
 template <int MODE, int VB, int P>
-__global__ void __launch_bounds__(kWarps * 32) attn_kernel(const __grid_constant__ AttnArgs a) {
+__global__ void __launch_bounds__(kWarps * 32, MODE == FORWARD ? 6 : 4) attn_kernel(const __grid_constant__ AttnArgs a) {
     constexpr int U = InFlight<MODE>::U;
     const int lane = threadIdx.x & 31;
     // ---- what this warp works on
-    int64_t w = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
+    const int64_t w = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
     int row = -1, beg = 0, end = 0, team = 32;
     int64_t unit = -1;
+    int place = 0;
     if (w < a.n_units) {
         unit = w;
         const int4 t = __ldg(a.units + w);
-        row = t.x; beg = t.y; end = t.z;
+        row = t.x; beg = t.y; end = t.z; place = t.w;
     } else {
         int64_t at = w - a.n_units + a.n_heavy;
         if (at >= a.n_long) {
@@ -237,33 +240,52 @@ __global__ void __launch_bounds__(kWarps * 32) attn_kernel(const __grid_constant
             at = a.n_long + (at - a.n_long) * (32 / team) + lane / team;
         }
         if (at < a.n_rows) {
-            row = a.row_order ? __ldg(a.row_order + at) : (int)at;
-            beg = __ldg(a.indptr + row);
-            end = __ldg(a.indptr + row + 1);
+            if (a.rows) {
+                const int4 t = __ldg(a.rows + at);
+                row = t.x; beg = t.y; end = t.z;
+            } else {
+                row = (int)at; beg = __ldg(a.indptr + at); end = __ldg(a.indptr + at + 1);
+            }
         }
     }
     const int L = a.hb * P, slots = team / L;
     const int slot = (lane & (team - 1)) / L, in_edge = lane & (L - 1);
     const int head = blockIdx.y * a.hb + in_edge / P, chunk = in_edge & (P - 1);
-    const bool has_head = head < a.heads, live = has_head && chunk * VB < a.pitch;
-    const int64_t off = (int64_t)head * a.pitch + chunk * VB;
+    const bool live = head < a.heads && chunk * VB < a.pitch;
+    // Lanes without a place in the row read along with one that has (their own operand is 0, their results go nowhere), and
+    // slots behind the row's end read its last edge once more without weight: no load and no register waits for a condition.
+    const int hd = head < a.heads ? head : a.heads - 1, off = live ? head * a.pitch + chunk * VB : hd * a.pitch;
 
     // ---- the row's own operands
     const bool mine = row >= 0 && live;
-    const int64_t rh = (int64_t)row * a.heads + head;
-    const Codes<VB> fa = load_codes<VB>(a.fixed_a + (int64_t)row * a.ld + off, mine);
-    Codes<VB> fb;
-    if constexpr (MODE != FORWARD) fb = load_codes<VB>(a.fixed_b + (int64_t)row * a.ld + off, mine);
+    const int64_t rh = (int64_t)row * a.heads + hd, at_row = (int64_t)row * a.ld + off;
+    Codes<VB> fa, fb;
+    if constexpr (MODE == BY_SRC) {
+#pragma unroll
+        for (int i = 0; i < VB / 4; ++i) fa.w[i] = fb.w[i] = 0;
+        if (mine) load_runs<VB>(a.kv + 2 * at_row, fa, fb);
+    } else {
+        fa = codes_if<VB>(mine, a.q + at_row);
+        if constexpr (MODE == BY_DST) fb = codes_if<VB>(mine, a.o + at_row);
+    }
     float sa = 0.f, sb = 0.f, top = 0.f, inv = 0.f;
-    if (row >= 0 && has_head) {
-        sa = __ldg(a.fixed_sa + rh);
-        if constexpr (MODE != FORWARD) sb = __ldg(a.fixed_sb + rh);
+    if (row >= 0) {
+        if constexpr (MODE == BY_SRC) {
+            const float2 t = __ldg(a.skv + rh);
+            sa = t.x; sb = t.y;
+        } else {
+            sa = __ldg(a.sq + rh) * a.qscale;
+        }
         if constexpr (MODE == BY_DST) {
+            sb = __ldg(a.so + rh);
             const float2 st = __ldg(a.stats + rh);
             top = st.x; inv = st.y;
         }
     }
-    if constexpr (MODE != BY_SRC) sa *= a.qscale;
+    const int8_t *base = (MODE == BY_SRC ? a.qo : a.kv) + 2 * off;
+    const int ld2 = 2 * a.ld;
+    const float2 *skv_base = a.skv + hd;
+    const float4 *rec_base = a.record + hd;
 
     Running<VB> run;                    // forward: the softmax; else acc = the first sum
     Pair acc2[VB / 2];
@@ -271,66 +293,77 @@ __global__ void __launch_bounds__(kWarps * 32) attn_kernel(const __grid_constant
 #pragma unroll
     for (int i = 0; i < VB / 2; ++i) acc2[i] = pair(0.f, 0.f);
 
+    // One trip of a row: U edges a slot.  The next trip's loads are under way while one is worked on.
+    struct Trip {
+        Codes<VB> a[U], b[U];
+        float2 kv[U];
+        float4 rec[U];
+    };
     const int stride = slots * U;
     const int trips = (int)__reduce_max_sync(0xffffffffu, (unsigned)((end - beg + stride - 1) / stride));
-    int j = beg + slot, next[U];
+    const int last = end > beg ? end - 1 : 0;
+    int next[U];
+    const auto ids = [&](int j) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) next[u] = j + u * slots < end ? __ldg(a.indices + j + u * slots) : -1;
-    for (int t = 0; t < trips; ++t) {
-        Codes<VB> ga[U], gb[U];
-        float ta[U], tb[U];
-        float4 rec[U];
-        bool there[U];
+        for (int u = 0; u < U; ++u) next[u] = __ldg(a.indices + min(j + u * slots, last));
+    };
+    const auto load = [&](Trip &t) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            there[u] = next[u] >= 0;
-            const int64_t at = (int64_t)next[u] * a.ld + off;
-            ga[u] = load_codes<VB>(a.gather_a + at, there[u] && live);
-            gb[u] = load_codes<VB>(a.gather_b + at, there[u] && live);
-            ta[u] = tb[u] = 0.f;
-            rec[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (there[u] && has_head) {
-                const int64_t h = (int64_t)next[u] * a.heads + head;
-                if constexpr (MODE == BY_SRC) {
-                    rec[u] = __ldg(a.record + h);
-                } else {
-                    ta[u] = __ldg(a.gather_sa + h);
-                    tb[u] = __ldg(a.gather_sb + h);
-                }
-            }
+            load_runs<VB>(base + (int64_t)next[u] * ld2, t.a[u], t.b[u]);
+            if constexpr (MODE == BY_SRC) t.rec[u] = __ldg(rec_base + (int64_t)next[u] * a.heads);
+            else t.kv[u] = __ldg(skv_base + (int64_t)next[u] * a.heads);
         }
-        j += stride;
-#pragma unroll
-        for (int u = 0; u < U; ++u) next[u] = j + u * slots < end ? __ldg(a.indices + j + u * slots) : -1;
+    };
+    const auto work = [&](const Trip &t, int j) {
         if constexpr (MODE == FORWARD) {
-            float z[U];
+            float z[U], sv[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const float s = dot<VB, P>(fa, ga[u]);
-                z[u] = there[u] ? __fmul_rn(s, __fmul_rn(ta[u], sa)) : -INFINITY;
+                const float s = dot<VB, P>(fa, t.a[u]);
+                z[u] = j + u * slots < end ? __fmul_rn(s, __fmul_rn(t.kv[u].x, sa)) : -INFINITY;
+                sv[u] = t.kv[u].y;
             }
-            softmax_step<VB, U>(run, z, tb, gb);
+            softmax_step<VB, U>(run, z, sv, t.b);
         } else if constexpr (MODE == BY_DST) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const float s = dot<VB, P>(fa, ga[u]), dp = dot<VB, P>(fb, gb[u]) * tb[u];
-                const float z = __fmul_rn(s, __fmul_rn(ta[u], sa));
-                const float p = there[u] ? exp2_fast(z - top) * inv : 0.f;
+                const float s = dot<VB, P>(fa, t.a[u]), dp = dot<VB, P>(fb, t.b[u]) * t.kv[u].y;
+                const float z = j + u * slots < end ? __fmul_rn(s, __fmul_rn(t.kv[u].x, sa)) : -INFINITY;
+                const float p = exp2_fast(z - top) * inv;
                 delta = fmaf(p, dp, delta);
-                const float pk = p * ta[u], pdk = pk * dp;
-                add_codes_twice<VB>(run.acc, acc2, ga[u], pair(pdk, pdk), pair(pk, pk));
+                const float pk = p * t.kv[u].x, pdk = pk * dp;
+                add_codes_twice<VB>(run.acc, acc2, t.a[u], pair(pdk, pdk), pair(pk, pk));
             }
         } else {
             // record of a destination: scale * log2(e) * scale of q, maximum, scale of o / sum, delta / scale of o
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const float s = dot<VB, P>(fa, ga[u]), dp = dot<VB, P>(fb, gb[u]) * sb;
-                const float z = __fmul_rn(s, __fmul_rn(sa, rec[u].x));
-                const float p = there[u] ? exp2_fast(z - rec[u].y) * rec[u].z : 0.f;
-                const float ds = p * (dp - rec[u].w) * rec[u].x;
-                add_codes<VB>(run.acc, ga[u], pair(ds, ds));
-                add_codes<VB>(acc2, gb[u], pair(p, p));
+                const float s = dot<VB, P>(fa, t.a[u]), dp = dot<VB, P>(fb, t.b[u]) * sb;
+                const float z = j + u * slots < end ? __fmul_rn(s, __fmul_rn(sa, t.rec[u].x)) : -INFINITY;
+                const float p = exp2_fast(z - t.rec[u].y) * t.rec[u].z;
+                const float ds = p * (dp - t.rec[u].w) * t.rec[u].x;
+                add_codes<VB>(run.acc, t.a[u], pair(ds, ds));
+                add_codes<VB>(acc2, t.b[u], pair(p, p));
             }
+        }
+    };
+    if (trips > 0) {
+        Trip even, odd;
+        int j = beg + slot;
+        ids(j);
+        load(even);
+        ids(j + stride);
+        for (int t = 0;; t += 2) {
+            load(odd);
+            ids(j + 2 * stride);
+            work(even, j);
+            if (t + 1 >= trips) break;
+            load(even);
+            ids(j + 3 * stride);
+            work(odd, j + stride);
+            if (t + 2 >= trips) break;
+            j += 2 * stride;
         }
     }
 
@@ -347,7 +380,15 @@ __global__ void __launch_bounds__(kWarps * 32) attn_kernel(const __grid_constant
             }
         }
     }
+    if (end == beg) {               // a row without edges read along with others, whose NaN is not its own
+        run.l = delta = 0.f;
+#pragma unroll
+        for (int i = 0; i < VB / 2; ++i) run.acc[i] = acc2[i] = pair(0.f, 0.f);
+    }
     if (slot != 0 || row < 0 || !live) return;
+    if constexpr (MODE == BY_DST) {
+        if (a.qo && place == 0) store_runs<VB>(a.qo + 2 * at_row, fa, fb);
+    }
     if (unit >= 0) {
         float *ws = a.ws + unit * partial_floats(MODE, a.heads, a.ld);
         if (chunk == 0) {
@@ -370,20 +411,21 @@ __global__ void __launch_bounds__(kWarps * 32) attn_kernel(const __grid_constant
 #pragma unroll
         for (int i = 0; i < VB / 2; ++i) run.acc[i] = fma2(acc2[i], nd, run.acc[i]);
         store_typed<VB>(a.out_a, out, a.type, e, a.d, run.acc, a.qscale * 0.69314718055994531f * sb);
-        if (chunk == 0) a.record[rh] = make_float4(sa, top, inv * sb, delta);
+        if (chunk == 0 && a.record) a.record[rh] = make_float4(sa, top, inv * sb, delta);
     } else {
         store_typed<VB>(a.out_a, out, a.type, e, a.d, run.acc, 0.69314718055994531f);
         store_typed<VB>(a.out_b, out, a.type, e, a.d, acc2, 1.f);
     }
 }
 
-// One block per heavy row: its units in order.
+// A block per heavy row.  Its threads stand for the codes of a row, several times over: each takes every G-th unit, and the G
+// partial results meet in shared memory.
 struct MergeArgs {
-    const int32_t *heavy_rows, *heavy_first;
-    int heads, d, pitch;
-    int64_t ld;
+    const int4 *rows;
+    const int32_t *heavy_first;
+    int heads, d, pitch, ld;
     const float *ws;
-    const float *fixed_sa, *fixed_sb;
+    const float *sq, *so;
     float qscale;
     float2 *stats;
     float4 *record;
@@ -395,48 +437,79 @@ __device__ __forceinline__ void store_one(void *out, int64_t at, int type, float
     else if (type == TANGO_BF16) from_float(v, static_cast<Bf16 *>(out)[at]);
     else from_float(v, static_cast<Fp16 *>(out)[at]);
 }
+constexpr int kMergeThreads = 512;
+
 template <int MODE>
-__global__ void __launch_bounds__(256) attn_merge_kernel(const __grid_constant__ MergeArgs a) {
-    const int64_t row = __ldg(a.heavy_rows + blockIdx.x);
-    const int first = __ldg(a.heavy_first + blockIdx.x), last = __ldg(a.heavy_first + blockIdx.x + 1);
+__global__ void __launch_bounds__(kMergeThreads) attn_merge_kernel(const __grid_constant__ MergeArgs a) {
+    __shared__ float s_x[kMergeThreads], s_y[kMergeThreads], s_z[kMergeThreads];
+    const int64_t row = __ldg(&a.rows[blockIdx.x].x);
+    const int first = __ldg(a.heavy_first + blockIdx.x), n = __ldg(a.heavy_first + blockIdx.x + 1) - first;
     const int64_t step = partial_floats(MODE, a.heads, a.ld);
     const float *ws = a.ws + (int64_t)first * step;
-    const int n = last - first, per_head = (partial_heads(MODE) * a.heads + 3) / 4 * 4;
-    for (int e = threadIdx.x; e < a.ld; e += blockDim.x) {
-        const int head = e / a.pitch, i = e - head * a.pitch;
-        const int64_t rh = row * a.heads + head, out = rh * a.d + i;
-        if (i >= a.d) continue;
-        if constexpr (MODE == FORWARD) {
-            float m = -INFINITY;
-            for (int u = 0; u < n; ++u) m = fmaxf(m, ws[u * step + 2 * head]);
-            float l = 0.f, s = 0.f;
-            for (int u = 0; u < n; ++u) {
-                const float mu = ws[u * step + 2 * head], c = mu == -INFINITY ? 0.f : exp2_fast(mu - m);
-                l = fmaf(ws[u * step + 2 * head + 1], c, l);
-                s = fmaf(ws[u * step + per_head + e], c, s);
+    const int per_head = (partial_heads(MODE) * a.heads + 3) / 4 * 4;
+    const int width = a.ld < kMergeThreads ? a.ld : kMergeThreads, G = kMergeThreads / width;
+    const int g = threadIdx.x / width, in = threadIdx.x % width;
+    for (int e0 = 0; e0 < a.ld; e0 += width) {
+        const int e = e0 + in, head = e / a.pitch, i = e - head * a.pitch;
+        const bool there = g < G && e < a.ld;
+        // forward: x sum, y maximum, z sum of weights; by destination: both sums and delta; by source: both sums
+        float x = 0.f, y = MODE == FORWARD ? kBelow : 0.f, z = 0.f;
+        if (there) {
+            if constexpr (MODE == FORWARD) {
+#pragma unroll 4
+                for (int u = g; u < n; u += G) y = fmaxf(y, ws[u * step + 2 * head]);
             }
-            const float by = l == 0.f ? 0.f : __fdiv_rn(1.f, l);
-            store_one(a.out_a, out, a.type, s * by);
-            if (i == 0 && a.stats) a.stats[rh] = make_float2(l == 0.f ? 0.f : m, by);
-        } else {
-            float delta = 0.f, x = 0.f, y = 0.f;
-            for (int u = 0; u < n; ++u) {
-                if constexpr (MODE == BY_DST) delta += ws[u * step + head];
-                x += ws[u * step + per_head + e];
-                y += ws[u * step + per_head + a.ld + e];
+#pragma unroll 4
+            for (int u = g; u < n; u += G) {
+                const float *p = ws + u * step;
+                if constexpr (MODE == FORWARD) {
+                    const float c = exp2_fast(p[2 * head] - y);
+                    z = fmaf(p[2 * head + 1], c, z);
+                    x = fmaf(p[per_head + e], c, x);
+                } else {
+                    if constexpr (MODE == BY_DST) z += p[head];
+                    x += p[per_head + e];
+                    y += p[per_head + a.ld + e];
+                }
             }
-            if constexpr (MODE == BY_DST) {
-                const float sb = a.fixed_sb[rh];
-                store_one(a.out_a, out, a.type, fmaf(y, -delta, x) * (a.qscale * 0.69314718055994531f * sb));
-                if (i == 0) {
+        }
+        s_x[threadIdx.x] = x; s_y[threadIdx.x] = y; s_z[threadIdx.x] = z;
+        __syncthreads();
+        if (g == 0 && there && i < a.d) {
+            const int64_t rh = row * a.heads + head, out = rh * a.d + i;
+            float m = y;
+            if constexpr (MODE == FORWARD) {
+                for (int k = 1; k < G; ++k) m = fmaxf(m, s_y[k * width + in]);
+                const float c = exp2_fast(y - m);
+                x *= c; z *= c;
+            }
+            for (int k = 1; k < G; ++k) {
+                const int at = k * width + in;
+                if constexpr (MODE == FORWARD) {
+                    const float c = exp2_fast(s_y[at] - m);
+                    x = fmaf(s_x[at], c, x);
+                    z = fmaf(s_z[at], c, z);
+                } else {
+                    x += s_x[at]; y += s_y[at]; z += s_z[at];
+                }
+            }
+            if constexpr (MODE == FORWARD) {
+                const float by = z == 0.f ? 0.f : __fdiv_rn(1.f, z);
+                store_one(a.out_a, out, a.type, x * by);
+                if (i == 0 && a.stats) a.stats[rh] = make_float2(z == 0.f ? 0.f : m, by);
+            } else if constexpr (MODE == BY_DST) {
+                const float sb = a.so[rh];
+                store_one(a.out_a, out, a.type, fmaf(y, -z, x) * (a.qscale * 0.69314718055994531f * sb));
+                if (i == 0 && a.record) {
                     const float2 st = a.stats[rh];
-                    a.record[rh] = make_float4(a.fixed_sa[rh] * a.qscale, st.x, st.y * sb, delta);
+                    a.record[rh] = make_float4(a.sq[rh] * a.qscale, st.x, st.y * sb, z);
                 }
             } else {
                 store_one(a.out_a, out, a.type, x * 0.69314718055994531f);
                 store_one(a.out_b, out, a.type, y);
             }
         }
+        __syncthreads();
     }
 }
 
@@ -448,7 +521,7 @@ struct RowsArgs {
     const void *q;
     int64_t ldq;                  // elements between two queries
     int heads, d, pitch, hb;
-    int64_t ld;
+    int ld;
     const int8_t *k, *v;
     const float *sk, *sv;
     float qscale;
@@ -470,16 +543,15 @@ __host__ __device__ inline int row_chunk(int len, int splits) {
 template <int VB, int P, class T>
 __device__ __forceinline__ Codes<VB> encode_query(const RowsArgs &a, int64_t r, int head, int chunk, bool live, float &s) {
     const int64_t at = r * a.ldq + (int64_t)head * a.d + chunk * VB;
-    float v[VB / 4][4];
-    uint32_t top = 0;
+    float v[VB / 4][4], top = 0.f;
 #pragma unroll
     for (int i = 0; i < VB / 4; ++i) {
         load4<T, 1>(static_cast<const T *>(a.q) + at + 4 * i, live ? min(4, a.d - chunk * VB - 4 * i) : 0, v[i]);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) top = max(top, __float_as_uint(v[i][k]) & 0x7fffffffu);
+        for (int k = 0; k < 4; k += 2) top = max_abs3(v[i][k], v[i][k + 1], top);
     }
 #pragma unroll
-    for (int o = P / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    for (int o = P / 2; o > 0; o >>= 1) top = max_or_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
     s = group_scale(top);
     const float inv = group_inverse(s);
     Codes<VB> c;
@@ -493,10 +565,10 @@ __device__ __forceinline__ Codes<VB> encode_query(const RowsArgs &a, int64_t r, 
 }
 
 template <int VB, int P>
-__global__ void __launch_bounds__(kWarps * 32) attn_rows_kernel(const __grid_constant__ RowsArgs a) {
+__global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(const __grid_constant__ RowsArgs a) {
     constexpr int U = InFlight<FORWARD>::U;
-    __shared__ float s_acc[kWarps][32 * VB];
-    __shared__ float2 s_ml[kWarps][32];
+    __shared__ float s_acc[kRowWarps][32 * VB];
+    __shared__ float2 s_ml[kRowWarps][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t r = blockIdx.x;
     const int64_t row = __ldg(a.rows + r);
@@ -510,41 +582,34 @@ __global__ void __launch_bounds__(kWarps * 32) attn_rows_kernel(const __grid_con
     const int L = a.hb * P, slots = 32 / L;
     const int slot = lane / L, in_edge = lane & (L - 1);
     const int head = blockIdx.z * a.hb + in_edge / P, chunk = in_edge & (P - 1);
-    const bool has_head = head < a.heads, live = has_head && chunk * VB < a.pitch;
-    const int64_t off = (int64_t)head * a.pitch + chunk * VB;
+    const bool live = head < a.heads && chunk * VB < a.pitch;
+    const int hd = head < a.heads ? head : a.heads - 1, off = live ? head * a.pitch + chunk * VB : hd * a.pitch;
     float sa;
     const Codes<VB> fa = a.type == TANGO_FP32   ? encode_query<VB, P, float>(a, r, head, chunk, live, sa)
                          : a.type == TANGO_BF16 ? encode_query<VB, P, Bf16>(a, r, head, chunk, live, sa)
                                                 : encode_query<VB, P, Fp16>(a, r, head, chunk, live, sa);
     sa *= a.qscale;
     Running<VB> run;
-    const int stride = slots * U * kWarps;
+    const int stride = slots * U * kRowWarps;
     for (int j = beg + warp * slots * U; j < end; j += stride) {
         Codes<VB> ga[U], gb[U];
-        float z[U], ta[U], tb[U];
+        float z[U], sk[U], sv[U];
         int at[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int e = j + u * slots + slot;
-            at[u] = e < end ? __ldg(a.indices + e) : -1;
-        }
+        for (int u = 0; u < U; ++u) at[u] = __ldg(a.indices + min(j + u * slots + slot, end - 1));
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const bool there = at[u] >= 0;
-            ga[u] = load_codes<VB>(a.k + (int64_t)at[u] * a.ld + off, there && live);
-            gb[u] = load_codes<VB>(a.v + (int64_t)at[u] * a.ld + off, there && live);
-            ta[u] = tb[u] = 0.f;
-            if (there && has_head) {
-                ta[u] = __ldg(a.sk + (int64_t)at[u] * a.heads + head);
-                tb[u] = __ldg(a.sv + (int64_t)at[u] * a.heads + head);
-            }
+            ga[u] = load_codes<VB>(a.k + (int64_t)at[u] * a.ld + off);
+            gb[u] = load_codes<VB>(a.v + (int64_t)at[u] * a.ld + off);
+            sk[u] = __ldg(a.sk + (int64_t)at[u] * a.heads + hd);
+            sv[u] = __ldg(a.sv + (int64_t)at[u] * a.heads + hd);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const float s = dot<VB, P>(fa, ga[u]);
-            z[u] = at[u] >= 0 ? __fmul_rn(s, __fmul_rn(ta[u], sa)) : -INFINITY;
+            z[u] = j + u * slots + slot < end ? __fmul_rn(s, __fmul_rn(sk[u], sa)) : -INFINITY;
         }
-        softmax_step<VB, U>(run, z, tb, gb);
+        softmax_step<VB, U>(run, z, sv, gb);
     }
     for (int o = L; o < 32; o <<= 1) run.merge(o);
     if (slot == 0) {
@@ -553,16 +618,16 @@ __global__ void __launch_bounds__(kWarps * 32) attn_rows_kernel(const __grid_con
         for (int i = 0; i < VB / 2; ++i) reinterpret_cast<float2 *>(s_acc[warp])[in_edge * (VB / 2) + i] = both(run.acc[i]);
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < L * VB; e += kWarps * 32) {
+    for (int e = threadIdx.x; e < L * VB; e += kRowWarps * 32) {
         const int ie = e / VB, hd = blockIdx.z * a.hb + ie / P, i = (ie & (P - 1)) * VB + e % VB;
         if (hd >= a.heads || i >= a.d) continue;
-        float m = -INFINITY, l = 0.f, s = 0.f;
+        float m = kBelow, l = 0.f, s = 0.f;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) m = fmaxf(m, s_ml[w][ie].x);
+        for (int w = 0; w < kRowWarps; ++w) m = fmaxf(m, s_ml[w][ie].x);
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
+        for (int w = 0; w < kRowWarps; ++w) {
             const float2 ml = s_ml[w][ie];
-            const float c = ml.x == -INFINITY ? 0.f : exp2_fast(ml.x - m);
+            const float c = exp2_fast(ml.x - m);
             l = fmaf(ml.y, c, l);
             s = fmaf(s_acc[w][e], c, s);
         }
@@ -588,10 +653,10 @@ __global__ void __launch_bounds__(256) attn_rows_merge_kernel(const __grid_const
     for (int e = threadIdx.x; e < a.ld; e += blockDim.x) {
         const int head = e / a.pitch, i = e - head * a.pitch;
         if (i >= a.d) continue;
-        float m = -INFINITY, l = 0.f, s = 0.f;
+        float m = kBelow, l = 0.f, s = 0.f;
         for (int u = 0; u < n; ++u) m = fmaxf(m, ws[u * step + 2 * head]);
         for (int u = 0; u < n; ++u) {
-            const float mu = ws[u * step + 2 * head], c = mu == -INFINITY ? 0.f : exp2_fast(mu - m);
+            const float c = exp2_fast(ws[u * step + 2 * head] - m);
             l = fmaf(ws[u * step + 2 * head + 1], c, l);
             s = fmaf(ws[u * step + per_head + e], c, s);
         }
@@ -632,15 +697,13 @@ template <int MODE>
 static int launch(AttnArgs a, const tango_edge_plan *plan, float *ws, int64_t ws_bytes, cudaStream_t st) {
     a.n_long = a.n_rows;
     if (plan) {
-        a.row_order = plan->row_order;
+        a.rows = reinterpret_cast<const int4 *>(plan->rows);
         a.units = reinterpret_cast<const int4 *>(plan->units);
-        a.n_units = plan->n_units; a.n_heavy = plan->n_heavy;
-        if (plan->row_order) a.n_long = plan->n_long_rows;
-        if (a.n_units < 0 || a.n_heavy < 0 || a.n_long < a.n_heavy || a.n_long > a.n_rows) return TANGO_EINVAL;
-        if (a.n_heavy > 0 && (!plan->units || !plan->row_order || !plan->heavy_rows || !plan->heavy_first || !ws ||
-                              ws_bytes < a.n_units * partial_floats(MODE, a.heads, a.ld) * 4))
+        a.n_units = plan->n_units; a.n_heavy = plan->n_heavy; a.n_long = plan->n_long;
+        if (!plan->rows || a.n_units < 0 || a.n_heavy < 0 || a.n_long < a.n_heavy || a.n_long > a.n_rows) return TANGO_EINVAL;
+        if (a.n_heavy > 0 && (!plan->units || !plan->heavy_first || !ws || ws_bytes < a.n_units * partial_floats(MODE, a.heads, a.ld) * 4))
             return TANGO_EINVAL;
-        if (!aligned(plan->units, 16) || !aligned(ws, 16)) return TANGO_EALIGN;
+        if (!aligned(plan->rows, 16) || !aligned(plan->units, 16) || !aligned(ws, 16)) return TANGO_EALIGN;
     }
     a.ws = ws;
     const int rc = with_shape(a.d, [&](auto vb, auto p) -> int {
@@ -655,19 +718,29 @@ static int launch(AttnArgs a, const tango_edge_plan *plan, float *ws, int64_t ws
         return TANGO_OK;
     });
     if (rc != TANGO_OK || a.n_heavy == 0) return rc;
-    MergeArgs m{plan->heavy_rows, plan->heavy_first, a.heads, a.d, a.pitch, a.ld, ws, a.fixed_sa, a.fixed_sb, a.qscale,
+    MergeArgs m{a.rows, plan->heavy_first, a.heads, a.d, a.pitch, a.ld, ws, a.sq, a.so, a.qscale,
                 a.stats, a.record, a.out_a, a.out_b, a.type};
-    attn_merge_kernel<MODE><<<(unsigned)a.n_heavy, 256, 0, st>>>(m);
+    attn_merge_kernel<MODE><<<(unsigned)a.n_heavy, kMergeThreads, 0, st>>>(m);
     TANGO_LAUNCH_CHECK();
     return TANGO_OK;
 }
 
-static bool good_codes(const tango_rows8 *r, int d) { return r && r->q && r->scales && aligned(r->q, d > 8 ? 16 : d > 4 ? 8 : 4); }
+static bool good_codes(const int8_t *q, int d) { return q && aligned(q, d > 8 ? 16 : d > 4 ? 8 : 4); }
+
+// The 8-bit operands of a pass; the gradient's belong to the backward pass.
+static int operands(AttnArgs &a, const tango_edge_operands *x, bool backward) {
+    if (!x || !good_codes(x->q, a.d) || !x->kv || !x->sq || !x->skv) return TANGO_EINVAL;
+    if (backward && (!good_codes(x->o, a.d) || !x->so)) return TANGO_EINVAL;
+    if (!aligned(x->skv, 8) || !aligned(x->kv, 32)) return TANGO_EALIGN;
+    a.q = x->q; a.kv = x->kv; a.o = x->o; a.sq = x->sq; a.so = x->so;
+    a.skv = reinterpret_cast<const float2 *>(x->skv);
+    return TANGO_OK;
+}
 
 static AttnArgs attn_args(const int32_t *indptr, const int32_t *indices, int64_t n_rows, int heads, int d, float scale, int type) {
     AttnArgs a{};
     a.indptr = indptr; a.indices = indices; a.n_rows = n_rows;
-    a.heads = heads; a.d = d; a.pitch = (int)tango_rows8_pitch(d); a.ld = (int64_t)heads * a.pitch;
+    a.heads = heads; a.d = d; a.pitch = (int)tango_rows8_pitch(d); a.ld = heads * a.pitch;
     a.qscale = scale * 1.4426950408889634f;
     a.type = type;
     return a;
@@ -684,51 +757,41 @@ extern "C" int64_t tango_edge_attention_workspace_bytes(int pass, int64_t n_unit
 }
 
 extern "C" int tango_edge_attention(const int32_t *indptr, const int32_t *indices, int64_t n_rows, const tango_edge_plan *plan,
-                                    int heads, int d, const tango_rows8 *q, const tango_rows8 *k, const tango_rows8 *v, float scale,
-                                    void *out, int type, float *stats, void *ws, int64_t ws_bytes, tango_stream_t stream) {
+                                    int heads, int d, const tango_edge_operands *x, float scale, void *out, int type, float *stats,
+                                    void *ws, int64_t ws_bytes, tango_stream_t stream) {
     const int rc = check_shape(n_rows, heads, d, type);
     if (rc != TANGO_OK || n_rows == 0) return rc;
     if (!indptr || !indices || !out) return TANGO_EINVAL;
-    for (const tango_rows8 *r : {q, k, v})
-        if (!good_codes(r, d)) return TANGO_EINVAL;
-    if (!aligned(out, 16) || !aligned(stats, 8)) return TANGO_EALIGN;
     AttnArgs a = attn_args(indptr, indices, n_rows, heads, d, scale, type);
-    a.fixed_a = q->q; a.fixed_sa = q->scales;
-    a.gather_a = k->q; a.gather_sa = k->scales; a.gather_b = v->q; a.gather_sb = v->scales;
+    if (const int bad = operands(a, x, false)) return bad;
+    if (!aligned(out, 16) || !aligned(stats, 8)) return TANGO_EALIGN;
     a.stats = reinterpret_cast<float2 *>(stats); a.out_a = out;
     return launch<FORWARD>(a, plan, static_cast<float *>(ws), ws_bytes, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int tango_edge_attention_bwd_dst(const int32_t *indptr, const int32_t *indices, int64_t n_rows, const tango_edge_plan *plan,
-                                            int heads, int d, const tango_rows8 *q, const tango_rows8 *k, const tango_rows8 *v,
-                                            const tango_rows8 *grad, float scale, const float *stats, void *dq, int type, float *record,
-                                            void *ws, int64_t ws_bytes, tango_stream_t stream) {
+                                            int heads, int d, const tango_edge_operands *x, float scale, const float *stats, void *dq,
+                                            int type, float *record, int8_t *qo, void *ws, int64_t ws_bytes, tango_stream_t stream) {
     const int rc = check_shape(n_rows, heads, d, type);
     if (rc != TANGO_OK || n_rows == 0) return rc;
-    if (!indptr || !indices || !dq || !stats || !record) return TANGO_EINVAL;
-    for (const tango_rows8 *r : {q, k, v, grad})
-        if (!good_codes(r, d)) return TANGO_EINVAL;
-    if (!aligned(dq, 16) || !aligned(stats, 8) || !aligned(record, 16)) return TANGO_EALIGN;
+    if (!indptr || !indices || !dq || !stats || !record != !qo) return TANGO_EINVAL;
     AttnArgs a = attn_args(indptr, indices, n_rows, heads, d, scale, type);
-    a.fixed_a = q->q; a.fixed_sa = q->scales; a.fixed_b = grad->q; a.fixed_sb = grad->scales;
-    a.gather_a = k->q; a.gather_sa = k->scales; a.gather_b = v->q; a.gather_sb = v->scales;
-    a.stats = reinterpret_cast<float2 *>(const_cast<float *>(stats)); a.record = reinterpret_cast<float4 *>(record); a.out_a = dq;
+    if (const int bad = operands(a, x, true)) return bad;
+    if (!aligned(dq, 16) || !aligned(stats, 8) || !aligned(record, 16) || !aligned(qo, 32)) return TANGO_EALIGN;
+    a.stats = reinterpret_cast<float2 *>(const_cast<float *>(stats)); a.record = reinterpret_cast<float4 *>(record); a.out_a = dq; a.qo = qo;
     return launch<BY_DST>(a, plan, static_cast<float *>(ws), ws_bytes, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int tango_edge_attention_bwd_src(const int32_t *indptr, const int32_t *indices, int64_t n_rows, const tango_edge_plan *plan,
-                                            int heads, int d, const tango_rows8 *q, const tango_rows8 *k, const tango_rows8 *v,
-                                            const tango_rows8 *grad, const float *record, void *dk, void *dv, int type, void *ws,
-                                            int64_t ws_bytes, tango_stream_t stream) {
+                                            int heads, int d, const int8_t *kv, const float *skv, const int8_t *qo, const float *record,
+                                            void *dk, void *dv, int type, void *ws, int64_t ws_bytes, tango_stream_t stream) {
     const int rc = check_shape(n_rows, heads, d, type);
     if (rc != TANGO_OK || n_rows == 0) return rc;
-    if (!indptr || !indices || !dk || !dv || !record) return TANGO_EINVAL;
-    for (const tango_rows8 *r : {q, k, v, grad})
-        if (!good_codes(r, d)) return TANGO_EINVAL;
-    if (!aligned(dk, 16) || !aligned(dv, 16) || !aligned(record, 16)) return TANGO_EALIGN;
+    if (!indptr || !indices || !dk || !dv || !kv || !skv || !qo || !record) return TANGO_EINVAL;
+    if (!aligned(dk, 16) || !aligned(dv, 16) || !aligned(record, 16) || !aligned(kv, 32) || !aligned(qo, 32) || !aligned(skv, 8))
+        return TANGO_EALIGN;
     AttnArgs a = attn_args(indptr, indices, n_rows, heads, d, 0.f, type);
-    a.fixed_a = k->q; a.fixed_sa = k->scales; a.fixed_b = v->q; a.fixed_sb = v->scales;
-    a.gather_a = q->q; a.gather_sa = q->scales; a.gather_b = grad->q; a.gather_sb = grad->scales;
+    a.kv = kv; a.skv = reinterpret_cast<const float2 *>(skv); a.qo = const_cast<int8_t *>(qo);
     a.record = reinterpret_cast<float4 *>(const_cast<float *>(record)); a.out_a = dk; a.out_b = dv;
     return launch<BY_SRC>(a, plan, static_cast<float *>(ws), ws_bytes, static_cast<cudaStream_t>(stream));
 }
@@ -757,13 +820,13 @@ extern "C" int tango_edge_attention_rows(const int32_t *indptr, const int32_t *i
     if (splits > 65535) return TANGO_ESIZE;
     if (n_rows == 0) return TANGO_OK;
     if (!indptr || !indices || !rows || !q || !out || (n_rows > 1 && ldq < (int64_t)heads * d)) return TANGO_EINVAL;
-    if (n_nodes > 0 && (!good_codes(k, d) || !good_codes(v, d))) return TANGO_EINVAL;
+    if (n_nodes > 0 && (!k || !v || !good_codes(k->q, d) || !good_codes(v->q, d) || !k->scales || !v->scales)) return TANGO_EINVAL;
     if (splits > 1 && (!ws || ws_bytes < tango_edge_attention_rows_workspace_bytes(n_rows, splits, heads, d))) return TANGO_EINVAL;
     if (!aligned(q, type == TANGO_FP32 ? 4 : 2) || !aligned(ws, 16)) return TANGO_EALIGN;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     RowsArgs a{};
     a.indptr = indptr; a.indices = indices; a.rows = rows; a.n_nodes = n_nodes; a.q = q; a.ldq = ldq;
-    a.heads = heads; a.d = d; a.pitch = (int)tango_rows8_pitch(d); a.ld = (int64_t)heads * a.pitch;
+    a.heads = heads; a.d = d; a.pitch = (int)tango_rows8_pitch(d); a.ld = heads * a.pitch;
     if (n_nodes > 0) { a.k = k->q; a.sk = k->scales; a.v = v->q; a.sv = v->scales; }
     a.qscale = scale * 1.4426950408889634f; a.splits = splits; a.out = out; a.type = type; a.ws = static_cast<float *>(ws);
     a.mode = mode; a.seed = seed; a.call = call; a.step = reinterpret_cast<const unsigned long long *>(step);
@@ -772,7 +835,7 @@ extern "C" int tango_edge_attention_rows(const int32_t *indptr, const int32_t *i
         a.hb = heads_of_a_block(heads, P);
         const int64_t bz = ceil_div(heads, a.hb);
         if (bz > 65535) return TANGO_ESIZE;
-        attn_rows_kernel<VB, P><<<dim3((unsigned)n_rows, (unsigned)splits, (unsigned)bz), kWarps * 32, 0, st>>>(a);
+        attn_rows_kernel<VB, P><<<dim3((unsigned)n_rows, (unsigned)splits, (unsigned)bz), kRowWarps * 32, 0, st>>>(a);
         TANGO_LAUNCH_CHECK();
         return TANGO_OK;
     });

@@ -5,9 +5,8 @@
 //   backward : dx = dy * f'(code * s), from the 8-bit copy alone
 //
 // Bound by HBM: pack 5 bytes an fp32 element (4 read, 1 written), unpack 5, activation forward 9, backward 9.  A group is
-// owned by up to 32 lanes with four neighbouring elements each (their codes are one 32-bit store), so that its maximum is a
-// handful of shuffles and x is read once and stays in registers; each lane has several groups in flight, because one group's
-// loads alone do not cover the latency of HBM.
+// owned by a few lanes, each with R times four neighbouring elements LPG * 4 apart (a load and the store of four codes are
+// contiguous over the lanes), so that x is read once and stays in registers.
 #include "rows8.cuh"
 
 namespace tango {
@@ -20,7 +19,9 @@ struct Rows8Args {
     const void *x[kMaxJobs];      // pack: input; backward: gradient dy
     int64_t ldx[kMaxJobs];
     int8_t *q[kMaxJobs];
-    float *scale[kMaxJobs];       // [rows, groups]
+    float *scale[kMaxJobs];       // [rows, groups], of group i at i * scale_stride
+    int64_t scale_stride[kMaxJobs];
+    int run[kMaxJobs];            // 0, or the codes of a run of an interleaved matrix
     void *y;                      // activation forward: y; unpack and backward: output
     int64_t ldy;
     int64_t rows, cols, items;    // items = rows * groups
@@ -95,30 +96,27 @@ __global__ void __launch_bounds__(kBlock) rows8_pack_kernel(const __grid_constan
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        uint32_t top = 0;
+        float top = 0.f;
 #pragma unroll
         for (int r = 0; r < R; ++r)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) top = max(top, __float_as_uint(v[u][r][k]) & 0x7fffffffu);
-        if constexpr (LPG == 32) {
-            top = __reduce_max_sync(0xffffffffu, top);
-        } else {
+            for (int k = 0; k < 4; k += 2) top = max_abs3(v[u][r][k], v[u][r][k + 1], top);
 #pragma unroll
-            for (int o = LPG / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-        }
+        for (int o = LPG / 2; o > 0; o >>= 1) top = max_or_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
         const int64_t i = first + u * NG;
         if (i >= a.items) continue;
         const float s = group_scale(top), inv = group_inverse(s);
         const int width = w[u].g == a.groups - 1 ? (int)(a.ldq - (int64_t)w[u].g * a.pitch) : a.pitch;
-        int8_t *q = a.q[job] ? a.q[job] + w[u].row * a.ldq + (int64_t)w[u].g * a.pitch : nullptr;
+        const int run = a.run[job];
+        int8_t *q = a.q[job] ? a.q[job] + ((w[u].row * a.ldq + (int64_t)w[u].g * a.pitch) << (run > 0)) : nullptr;
         const bool keep = !ACT || q;          // an activation without a backward pass keeps nothing
-        if (lane == 0 && keep) a.scale[job][i] = s;
+        if (lane == 0 && keep) a.scale[job][i * a.scale_stride[job]] = s;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const int e = (lane + r * LPG) * 4;
             if (e >= width) continue;
             if (keep)
-                *reinterpret_cast<uint32_t *>(q + e) =
+                *reinterpret_cast<uint32_t *>(q + (run ? ((e & -run) << 1 | (e & (run - 1))) : e)) =
                     a.mode == TANGO_ROUND_NEAREST ? encode4(v[u][r], s, inv)
                                                   : encode4_mode(v[u][r], s, a.mode, a.seed, effective_call(a.call + job, a.step),
                                                                  (uint64_t)w[u].row * a.cols + (int64_t)w[u].g * a.group + e);
@@ -162,12 +160,13 @@ __global__ void __launch_bounds__(kBlock) rows8_unpack_kernel(const __grid_const
         for (int r = 0; r < R; ++r) {
             const int e = (lane + r * LPG) * 4;
             if (e >= w[u].n) continue;
-            float c[4], o[4];
-            decode4(word[u][r], c);
+            Pair lo, hi;
+            decode4(word[u][r], lo, hi);
+            const float2 l = both(mul2(lo, pair(s[u], s[u]))), h = both(mul2(hi, pair(s[u], s[u])));
+            float o[4] = {l.x, l.y, h.x, h.y};
+            if constexpr (ACT) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                o[k] = __fmul_rn(c[k], s[u]);
-                if constexpr (ACT) o[k] = __fmul_rn(dy[u][r][k], slope_of(o[k], a.act));
+                for (int k = 0; k < 4; ++k) o[k] = __fmul_rn(dy[u][r][k], slope_of(o[k], a.act));
             }
             store4<T, VL>(static_cast<T *>(a.y) + w[u].row * a.ldy + (int64_t)w[u].g * a.group + e, w[u].n - e, o);
         }
@@ -187,12 +186,13 @@ static int launch_tile(const Rows8Args &a, int jobs, cudaStream_t st) {
     return PACK ? go(Tile<LPG, R>{}, rows8_pack_kernel<T, VL, LPG, R, ACT>)                 \
                 : go(Tile<LPG, R>{}, rows8_unpack_kernel<T, VL, LPG, R, ACT>)
     if (a.group <= 4) TANGO_ROWS8_TILE(1, 1);
-    if (a.group <= 8) TANGO_ROWS8_TILE(2, 1);
-    if (a.group <= 16) TANGO_ROWS8_TILE(4, 1);
-    if (a.group <= 32) TANGO_ROWS8_TILE(8, 1);
-    if (a.group <= 64) TANGO_ROWS8_TILE(16, 1);
-    if (a.group <= 128) TANGO_ROWS8_TILE(32, 1);
-    if (a.group <= 256) TANGO_ROWS8_TILE(32, 2);
+    if (a.group <= 8) TANGO_ROWS8_TILE(1, 2);
+    if (a.group <= 16) TANGO_ROWS8_TILE(1, 4);
+    if (a.group <= 32) TANGO_ROWS8_TILE(2, 4);
+    if (a.group <= 64) TANGO_ROWS8_TILE(4, 4);
+    if (a.group <= 128) TANGO_ROWS8_TILE(8, 4);
+    if (a.group <= 256) TANGO_ROWS8_TILE(16, 4);
+    if (a.group <= 512) TANGO_ROWS8_TILE(32, 4);
     TANGO_ROWS8_TILE(32, 8);
 #undef TANGO_ROWS8_TILE
 }
@@ -236,16 +236,15 @@ static int vector_length(const void *p, int64_t ld, int64_t rows, int64_t group,
 
 using namespace tango;
 
-extern "C" int64_t tango_rows8_pitch(int64_t group) {
-    if (group < 1) return TANGO_EINVAL;
-    return round_up(group, group > 8 ? 16 : group > 4 ? 8 : 4);
-}
+extern "C" int64_t tango_rows8_run(int64_t group) { return group < 1 ? TANGO_EINVAL : group > 8 ? 16 : group > 4 ? 8 : 4; }
+
+extern "C" int64_t tango_rows8_pitch(int64_t group) { return group < 1 ? TANGO_EINVAL : round_up(group, tango_rows8_run(group)); }
 
 extern "C" int64_t tango_rows8_ld(int64_t cols, int64_t group) {
     if (cols < 0 || group < 1) return TANGO_EINVAL;
     if (cols == 0) return 0;
     const int64_t before = (cols - 1) / group;
-    return before * tango_rows8_pitch(group) + round_up(cols - before * group, group > 8 ? 16 : group > 4 ? 8 : 4);
+    return before * tango_rows8_pitch(group) + round_up(cols - before * group, tango_rows8_run(group));
 }
 
 extern "C" int tango_rows8_pack(const tango_rows8_job *jobs, int n_jobs, int64_t rows, int64_t cols, int64_t group, int type,
@@ -257,9 +256,11 @@ extern "C" int tango_rows8_pack(const tango_rows8_job *jobs, int n_jobs, int64_t
     int vl = 4;
     for (int k = 0; k < n_jobs; ++k) {
         const tango_rows8_job &j = jobs[k];
-        if (!j.x || !j.q || !j.scales || (rows > 1 && j.ldx < cols)) return TANGO_EINVAL;
+        if (!j.x || !j.q || !j.scales || j.scale_stride < 1 || (rows > 1 && j.ldx < cols)) return TANGO_EINVAL;
         if (!aligned(j.x, element_bytes(type)) || !aligned(j.q, 4)) return TANGO_EALIGN;
         a.x[k] = j.x; a.ldx[k] = j.ldx; a.q[k] = j.q; a.scale[k] = j.scales;
+        a.scale_stride[k] = j.scale_stride;
+        a.run[k] = j.interleaved ? (int)tango_rows8_run(group) : 0;
         const int v = vector_length(j.x, j.ldx, rows, group, a.groups, type);
         if (v < vl) vl = v;
     }
@@ -285,9 +286,9 @@ extern "C" int tango_act8_forward(int act, const tango_rows8_job *job, int64_t r
     Rows8Args a{};
     const int rc = fill(a, rows, cols, group, type);
     if (rc != TANGO_OK || rows == 0 || cols == 0) return rc;
-    if (!job->x || !job->q != !job->scales || !y || (rows > 1 && (job->ldx < cols || ldy < cols))) return TANGO_EINVAL;
+    if (!job->x || !job->q != !job->scales || (job->q && job->scale_stride < 1) || !y || (rows > 1 && (job->ldx < cols || ldy < cols))) return TANGO_EINVAL;
     if (!aligned(job->x, element_bytes(type)) || !aligned(y, element_bytes(type)) || !aligned(job->q, 4)) return TANGO_EALIGN;
-    a.x[0] = job->x; a.ldx[0] = job->ldx; a.q[0] = job->q; a.scale[0] = job->scales; a.y = y; a.ldy = ldy;
+    a.x[0] = job->x; a.ldx[0] = job->ldx; a.q[0] = job->q; a.scale[0] = job->scales; a.scale_stride[0] = job->scale_stride; a.y = y; a.ldy = ldy;
     a.mode = mode; a.act = act; a.seed = seed; a.call = call;
     a.step = reinterpret_cast<const unsigned long long *>(step);
     const int vx = vector_length(job->x, job->ldx, rows, group, a.groups, type), vy = vector_length(y, ldy, rows, group, a.groups, type);

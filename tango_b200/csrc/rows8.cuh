@@ -7,11 +7,51 @@ namespace tango {
 constexpr float kSmallestNormal = 1.1754943508222875e-38f;      // 2^-126
 constexpr float kRoundMagic = 12582912.f;                       // 1.5 * 2^23: adding it leaves round-to-even(t) in the low bits
 
-// Scale of a group from the bits of its largest magnitude.  Bits of magnitudes order like the magnitudes, infinity and NaN
-// above all numbers: a group that holds one gets the scale NaN, so that its values come back as NaN, not as something else.
-__device__ __forceinline__ float group_scale(uint32_t top) {
-    if (top >= 0x7f800000u) return __int_as_float(0x7fffffff);
-    const float s = __fdiv_rn(__uint_as_float(top), 127.0f);
+// Two floats that one instruction works on.
+struct Pair { uint64_t v; };
+__device__ __forceinline__ Pair pair(float a, float b) {
+    Pair p;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p.v) : "f"(a), "f"(b));
+    return p;
+}
+__device__ __forceinline__ float2 both(Pair p) {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p.v));
+    return f;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+    Pair o;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(o.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return o;
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+    Pair o;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(o.v) : "l"(a.v), "l"(b.v));
+    return o;
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+    Pair o;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(o.v) : "l"(a.v), "l"(b.v));
+    return o;
+}
+
+// max(|a|, |b|, |c|), NaN if one of them is.
+__device__ __forceinline__ float max_abs3(float a, float b, float c) {
+    float o;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(o) : "f"(a), "f"(b), "f"(c));
+    return o;
+}
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+    float o;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(o) : "f"(a), "f"(b));
+    return o;
+}
+
+// Scale of a group from its largest magnitude.  A group that holds an infinity or a NaN gets the scale NaN, so that its values
+// come back as NaN, not as something else.
+__device__ __forceinline__ float group_scale(float top) {
+    if (!(top < INFINITY)) return __int_as_float(0x7fffffff);
+    const float s = __fdiv_rn(top, 127.0f);
     return s < kSmallestNormal ? 0.f : s;
 }
 // About 1 / s; 0 for the scales 0 and NaN.
@@ -21,18 +61,16 @@ __device__ __forceinline__ float group_inverse(float s) { return s > 0.f ? __fdi
 // values that close to a border between two codes.  For those x - q * s is exact in one fused operation (a multiple of half
 // an ulp of s, at most about s / 2), and its double is compared with s.
 __device__ __forceinline__ uint32_t encode4(const float (&x)[4], float s, float inv) {
-    float b[4], far = 0.f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float t = __fmul_rn(x[i], inv);
-        b[i] = __fadd_rn(t, kRoundMagic);
-        far = fmaxf(far, fabsf(__fsub_rn(t, __fsub_rn(b[i], kRoundMagic))));
-    }
-    if (far > 0.4999f) {
+    const Pair by = pair(inv, inv), magic = pair(kRoundMagic, kRoundMagic), minus = pair(-1.f, -1.f);
+    const Pair x0 = pair(x[0], x[1]), x1 = pair(x[2], x[3]);
+    const Pair b0 = fma2(x0, by, magic), b1 = fma2(x1, by, magic);
+    const float2 d0 = both(fma2(x0, by, fma2(b0, minus, magic))), d1 = both(fma2(x1, by, fma2(b1, minus, magic)));
+    const float2 c0 = both(b0), c1 = both(b1);
+    float b[4] = {c0.x, c0.y, c1.x, c1.y};
+    if (max_abs3(max_abs3(d0.x, d0.y, d1.x), d1.y, 0.f) > 0.4999f) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            float q = __fsub_rn(b[i], kRoundMagic);
-            const float r = fmaf(-q, s, x[i]), twice = 2.f * fabsf(r);
+            const float r = fmaf(__fsub_rn(kRoundMagic, b[i]), s, x[i]), twice = 2.f * fabsf(r);
             if (twice > s || (twice == s && (__float_as_int(b[i]) & 1))) b[i] = __fadd_rn(b[i], r > 0.f ? 1.f : -1.f);
         }
     }
@@ -57,12 +95,11 @@ static __device__ __noinline__ uint32_t encode4_mode(const float (&x)[4], float 
 }
 
 // The four codes of a word as floats: the biased code lands in the mantissa of 2^23, exactly.
-__device__ __forceinline__ void decode4(uint32_t word, float (&v)[4]) {
+__device__ __forceinline__ void decode4(uint32_t word, Pair &lo, Pair &hi) {
     const uint32_t w = word ^ 0x80808080u;
-    v[0] = __fsub_rn(__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7440)), 8388736.f);
-    v[1] = __fsub_rn(__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7441)), 8388736.f);
-    v[2] = __fsub_rn(__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7442)), 8388736.f);
-    v[3] = __fsub_rn(__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7443)), 8388736.f);
+    const Pair bias = pair(-8388736.f, -8388736.f);
+    lo = add2(pair(__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7440)), __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7441))), bias);
+    hi = add2(pair(__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7442)), __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7443))), bias);
 }
 
 // Quotients of indices below 2^31 by a fixed divisor: floor(i * m / 2^(32 + shift)), with m rounded up.

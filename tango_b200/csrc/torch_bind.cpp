@@ -16,8 +16,6 @@ static Schedule schedule(const py::object &s, bool with_hub) {
     out.present = true;
     out.units = tensor_attr(s, "units");
     out.heavy_rows = tensor_attr(s, "heavy_rows");
-    out.heavy_first = tensor_attr(s, "heavy_first");
-    out.longest = s.attr("longest").cast<int64_t>();
     out.row_order = tensor_attr(s, "row_order");
     if (const py::object info = s.attr("row_info"); !info.is_none()) out.row_info = info.cast<Tensor>();
     out.n_over_few = s.attr("n_over_few").cast<int64_t>();
@@ -57,6 +55,19 @@ static std::shared_ptr<Direction> direction(const py::tuple &bundle, const py::o
     return d;
 }
 
+static EdgeSchedule edge_schedule(const py::object &s) {
+    EdgeSchedule out;
+    out.rows = tensor_attr(s, "rows");
+    out.units = tensor_attr(s, "units");
+    out.heavy_first = tensor_attr(s, "heavy_first");
+    out.n_long = s.attr("n_long").cast<int64_t>();
+    out.n_units = s.attr("n_units").cast<int64_t>();
+    out.n_heavy = s.attr("n_heavy").cast<int64_t>();
+    out.longest = s.attr("longest").cast<int64_t>();
+    out.present = true;
+    return out;
+}
+
 static py::object wrap(const Tensor &t) { return t.defined() ? py::cast(t) : py::none(); }
 
 PYBIND11_MODULE(_torch_ops, m) {
@@ -78,7 +89,12 @@ PYBIND11_MODULE(_torch_ops, m) {
             auto g = std::make_shared<Graph>();
             g->csc = std::move(csc); g->csr = std::move(csr); g->src = std::move(src); g->dst = std::move(dst); g->n_nodes = n;
             return g;
-        }));
+        }))
+        .def("has_edge_schedules", [](const Graph &g) { return g.csc->edge_sched.present && g.csr->edge_sched.present; })
+        .def("set_edge_schedules", [](Graph &g, const py::object &csc, const py::object &csr) {
+            g.csc->edge_sched = edge_schedule(csc);
+            g.csr->edge_sched = edge_schedule(csr);
+        });
 
     m.def("set_rounding", [](int gemm, int quantize, uint64_t seed) {
         settings().mode_gemm = gemm; settings().mode_quantize = quantize; settings().seed = seed;

@@ -47,14 +47,21 @@ inline void count(int64_t n) { settings().launches.fetch_add(n, std::memory_orde
 
 // The row schedule of one index bundle (tango_b200.graph.SpmmSchedule) and its dense hub region, if any.
 struct Schedule {
-    Tensor units, heavy_rows, heavy_first, row_order, row_info;
-    int64_t longest = 0, n_units = 0, n_heavy = 0, n_long = 0, n_block_rows = 0, n_skip = 0, n_over_few = 0, n_over_one = 0;
+    Tensor units, heavy_rows, row_order, row_info;
+    int64_t n_units = 0, n_heavy = 0, n_long = 0, n_block_rows = 0, n_skip = 0, n_over_few = 0, n_over_one = 0;
     int threshold = 0, unit = 0;
     bool present = false;
     // hub region (tango_b200.graph.HubBlock)
     Tensor dense, dense_units, dense_cols;
     int64_t n_tiles = 0, dense_rows = 0;
     bool has_hub = false;
+};
+
+// The row schedule of the edge-attention kernels (tango_b200.graph.EdgeSchedule).
+struct EdgeSchedule {
+    Tensor rows, units, heavy_first;
+    int64_t n_long = 0, n_units = 0, n_heavy = 0, longest = 0;
+    bool present = false;
 };
 
 // One direction of a graph: CSC rows are destinations, CSR rows are sources.
@@ -64,6 +71,7 @@ struct Direction {
     bool has_hub = false;
     Tensor hub_indptr, hub_indices;      // the edges outside the hub region
     Schedule hub_sched;
+    EdgeSchedule edge_sched;             // made at the first call of an operator that takes it
     int64_t n_rows() const { return indptr.numel() - 1; }
 };
 

@@ -28,20 +28,31 @@ static Rows8 alloc_rows8(int64_t rows, int64_t cols, int64_t group, const Tensor
             at::empty({rows, groups}, like.options().dtype(at::kFloat))};
 }
 
-// Up to four matrices of one shape and type in one launch.
-static std::vector<Rows8> pack_all(std::initializer_list<Tensor> tensors, int64_t group) {
+// Up to four matrices of one shape and type in one launch.  paired: the last two become one tensor of codes, interleaved, with
+// their scales in pairs.
+static std::vector<Rows8> pack_all(std::initializer_list<Tensor> tensors, int64_t group, bool paired = false) {
     const Tensor &first = *tensors.begin();
     const c10::cuda::CUDAGuard guard(first.device());
     std::vector<Matrix> x;
     std::vector<Rows8> out;
     tango_rows8_job jobs[4];
-    for (const Tensor &t : tensors) {
-        x.push_back(matrix(t));
-        out.push_back(alloc_rows8(x.back().rows, x.back().cols, group, t));
-        jobs[x.size() - 1] = {ptr(x.back().t), x.back().ld, ptr<int8_t>(out.back().q), ptr<float>(out.back().scale)};
+    for (const Tensor &t : tensors) x.push_back(matrix(t));
+    const size_t apart = x.size() - (paired ? 2 : 0);
+    for (size_t k = 0; k < apart; ++k) {
+        out.push_back(alloc_rows8(x[k].rows, x[k].cols, group, first));
+        jobs[k] = {ptr(x[k].t), x[k].ld, ptr<int8_t>(out[k].q), ptr<float>(out[k].scale), 1, 0};
+    }
+    if (paired) {
+        const int64_t groups = (x[0].cols + group - 1) / group, run = tango_rows8_run(group);
+        const Rows8 both{at::empty({x[0].rows, 2 * tango_rows8_ld(x[0].cols, group)}, first.options().dtype(at::kChar)),
+                         at::empty({x[0].rows, groups, 2}, first.options().dtype(at::kFloat))};
+        out.push_back(both);
+        for (size_t k = apart; k < x.size(); ++k)
+            jobs[k] = {ptr(x[k].t), x[k].ld, ptr<int8_t>(both.q) ? ptr<int8_t>(both.q) + (k - apart) * run : nullptr,
+                       ptr<float>(both.scale) ? ptr<float>(both.scale) + (k - apart) : nullptr, 2, 1};
     }
     if (x[0].rows == 0 || x[0].cols == 0) return out;
-    const int mode = settings().mode_quantize, n = (int)out.size();
+    const int mode = settings().mode_quantize, n = (int)x.size();
     const uint64_t call = mode == TANGO_ROUND_STOCHASTIC ? next_call() : 0;
     for (int k = 1; k < n && call; ++k) next_call();
     check(tango_rows8_pack(jobs, n, x[0].rows, x[0].cols, group, type_code(first), mode, settings().seed, call, settings().step,
@@ -113,7 +124,7 @@ Tensor activation8_fn(const Tensor &x_, int act, int64_t group) {
         if (y.numel() > 0) {
             const int mode = settings().mode_quantize;
             const uint64_t call = saves && mode == TANGO_ROUND_STOCHASTIC ? next_call() : 0;
-            const tango_rows8_job job{ptr(x.t), x.ld, ptr<int8_t>(copy.q), ptr<float>(copy.scale)};
+            const tango_rows8_job job{ptr(x.t), x.ld, ptr<int8_t>(copy.q), ptr<float>(copy.scale), 1, 0};
             check(tango_act8_forward(act, &job, x.rows, x.cols, group, type_code(x_), ptr(y), x.cols, mode, settings().seed, call,
                                      settings().step, cuda_stream()), "activation8");
             count(1);
@@ -137,15 +148,14 @@ struct EdgePlan {
     int64_t bytes() const { return ws.defined() ? ws.numel() : 0; }
     int launches() const { return p.n_heavy > 0 ? 2 : 1; }
 };
-static EdgePlan edge_plan(const Schedule &s, int pass, int heads, int d, const Tensor &like) {
+static EdgePlan edge_plan(const EdgeSchedule &s, int pass, int heads, int d, const Tensor &like) {
     EdgePlan plan;
-    plan.present = s.present && s.row_order.numel() > 0;
+    plan.present = s.present;
     if (!plan.present) return plan;
-    plan.p.row_order = ptr<int32_t>(s.row_order);
-    plan.p.n_long_rows = s.n_long;
+    plan.p.rows = ptr<int32_t>(s.rows); plan.p.n_long = s.n_long;
     if (s.n_heavy == 0) return plan;
     plan.p.units = ptr<int32_t>(s.units); plan.p.n_units = s.n_units;
-    plan.p.heavy_rows = ptr<int32_t>(s.heavy_rows); plan.p.heavy_first = ptr<int32_t>(s.heavy_first); plan.p.n_heavy = s.n_heavy;
+    plan.p.heavy_first = ptr<int32_t>(s.heavy_first); plan.p.n_heavy = s.n_heavy;
     plan.ws = at::empty({tango_edge_attention_workspace_bytes(pass, s.n_units, heads, d)}, like.options().dtype(at::kByte));
     return plan;
 }
@@ -163,30 +173,36 @@ struct EdgeAttentionBackward : SavingNode {
         if (!grads[0].defined()) return variable_list(3);
         const Tensor grad = grads[0].to(type);
         const c10::cuda::CUDAGuard guard(grad.device());
-        const Rows8 q8{k[0].contiguous(), numbers(k[3])}, k8{k[1].contiguous(), numbers(k[4])}, v8{k[2].contiguous(), numbers(k[5])};
-        const Tensor stats = numbers(k[6]);
+        const Tensor q8 = k[0].contiguous(), kv8 = k[1].contiguous();
+        const Tensor sq = numbers(k[2]), skv = numbers(k[3]), stats = numbers(k[4]);
         const int64_t n = g->n_nodes;
         const auto out = [&] { return at::empty({n, heads, d}, grad.options()); };
         const Tensor dq = out();
         if (n == 0) return {dq, out(), out()};
         const Rows8 o8 = pack_all({grad}, d)[0];
-        const Tensor record = at::empty({n, heads, 4}, grad.options().dtype(at::kFloat));
-        const tango_rows8 q = view(q8), key = view(k8), v = view(v8), o = view(o8);
+        const bool sources = needs(1) || needs(2);
+        Tensor record, qo8;       // what the second pass reads of a destination
+        if (sources) {
+            record = at::empty({n, heads, 4}, grad.options().dtype(at::kFloat));
+            qo8 = at::empty_like(kv8);
+        }
+        tango_edge_operands x{ptr<int8_t>(q8), ptr<int8_t>(kv8), ptr<int8_t>(o8.q), ptr<float>(sq), ptr<float>(skv),
+                              ptr<float>(o8.scale)};
         const int code = type_code(grad);
         {
             const Direction &in = g->dir(false);
-            const EdgePlan plan = edge_plan(in.sched, 1, heads, d, grad);
-            check(tango_edge_attention_bwd_dst(ptr<int32_t>(in.indptr), index_ptr(in), n, plan.get(), heads, d, &q, &key, &v, &o, scale,
-                                               ptr<float>(stats), ptr(dq), code, ptr<float>(record), ptr(plan.ws), plan.bytes(),
-                                               cuda_stream()), "edge_attention_bwd_dst");
+            const EdgePlan plan = edge_plan(in.edge_sched, 1, heads, d, grad);
+            check(tango_edge_attention_bwd_dst(ptr<int32_t>(in.indptr), index_ptr(in), n, plan.get(), heads, d, &x, scale,
+                                               ptr<float>(stats), ptr(dq), code, ptr<float>(record), ptr<int8_t>(qo8), ptr(plan.ws),
+                                               plan.bytes(), cuda_stream()), "edge_attention_bwd_dst");
             count(plan.launches());
         }
-        if (!needs(1) && !needs(2)) return {dq, Tensor(), Tensor()};
+        if (!sources) return {dq, Tensor(), Tensor()};
         const Tensor dk = out(), dv = out();
         const Direction &from = g->dir(true);
-        const EdgePlan plan = edge_plan(from.sched, 2, heads, d, grad);
-        check(tango_edge_attention_bwd_src(ptr<int32_t>(from.indptr), index_ptr(from), n, plan.get(), heads, d, &q, &key, &v, &o,
-                                           ptr<float>(record), ptr(dk), ptr(dv), code, ptr(plan.ws), plan.bytes(), cuda_stream()),
+        const EdgePlan plan = edge_plan(from.edge_sched, 2, heads, d, grad);
+        check(tango_edge_attention_bwd_src(ptr<int32_t>(from.indptr), index_ptr(from), n, plan.get(), heads, d, ptr<int8_t>(kv8),
+                                           ptr<float>(skv), ptr<int8_t>(qo8), ptr<float>(record), ptr(dk), ptr(dv), code, ptr(plan.ws), plan.bytes(), cuda_stream()),
               "edge_attention_bwd_src");
         count(plan.launches());
         return {needs(0) ? dq : Tensor(), needs(1) ? dk : Tensor(), needs(2) ? dv : Tensor()};
@@ -216,14 +232,15 @@ Tensor edge_attention_fn(const GraphPtr &g, const Tensor &q, const Tensor &k, co
         const Raw raw;
         const c10::cuda::CUDAGuard guard(q.device());
         out = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
-        r = pack_all({q, k, v}, d);
+        r = pack_all({q, k, v}, d, true);
         if (saves) stats = floats({q.size(0), heads, 2}, q);
         if (q.size(0) > 0) {
             const Direction &in = g->dir(false);
-            const EdgePlan plan = edge_plan(in.sched, 0, heads, d, q);
-            const tango_rows8 q8 = view(r[0]), k8 = view(r[1]), v8 = view(r[2]);
-            check(tango_edge_attention(ptr<int32_t>(in.indptr), index_ptr(in), q.size(0), plan.get(), heads, d, &q8, &k8, &v8, (float)scale,
-                                       ptr(out), type_code(q), ptr<float>(stats), ptr(plan.ws), plan.bytes(), cuda_stream()),
+            const EdgePlan plan = edge_plan(in.edge_sched, 0, heads, d, q);
+            const tango_edge_operands x{ptr<int8_t>(r[0].q), ptr<int8_t>(r[1].q), nullptr, ptr<float>(r[0].scale),
+                                        ptr<float>(r[1].scale), nullptr};
+            check(tango_edge_attention(ptr<int32_t>(in.indptr), index_ptr(in), q.size(0), plan.get(), heads, d, &x, (float)scale, ptr(out),
+                                       type_code(q), ptr<float>(stats), ptr(plan.ws), plan.bytes(), cuda_stream()),
                   "edge_attention");
             count(plan.launches());
         }
@@ -231,7 +248,7 @@ Tensor edge_attention_fn(const GraphPtr &g, const Tensor &q, const Tensor &k, co
     if (auto node = make_node<EdgeAttentionBackward>(q, k, v)) {
         node->g = g; node->heads = heads; node->d = d; node->scale = (float)scale; node->type = q.scalar_type();
         torch::autograd::set_history(out, node);
-        node->keep({r[0].q, r[1].q, r[2].q, bytes(r[0].scale), bytes(r[1].scale), bytes(r[2].scale), bytes(stats)});
+        node->keep({r[0].q, r[1].q, bytes(r[0].scale), bytes(r[1].scale), bytes(stats)});
     }
     return out;
 }
@@ -257,7 +274,7 @@ Tensor edge_attention_rows(const GraphPtr &g, const Tensor &rows_, const Tensor 
     const Tensor rows = rows_.to(at::kLong).contiguous();
     const Matrix qm = matrix(q);
     const Direction &in = g->dir(false);
-    const int splits = tango_edge_attention_rows_splits(r, in.sched.present ? in.sched.longest : g->n_edges());
+    const int splits = tango_edge_attention_rows_splits(r, in.edge_sched.present ? in.edge_sched.longest : g->n_edges());
     const int64_t bytes = tango_edge_attention_rows_workspace_bytes(r, splits, (int)heads, (int)d);
     if (bytes < 0) check((int)bytes, "edge_attention_rows");
     const Tensor ws = at::empty({bytes}, q.options().dtype(at::kByte));

@@ -257,11 +257,9 @@ class SpmmSchedule:
 
     force_heavy (optional, nseg == 1): row ids that are finished through the int32 scratch whatever their length (the
     rows of a dense hub block, in the block's row order); they come first in `heavy_rows`, every heavy row comes
-    first in `row_order`, and `n_skip` = n_heavy tells the row kernels to start after them.
+    first in `row_order`, and `n_skip` = n_heavy tells the row kernels to start after them."""
 
-    `heavy_first` [n_heavy * nseg + 1]: the first unit of every heavy segment row; `longest`: slots of the longest row."""
-
-    LAYOUT = 4      # counts up when the fields or their meaning change: see Graph.__setstate__
+    LAYOUT = 3      # counts up when the fields or their meaning change: see Graph.__setstate__
 
     def __init__(self, indptr: torch.Tensor, nseg: int = 1, threshold: Optional[int] = None,
                  unit: Optional[int] = None, force_heavy: Optional[torch.Tensor] = None):
@@ -317,12 +315,10 @@ class SpmmSchedule:
         # Rows that deserve a whole CTA in row-team kernels.  The line is the same for every graph: the order in which a row's
         # softmax terms are added depends on it.
         self.n_block_rows = int((row_deg > BLOCK_ROW_NNZ).sum())
-        self.longest = int(row_deg.max()) if n_rows else 0
         self.n_heavy = int(heavy.numel())
         self.heavy_rows = heavy.to(torch.int32)
         if self.n_heavy == 0:
             self.units = torch.zeros((0, 4), dtype=torch.int32, device=indptr.device)
-            self.heavy_first = torch.zeros(1, dtype=torch.int32, device=indptr.device)
             self.n_units = 0
             return
         # segment rows of the heavy rows, their scratch slots, and the slices of each
@@ -331,15 +327,51 @@ class SpmmSchedule:
         beg, end = ip[seg_rows], ip[seg_rows + 1]
         n_chunks = (end - beg + unit - 1) // unit
         rep = torch.repeat_interleave(torch.arange(seg_rows.numel(), device=indptr.device), n_chunks)
-        last = torch.cumsum(n_chunks, 0)
-        first = last - n_chunks
-        self.heavy_first = torch.cat([first[:1], last]).to(torch.int32)
+        first = torch.cumsum(n_chunks, 0) - n_chunks
         k = torch.arange(rep.numel(), device=indptr.device) - first[rep]
         ub = beg[rep] + k * unit
         ue = torch.minimum(ub + unit, end[rep])
         units = torch.stack([seg_rows[rep], ub, ue, slots[rep]], dim=1)
         # longest slices first
         self.units = units.to(torch.int32).contiguous()
+        self.n_units = int(self.units.shape[0])
+
+
+class EdgeSchedule:
+    """The rows of one direction of a graph as the edge-attention kernels take them, by decreasing length: `rows` [N, 4] int32 =
+    (row, first slot, end slot, 0); the first `n_heavy` are cut into `units` [n_units, 4] = (row, first slot, end slot, place of
+    the unit in its row), those of the i-th being units heavy_first[i] .. heavy_first[i + 1]; rows up to `n_long` get a warp, the
+    rest a part of one.  `longest`: slots of the longest row.
+
+    Both limits follow the number of edges.  A part of a warp wastes fewer slots at a row's end and merges less than a warp
+    does, but walks the row alone: on 20 M edges rows of up to 512 by parts of a warp took 631 us forward against 737 with up to
+    48 (head of the row order first, so that the walk of the longest is hidden), on 1.2 M edges 160 to 200 us against 96 with
+    up to 160.  Units keep the longest walk short on small graphs (128 edges) and their partial results few on large ones."""
+
+    def __init__(self, indptr: torch.Tensor):
+        ip = indptr.long()
+        length = ip[1:] - ip[:-1]
+        n, dev = length.numel(), indptr.device
+        order = torch.argsort(length, descending=True, stable=True)
+        nnz = int(ip[-1]) if n else 0
+        team = min(512, max(48, nnz // 8192))
+        unit = 128
+        while unit < 1024 and unit * 16384 < nnz:
+            unit *= 2
+        self.threshold = 2 * unit
+        self.rows = torch.stack([order, ip[:-1][order], ip[1:][order], torch.zeros_like(order)], 1).to(torch.int32).contiguous()
+        counts = torch.stack([(length > team).sum(), (length > self.threshold).sum(),
+                              length.max() if n else torch.zeros((), dtype=torch.int64, device=dev)]).tolist()
+        self.n_heavy, self.longest = counts[1], counts[2]
+        self.n_long = max(counts[0], self.n_heavy)
+        heavy = order[:self.n_heavy]
+        n_units = (length[heavy] + unit - 1) // unit
+        last = torch.cumsum(n_units, 0)
+        self.heavy_first = torch.cat([torch.zeros(1, dtype=torch.int64, device=dev), last]).to(torch.int32)
+        of = torch.repeat_interleave(torch.arange(self.n_heavy, device=dev), n_units)
+        place = torch.arange(of.numel(), device=dev) - (last - n_units)[of]
+        begin = ip[heavy[of]] + place * unit
+        self.units = torch.stack([heavy[of], begin, torch.minimum(begin + unit, ip[heavy[of] + 1]), place], 1).to(torch.int32).contiguous()
         self.n_units = int(self.units.shape[0])
 
 

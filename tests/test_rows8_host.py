@@ -1,5 +1,5 @@
 """8-bit rows and edge attention without a GPU: layouts, refusals before any launch, the C entry points' error codes, and the
-row schedule's unit index."""
+row schedule."""
 import ctypes
 import math
 
@@ -20,16 +20,21 @@ def test_layout(cols, group, pitch, ld):
 
 
 class _Job(ctypes.Structure):
-    _fields_ = [("x", ctypes.c_void_p), ("ldx", ctypes.c_int64), ("q", ctypes.c_void_p), ("scales", ctypes.c_void_p)]
+    _fields_ = [("x", ctypes.c_void_p), ("ldx", ctypes.c_int64), ("q", ctypes.c_void_p), ("scales", ctypes.c_void_p),
+                ("scale_stride", ctypes.c_int64), ("interleaved", ctypes.c_int)]
 
 
 class _Rows(ctypes.Structure):
     _fields_ = [("q", ctypes.c_void_p), ("scales", ctypes.c_void_p)]
 
 
+class _Operands(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("q", "kv", "o", "sq", "skv", "so")]
+
+
 class _Plan(ctypes.Structure):
-    _fields_ = [("row_order", ctypes.c_void_p), ("n_long", ctypes.c_int64), ("units", ctypes.c_void_p), ("n_units", ctypes.c_int64),
-                ("heavy_rows", ctypes.c_void_p), ("heavy_first", ctypes.c_void_p), ("n_heavy", ctypes.c_int64)]
+    _fields_ = [("rows", ctypes.c_void_p), ("n_long", ctypes.c_int64), ("units", ctypes.c_void_p), ("n_units", ctypes.c_int64),
+                ("heavy_first", ctypes.c_void_p), ("n_heavy", ctypes.c_int64)]
 
 
 def _ref(x):
@@ -38,21 +43,22 @@ def _ref(x):
 
 def test_pack_arguments_are_checked_before_any_launch():
     lib = _lib()
-    ok = _Job(0x1000, 16, 0x2000, 0x3000)
+    ok = _Job(0x1000, 16, 0x2000, 0x3000, 1, 0)
 
     def pack(job=ok, n=1, rows=4, cols=16, group=16, kind=0, mode=1):
         return lib.tango_rows8_pack(_ref(job), n, rows, cols, group, kind, mode, 0, 0, None, None)
 
     assert pack(n=0) == -1 and pack(n=5) == -1 and pack(rows=-1) == -1 and pack(group=0) == -1 and pack(kind=3) == -1
     assert pack(mode=3) == -1 and pack(group=1025) == -5
-    assert pack(job=_Job(0x1000, 8, 0x2000, 0x3000)) == -1           # leading dimension below the width
-    assert pack(job=_Job(None, 16, 0x2000, 0x3000)) == -1
-    assert pack(job=_Job(0x1002, 16, 0x2000, 0x3000)) == -2 and pack(job=_Job(0x1000, 16, 0x2002, 0x3000)) == -2
+    assert pack(job=_Job(0x1000, 8, 0x2000, 0x3000, 1, 0)) == -1           # leading dimension below the width
+    assert pack(job=_Job(None, 16, 0x2000, 0x3000, 1, 0)) == -1
+    assert pack(job=_Job(0x1002, 16, 0x2000, 0x3000, 1, 0)) == -2 and pack(job=_Job(0x1000, 16, 0x2002, 0x3000, 1, 0)) == -2
+    assert pack(job=_Job(0x1000, 16, 0x2000, 0x3000, 0, 0)) == -1
     assert pack(rows=0) == 0 and pack(cols=0) == 0
     assert lib.tango_rows8_unpack(None, None, 4, 4, 4, 0, None, 4, None) == -1
     assert lib.tango_rows8_unpack(0x1000, 0x2000, 4, 4, 4, 0, 0x3000, 2, None) == -1
     assert lib.tango_act8_forward(3, _ref(ok), 4, 16, 16, 0, 0x4000, 16, 1, 0, 0, None, None) == -1
-    half = _Job(0x1000, 16, None, 0x3000)                            # codes without scales or the reverse
+    half = _Job(0x1000, 16, None, 0x3000, 1, 0)                            # codes without scales or the reverse
     assert lib.tango_act8_forward(0, _ref(half), 4, 16, 16, 0, 0x4000, 16, 1, 0, 0, None, None) == -1
     assert lib.tango_act8_backward(-1, 0x1000, 0x2000, 4, 16, 16, 0, 0x3000, 16, 0x4000, 16, None) == -1
     assert lib.tango_act8_backward(0, 0x1000, 0x2000, 4, 16, 16, 0, 0x3000, 8, 0x4000, 16, None) == -1
@@ -62,22 +68,36 @@ def test_attention_arguments_are_checked_before_any_launch():
     lib = _lib()
     r = _Rows(0x1000, 0x2000)
 
-    def forward(rows=4, heads=2, d=16, kind=0, q=r, k=r, out=0x3000, plan=None, ws=None, nbytes=0):
-        return lib.tango_edge_attention(0x100, 0x200, rows, plan, heads, d, _ref(q), _ref(k), _ref(r), 1.0, out, kind, None, ws, nbytes, None)
+    kept = []
+
+    def x(q=0x1000, kv=0x1000, o=0x1000, skv=0x2000):
+        kept.append(_Operands(q, kv, o, 0x2000, skv, 0x2000))
+        return _ref(kept[-1])
+
+    def forward(rows=4, heads=2, d=16, kind=0, x=x(o=None), out=0x3000, plan=None, ws=None, nbytes=0):
+        return lib.tango_edge_attention(0x100, 0x200, rows, plan, heads, d, x, 1.0, out, kind, None, ws, nbytes, None)
 
     assert forward(rows=-1) == -1 and forward(heads=0) == -1 and forward(d=0) == -1 and forward(kind=7) == -1
     assert forward(d=513) == -5 and forward(heads=70000) == -5 and forward(rows=1 << 31) == -5
     assert forward(rows=0) == 0
-    assert forward(q=_Rows(None, 0x2000)) == -1 and forward(k=_Rows(0x1008, 0x2000)) == -1 and forward(out=0x3004) == -2
+    assert forward(x=x(q=None)) == -1 and forward(x=x(kv=None)) == -1 and forward(x=x(q=0x1008)) == -1 and forward(x=x(skv=None)) == -1 and forward(x=None) == -1
+    assert forward(out=0x3004) == -2 and forward(x=x(skv=0x2004)) == -2 and forward(x=x(kv=0x1010)) == -2
     # long rows without a workspace that holds their units, and schedules that contradict themselves
-    plan = _Plan(0x10, 2, 0x20, 3, 0x30, 0x40, 1)
+    plan = _Plan(0x10, 2, 0x20, 3, 0x40, 1)
     assert forward(plan=_ref(plan)) == -1 and forward(plan=_ref(plan), ws=0x1000, nbytes=16) == -1
-    assert forward(plan=_ref(_Plan(0x10, 0, 0x20, 3, 0x30, 0x40, 1)), ws=0x1000, nbytes=1 << 20) == -1
-    assert forward(plan=_ref(_Plan(0x10, 5, 0x20, 0, 0x30, 0x40, 0))) == -1
-    assert lib.tango_edge_attention_bwd_dst(0x100, 0x200, 4, None, 2, 16, _ref(r), _ref(r), _ref(r), _ref(r), 1.0, None, 0x3000, 0, 0x4000,
-                                            None, 0, None) == -1
-    assert lib.tango_edge_attention_bwd_src(0x100, 0x200, 4, None, 2, 16, _ref(r), _ref(r), _ref(r), _ref(r), None, 0x3000, 0x3000, 0, None,
-                                            0, None) == -1
+    assert forward(plan=_ref(_Plan(0x10, 0, 0x20, 3, 0x40, 1)), ws=0x1000, nbytes=1 << 20) == -1
+    assert forward(plan=_ref(_Plan(0x10, 5, 0x20, 0, 0x40, 0))) == -1
+    assert forward(plan=_ref(_Plan(None, 2, None, 0, None, 0))) == -1 and forward(plan=_ref(_Plan(0x18, 2, None, 0, None, 0))) == -2
+    def by_dst(x=x(), stats=0x4000, record=0x4000, qo=0x6000):
+        return lib.tango_edge_attention_bwd_dst(0x100, 0x200, 4, None, 2, 16, x, 1.0, stats, 0x3000, 0, record, qo, None, 0, None)
+
+    def by_src(kv=0x1000, skv=0x2000, qo=0x6000, record=0x4000):
+        return lib.tango_edge_attention_bwd_src(0x100, 0x200, 4, None, 2, 16, kv, skv, qo, record, 0x3000, 0x3000, 0, None, 0, None)
+
+    assert by_dst(x(o=None)) == -1 and by_dst(stats=None) == -1 and by_dst(stats=0x4004) == -2 and by_dst(qo=0x6010) == -2
+    assert by_dst(record=None) == -1 and by_dst(qo=None) == -1
+    assert by_src(kv=None) == -1 and by_src(qo=None) == -1 and by_src(record=None) == -1 and by_src(record=0x4008) == -2
+    assert by_src(kv=0x1010) == -2 and by_src(skv=0x2004) == -2
     assert lib.tango_edge_attention_workspace_bytes(0, 3, 2, 16) == 3 * (4 + 32) * 4
     assert lib.tango_edge_attention_workspace_bytes(1, 3, 2, 41) == 3 * (4 + 2 * 96) * 4
     assert lib.tango_edge_attention_workspace_bytes(2, 3, 3, 8) == 3 * (2 * 24) * 4
@@ -147,27 +167,31 @@ def test_activations_that_have_an_8_bit_form():
         GAT(None, 2, 8, 4, 3, [2, 1], activation=F.relu, checkpoint="int8")
 
 
-@pytest.mark.parametrize("nseg", [1, 3])
-def test_units_of_every_long_row_are_found_by_its_place(nseg):
-    from tango_b200.graph import SpmmSchedule
-    lengths = torch.tensor([0, 700, 5, 513, 512, 1, 3000] * nseg)
+@pytest.mark.parametrize("scale", [1, 3000])
+def test_units_cover_every_long_row_once(scale):
+    """Also with enough edges for the limits to grow (lengths alone: the schedule reads nothing else)."""
+    from tango_b200.graph import EdgeSchedule
+    lengths = torch.tensor([0, 700, 5, 257, 256, 1, 3000, 0, 130, 49, 48]) * scale
     indptr = torch.zeros(lengths.numel() + 1, dtype=torch.int32)
     indptr[1:] = lengths.cumsum(0)
-    s = SpmmSchedule(indptr, nseg=nseg, threshold=512, unit=256)
-    rows = lengths.view(-1, nseg).sum(1)
-    assert s.longest == int(rows.max())
-    assert s.heavy_first.dtype == torch.int32 and s.heavy_first.numel() == s.n_heavy * nseg + 1
+    s = EdgeSchedule(indptr)
+    assert s.longest == 3000 * scale
+    rows = s.rows.long()
+    length = rows[:, 2] - rows[:, 1]
+    assert torch.equal(rows[:, 0].sort().values, torch.arange(11)) and (length.diff() <= 0).all()
+    assert torch.equal(rows[:, 1], indptr.long()[rows[:, 0]]) and torch.equal(length, lengths[rows[:, 0]])
+    assert s.n_heavy == int((lengths > s.threshold).sum()) <= s.n_long <= 11
+    assert (length[:s.n_long] > 48).all()
     first = s.heavy_first.tolist()
-    assert first[0] == 0 and first[-1] == s.n_units
-    for i, row in enumerate(s.heavy_rows.tolist()):
-        for k in range(nseg):
-            units = s.units[first[i * nseg + k]:first[i * nseg + k + 1]]
-            seg = row * nseg + k
-            covered = torch.cat([torch.arange(b, e) for _, b, e, _ in units.tolist()]) if len(units) else torch.arange(0)
-            assert (units[:, 0] == seg).all() and torch.equal(covered, torch.arange(int(indptr[seg]), int(indptr[seg + 1])))
-    none = SpmmSchedule(torch.tensor([0, 3, 4], dtype=torch.int32))
-    assert none.heavy_first.tolist() == [0] and none.longest == 3
-    assert SpmmSchedule(torch.tensor([0], dtype=torch.int32)).longest == 0
+    assert s.heavy_first.dtype == torch.int32 and first[0] == 0 and first[-1] == s.n_units and len(first) == s.n_heavy + 1
+    for i in range(s.n_heavy):
+        units = s.units[first[i]:first[i + 1]].tolist()
+        assert [u[3] for u in units] == list(range(len(units))) and all(u[0] == int(rows[i, 0]) for u in units)
+        assert units[0][1] == int(rows[i, 1]) and units[-1][2] == int(rows[i, 2])
+        assert all(a[2] == b[1] and a[2] > a[1] for a, b in zip(units, units[1:]))
+    for none in (torch.tensor([0, 3, 4], dtype=torch.int32), torch.tensor([0], dtype=torch.int32)):
+        s = EdgeSchedule(none)
+        assert s.heavy_first.tolist() == [0] and s.n_units == s.n_heavy == 0 and s.rows.shape == (none.numel() - 1, 4)
 
 
 def test_quotients_without_division_are_exact():
