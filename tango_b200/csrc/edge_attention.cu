@@ -543,24 +543,26 @@ __host__ __device__ inline int row_chunk(int len, int splits) {
 template <int VB, int P, class T>
 __device__ __forceinline__ Codes<VB> encode_query(const RowsArgs &a, int64_t r, int head, int chunk, bool live, float &s) {
     const int64_t at = r * a.ldq + (int64_t)head * a.d + chunk * VB;
-    float v[VB / 4][4], top = 0.f;
+    float v[VB], top = 0.f;
 #pragma unroll
     for (int i = 0; i < VB / 4; ++i) {
-        load4<T, 1>(static_cast<const T *>(a.q) + at + 4 * i, live ? min(4, a.d - chunk * VB - 4 * i) : 0, v[i]);
+        load4<T, 1>(static_cast<const T *>(a.q) + at + 4 * i, live ? min(4, a.d - chunk * VB - 4 * i) : 0, v + 4 * i);
 #pragma unroll
-        for (int k = 0; k < 4; k += 2) top = max_abs3(v[i][k], v[i][k + 1], top);
+        for (int k = 4 * i; k < 4 * i + 4; k += 2) top = max_abs3(v[k], v[k + 1], top);
     }
 #pragma unroll
     for (int o = P / 2; o > 0; o >>= 1) top = max_or_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
     s = group_scale(top);
     const float inv = group_inverse(s);
     Codes<VB> c;
+    if (a.mode == TANGO_ROUND_NEAREST) {
+        encode_nearest<VB / 4>(v, s, inv, c.w);
+    } else {
 #pragma unroll
-    for (int i = 0; i < VB / 4; ++i)
-        c.w[i] = a.mode == TANGO_ROUND_NEAREST
-                     ? encode4(v[i], s, inv)
-                     : encode4_mode(v[i], s, a.mode, a.seed, effective_call(a.call, a.step),
-                                    (uint64_t)r * a.heads * a.d + head * a.d + chunk * VB + 4 * i);
+        for (int i = 0; i < VB / 4; ++i)
+            c.w[i] = encode4_mode(v + 4 * i, s, a.mode, a.seed, effective_call(a.call, a.step),
+                                  (uint64_t)r * a.heads * a.d + head * a.d + chunk * VB + 4 * i);
+    }
     return c;
 }
 

@@ -57,30 +57,43 @@ __device__ __forceinline__ float group_scale(float top) {
 // About 1 / s; 0 for the scales 0 and NaN.
 __device__ __forceinline__ float group_inverse(float s) { return s > 0.f ? __fdividef(1.0f, s) : 0.f; }
 
-// Four codes: x / s exactly rounded, ties to even.  x * inv is within 127 * 2^-21 of the quotient, which decides all but the
-// values that close to a border between two codes.  For those x - q * s is exact in one fused operation (a multiple of half
+// N codes: x / s exactly rounded, ties to even.  x * inv is within 127 * 2^-21 of the quotient, which decides all but
+// the values that close to a border between two codes.  For those x - q * s is exact in one fused operation (a multiple of half
 // an ulp of s, at most about s / 2), and its double is compared with s.
-__device__ __forceinline__ uint32_t encode4(const float (&x)[4], float s, float inv) {
+// The codes come as floats whose bits hold them in the low byte.
+template <int N>
+__device__ __forceinline__ void round_nearest(const float *x, float s, float inv, float *b) {
     const Pair by = pair(inv, inv), magic = pair(kRoundMagic, kRoundMagic), minus = pair(-1.f, -1.f);
-    const Pair x0 = pair(x[0], x[1]), x1 = pair(x[2], x[3]);
-    const Pair b0 = fma2(x0, by, magic), b1 = fma2(x1, by, magic);
-    const float2 d0 = both(fma2(x0, by, fma2(b0, minus, magic))), d1 = both(fma2(x1, by, fma2(b1, minus, magic)));
-    const float2 c0 = both(b0), c1 = both(b1);
-    float b[4] = {c0.x, c0.y, c1.x, c1.y};
-    if (max_abs3(max_abs3(d0.x, d0.y, d1.x), d1.y, 0.f) > 0.4999f) {
+    float far = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float r = fmaf(__fsub_rn(kRoundMagic, b[i]), s, x[i]), twice = 2.f * fabsf(r);
-            if (twice > s || (twice == s && (__float_as_int(b[i]) & 1))) b[i] = __fadd_rn(b[i], r > 0.f ? 1.f : -1.f);
+    for (int k = 0; k < N; k += 2) {
+        const Pair v = pair(x[k], x[k + 1]), c = fma2(v, by, magic);
+        const float2 d = both(fma2(v, by, fma2(c, minus, magic))), f = both(c);
+        far = max_abs3(d.x, d.y, far);
+        b[k] = f.x; b[k + 1] = f.y;
+    }
+    if (far > 0.4999f) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const float rest = fmaf(__fsub_rn(kRoundMagic, b[k]), s, x[k]), twice = 2.f * fabsf(rest);
+            if (twice > s || (twice == s && (__float_as_int(b[k]) & 1))) b[k] = __fadd_rn(b[k], rest > 0.f ? 1.f : -1.f);
         }
     }
-    const uint32_t lo = __byte_perm(__float_as_uint(b[0]), __float_as_uint(b[1]), 0x0040);
-    const uint32_t hi = __byte_perm(__float_as_uint(b[2]), __float_as_uint(b[3]), 0x0040);
-    return inv == 0.f ? 0u : __byte_perm(lo, hi, 0x5410);
+}
+template <int R>
+__device__ __forceinline__ void encode_nearest(const float *x, float s, float inv, uint32_t *word) {
+    float b[R * 4];
+    round_nearest<R * 4>(x, s, inv, b);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const uint32_t lo = __byte_perm(__float_as_uint(b[4 * r]), __float_as_uint(b[4 * r + 1]), 0x0040);
+        const uint32_t hi = __byte_perm(__float_as_uint(b[4 * r + 2]), __float_as_uint(b[4 * r + 3]), 0x0040);
+        word[r] = inv == 0.f ? 0u : __byte_perm(lo, hi, 0x5410);
+    }
 }
 
-// The other rounding modes: truncation, and the seeded stochastic stream keyed by the element's flat index.
-static __device__ __noinline__ uint32_t encode4_mode(const float (&x)[4], float s, int mode, uint64_t seed, uint64_t call, uint64_t flat) {
+// The other rounding modes: truncation, and the seeded stochastic stream keyed by the elements' flat indices.
+static __device__ __noinline__ uint32_t encode4_mode(const float *x, float s, int mode, uint64_t seed, uint64_t call, uint64_t flat) {
     if (!(s > 0.f)) return 0u;
     const Philox ph{(uint32_t)seed, (uint32_t)(seed >> 32)};
     uint64_t blk = ~0ull;
@@ -100,6 +113,15 @@ __device__ __forceinline__ void decode4(uint32_t word, Pair &lo, Pair &hi) {
     const Pair bias = pair(-8388736.f, -8388736.f);
     lo = add2(pair(__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7440)), __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7441))), bias);
     hi = add2(pair(__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7442)), __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7443))), bias);
+}
+
+// One element of the same.
+static __device__ __noinline__ int encode_mode(float x, float s, int mode, uint64_t seed, uint64_t call, uint64_t flat) {
+    if (!(s > 0.f)) return 0;
+    const Philox ph{(uint32_t)seed, (uint32_t)(seed >> 32)};
+    uint64_t blk = ~0ull;
+    uint4 rnd = make_uint4(0, 0, 0, 0);
+    return round_to_i8(__fdiv_rn(x, s), mode, mode == TANGO_ROUND_STOCHASTIC ? sr_uniform(ph, flat, call, blk, rnd) : 0.f);
 }
 
 // Quotients of indices below 2^31 by a fixed divisor: floor(i * m / 2^(32 + shift)), with m rounded up.
@@ -142,41 +164,32 @@ template <class T, int VL> union Pack {
 };
 // Four neighbouring elements, of which the first n exist (the others read as 0).
 template <class T, int VL>
-__device__ __forceinline__ void load4(const T *p, int n, float (&v)[4]) {
-    if (n >= 4) {
+__device__ __forceinline__ void load4(const T *p, int n, float *v) {
 #pragma unroll
-        for (int i = 0; i < 4; i += VL) {
-            Pack<T, VL> k;
+    for (int i = 0; i < 4; i += VL) {
+        Pack<T, VL> k;
+        k.w = {};
+        if (i + VL <= n) {
             k.w = __ldg(reinterpret_cast<const typename Word<VL * sizeof(T)>::T *>(p + i));
-#pragma unroll
-            for (int j = 0; j < VL; ++j) v[i + j] = to_float(k.e[j]);
+        } else if (VL > 1 && i < n) {
+            for (int j = 0; j < VL - 1 && i + j < n; ++j) k.e[j] = p[i + j];
         }
-    } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            v[i] = 0.f;
-            if (i < n) {
-                Pack<T, 1> k;
-                k.w = __ldg(reinterpret_cast<const typename Word<sizeof(T)>::T *>(p + i));
-                v[i] = to_float(k.e[0]);
-            }
-        }
+        for (int j = 0; j < VL; ++j) v[i + j] = to_float(k.e[j]);
     }
 }
 template <class T, int VL>
-__device__ __forceinline__ void store4(T *p, int n, const float (&v)[4]) {
-    if (n >= 4) {
+__device__ __forceinline__ void store4(T *p, int n, const float *v) {
 #pragma unroll
-        for (int i = 0; i < 4; i += VL) {
-            Pack<T, VL> k;
+    for (int i = 0; i < 4; i += VL) {
+        Pack<T, VL> k;
 #pragma unroll
-            for (int j = 0; j < VL; ++j) from_float(v[i + j], k.e[j]);
+        for (int j = 0; j < VL; ++j) from_float(v[i + j], k.e[j]);
+        if (i + VL <= n) {
             *reinterpret_cast<typename Word<VL * sizeof(T)>::T *>(p + i) = k.w;
+        } else if (VL > 1 && i < n) {
+            for (int j = 0; j < VL - 1 && i + j < n; ++j) p[i + j] = k.e[j];
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (i < n) from_float(v[i], p[i]);
     }
 }
 
