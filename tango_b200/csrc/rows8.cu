@@ -385,21 +385,23 @@ __global__ void __launch_bounds__(kBlock, 4) rows8_staged_kernel(const __grid_co
         return reinterpret_cast<int8_t *>(room + Room::kXs * Room::kX + (Room::kQs > 1 ? (t & 1) * Room::kQ : 0));
     };
     const auto fetch = [&](int64_t tile, int64_t t) {
+        Run run{};
         if (tile < tiles) {
-            const Run run = run_of(a, Shape::kItems, tile * Shape::kItems);
+            run = run_of(a, Shape::kItems, tile * Shape::kItems);
             if constexpr (PACK || ACT) copy_in(buffer_x(t), static_cast<const T *>(a.x[job]), run.x, run.n, total);
             if constexpr (!PACK) copy_in(buffer_q(t), a.q[0], run.q, run.nq, total_q);
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
+        return run;
     };
     const bool keep = !PACK || !ACT || a.q[job];
-    fetch(blockIdx.x, 0);
+    Run next = fetch(blockIdx.x, 0);
     for (int64_t t = 0, tile = blockIdx.x; tile < tiles; ++t, tile += gridDim.x) {
-        fetch(tile + gridDim.x, t + 1);
+        const Run run = next;
+        next = fetch(tile + gridDim.x, t + 1);
         asm volatile("cp.async.wait_group 1;" ::: "memory");
         __syncthreads();
         const int64_t first = tile * Shape::kItems;
-        const Run run = run_of(a, Shape::kItems, first);
         T *s_x = buffer_x(t);
         int8_t *s_q = buffer_q(t);
         const int lead = (int)(run.x & (16 / sizeof(T) - 1)), lead_q = (int)(run.q & 15);

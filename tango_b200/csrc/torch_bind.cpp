@@ -152,8 +152,8 @@ PYBIND11_MODULE(_torch_ops, m) {
         const Rows8 r = pack8(x, group);
         return py::make_tuple(r.q, r.scale);
     });
-    m.def("unpack8", [](const Tensor &q, const Tensor &scale, const std::vector<int64_t> &sizes, int64_t group, const Tensor &like) {
-        return unpack8({q, scale}, sizes, group, like.scalar_type());
+    m.def("unpack8", [](const Tensor &q, const Tensor &scale, const std::vector<int64_t> &sizes, int64_t group, at::ScalarType type) {
+        return unpack8({q, scale}, sizes, group, type);
     });
     m.def("activation8", &activation8_fn);
     m.def("edge_attention", &edge_attention_fn);

@@ -1,6 +1,6 @@
-// 8-bit rows and what reads them, over at::Tensor, with autograd nodes.  The nodes keep codes and scales through the
-// saved-tensor hooks; scales and softmax statistics go through them as bytes, so that a hook that stores floating activations
-// in fewer bits leaves them alone.
+// 8-bit rows and what reads them, over at::Tensor, with autograd nodes.  What a node keeps -- codes, scales, softmax statistics
+// -- is one allocation of bytes, a saved tensor like any other (an allocation and a saved variable cost about a microsecond
+// each, which a small graph's pass notices).
 #include "torch_rows8.h"
 #include "torch_nodes.h"
 
@@ -19,53 +19,48 @@ static void require_matrix(const Tensor &t) {
 }
 static void require_group(int64_t group) { require(group >= 1 && group <= kMaxGroup, "groups of 1 to 1024 columns"); }
 
-static Tensor bytes(const Tensor &t) { return t.defined() ? t.view(at::kByte) : t; }
-static Tensor numbers(const Tensor &t) { return t.contiguous().view(at::kFloat); }
-
-static Rows8 alloc_rows8(int64_t rows, int64_t cols, int64_t group, const Tensor &like) {
-    const int64_t groups = cols ? (cols + group - 1) / group : 0;
-    return {at::empty({rows, tango_rows8_ld(cols, group)}, like.options().dtype(at::kChar)),
-            at::empty({rows, groups}, like.options().dtype(at::kFloat))};
+// Several arrays in one allocation, each on a 256-byte boundary.
+struct Layout {
+    int64_t bytes = 0;
+    int64_t add(int64_t n) {
+        const int64_t at = bytes;
+        bytes += (n + 255) / 256 * 256;
+        return at;
+    }
+};
+static Tensor allocate(const Layout &l, const Tensor &like) { return at::empty({l.bytes}, like.options().dtype(at::kByte)); }
+template <class T>
+static T *part(const Tensor &t, int64_t at) {
+    return reinterpret_cast<T *>(static_cast<char *>(t.data_ptr()) + at);
 }
 
-// Up to four matrices of one shape and type in one launch.  paired: the last two become one tensor of codes, interleaved, with
-// their scales in pairs.
-static std::vector<Rows8> pack_all(std::initializer_list<Tensor> tensors, int64_t group, bool paired = false) {
-    const Tensor &first = *tensors.begin();
-    const c10::cuda::CUDAGuard guard(first.device());
-    std::vector<Matrix> x;
-    std::vector<Rows8> out;
-    tango_rows8_job jobs[4];
-    for (const Tensor &t : tensors) x.push_back(matrix(t));
-    const size_t apart = x.size() - (paired ? 2 : 0);
-    for (size_t k = 0; k < apart; ++k) {
-        out.push_back(alloc_rows8(x[k].rows, x[k].cols, group, first));
-        jobs[k] = {ptr(x[k].t), x[k].ld, ptr<int8_t>(out[k].q), ptr<float>(out[k].scale), 1, 0};
-    }
-    if (paired) {
-        const int64_t groups = (x[0].cols + group - 1) / group, run = tango_rows8_run(group);
-        const Rows8 both{at::empty({x[0].rows, 2 * tango_rows8_ld(x[0].cols, group)}, first.options().dtype(at::kChar)),
-                         at::empty({x[0].rows, groups, 2}, first.options().dtype(at::kFloat))};
-        out.push_back(both);
-        for (size_t k = apart; k < x.size(); ++k)
-            jobs[k] = {ptr(x[k].t), x[k].ld, ptr<int8_t>(both.q) ? ptr<int8_t>(both.q) + (k - apart) * run : nullptr,
-                       ptr<float>(both.scale) ? ptr<float>(both.scale) + (k - apart) : nullptr, 2, 1};
-    }
-    if (x[0].rows == 0 || x[0].cols == 0) return out;
-    const int mode = settings().mode_quantize, n = (int)x.size();
-    const uint64_t call = mode == TANGO_ROUND_STOCHASTIC ? next_call() : 0;
-    for (int k = 1; k < n && call; ++k) next_call();
-    check(tango_rows8_pack(jobs, n, x[0].rows, x[0].cols, group, type_code(first), mode, settings().seed, call, settings().step,
+// The call number of a pack of n matrices: each draws with a number of its own when rounding is stochastic.
+static uint64_t calls_of(int mode, int n) {
+    if (mode != TANGO_ROUND_STOCHASTIC) return 0;
+    const uint64_t call = next_call();
+    for (int k = 1; k < n; ++k) next_call();
+    return call;
+}
+static void pack(const tango_rows8_job *jobs, int n, const Matrix &x, int64_t group) {
+    const int mode = settings().mode_quantize;
+    check(tango_rows8_pack(jobs, n, x.rows, x.cols, group, type_code(x.t), mode, settings().seed, calls_of(mode, n), settings().step,
                            cuda_stream()), "pack8");
     count(1);
-    return out;
 }
 
 Rows8 pack8(const Tensor &x, int64_t group) {
     require_matrix(x);
     require_group(group);
     const Raw raw;
-    return pack_all({x}, group)[0];
+    const c10::cuda::CUDAGuard guard(x.device());
+    const Matrix m = matrix(x);
+    const int64_t groups = (m.cols + group - 1) / group;
+    const Rows8 out{at::empty({m.rows, tango_rows8_ld(m.cols, group)}, x.options().dtype(at::kChar)),
+                    at::empty({m.rows, groups}, x.options().dtype(at::kFloat))};
+    if (m.rows == 0 || m.cols == 0) return out;
+    const tango_rows8_job job{ptr(m.t), m.ld, ptr<int8_t>(out.q), ptr<float>(out.scale), 1, 0};
+    pack(&job, 1, m, group);
+    return out;
 }
 
 Tensor unpack8(const Rows8 &r, at::IntArrayRef sizes, int64_t group, at::ScalarType type) {
@@ -88,6 +83,14 @@ Tensor unpack8(const Rows8 &r, at::IntArrayRef sizes, int64_t group, at::ScalarT
 }
 
 // ------------------------------------------------------------------------------------------------ activations
+// What an activation keeps of a matrix: codes, then scales.
+struct Copy8 {
+    Layout l;
+    int64_t codes, scales;
+    Copy8(int64_t rows, int64_t cols, int64_t group)
+        : codes(l.add(rows * tango_rows8_ld(cols, group))), scales(l.add(rows * ((cols + group - 1) / group) * 4)) {}
+};
+
 struct Activation8Backward : SavingNode {
     std::string name() const override { return "Activation8Backward"; }
     int act = 0;
@@ -101,9 +104,10 @@ struct Activation8Backward : SavingNode {
         const Matrix dy = matrix(grads[0].to(type));
         const Tensor dx = at::empty(sizes, grads[0].options().dtype(type));
         if (dx.numel() == 0) return {dx};
-        const Tensor q = k[0].contiguous(), scale = numbers(k[1]);
-        check(tango_act8_backward(act, ptr<int8_t>(q), ptr<float>(scale), dy.rows, dy.cols, group, type_code(dx), ptr(dy.t), dy.ld,
-                                  ptr(dx), std::max<int64_t>(dy.cols, 1), cuda_stream()), "activation8_backward");
+        const Tensor copy = k[0].contiguous();
+        const Copy8 at(dy.rows, dy.cols, group);
+        check(tango_act8_backward(act, part<int8_t>(copy, at.codes), part<float>(copy, at.scales), dy.rows, dy.cols, group,
+                                  type_code(dx), ptr(dy.t), dy.ld, ptr(dx), dy.cols, cuda_stream()), "activation8_backward");
         count(1);
         return {dx};
     }
@@ -112,55 +116,61 @@ struct Activation8Backward : SavingNode {
 Tensor activation8_fn(const Tensor &x_, int act, int64_t group) {
     require_matrix(x_);
     require_group(group);
-    Tensor y;
-    Rows8 copy;
-    const bool saves = torch::autograd::compute_requires_grad(x_);
+    Tensor y, copy;
+    auto node = make_node<Activation8Backward>(x_);
     {
         const Raw raw;
         const c10::cuda::CUDAGuard guard(x_.device());
         const Matrix x = matrix(x_);
+        const Copy8 at(x.rows, x.cols, group);
         y = at::empty(x_.sizes(), x_.options());
-        if (saves) copy = alloc_rows8(x.rows, x.cols, group, x_);
+        if (node) copy = allocate(at.l, x_);
         if (y.numel() > 0) {
             const int mode = settings().mode_quantize;
-            const uint64_t call = saves && mode == TANGO_ROUND_STOCHASTIC ? next_call() : 0;
-            const tango_rows8_job job{ptr(x.t), x.ld, ptr<int8_t>(copy.q), ptr<float>(copy.scale), 1, 0};
-            check(tango_act8_forward(act, &job, x.rows, x.cols, group, type_code(x_), ptr(y), x.cols, mode, settings().seed, call,
-                                     settings().step, cuda_stream()), "activation8");
+            tango_rows8_job job{ptr(x.t), x.ld, nullptr, nullptr, 1, 0};
+            if (node) { job.q = part<int8_t>(copy, at.codes); job.scales = part<float>(copy, at.scales); }
+            check(tango_act8_forward(act, &job, x.rows, x.cols, group, type_code(x_), ptr(y), x.cols, mode, settings().seed,
+                                     node ? calls_of(mode, 1) : 0, settings().step, cuda_stream()), "activation8");
             count(1);
         }
     }
-    if (auto node = make_node<Activation8Backward>(x_)) {
+    if (node) {
         node->act = act; node->group = group; node->sizes = x_.sizes().vec(); node->type = x_.scalar_type();
         torch::autograd::set_history(y, node);
-        node->keep({copy.q, bytes(copy.scale)});
+        node->keep({copy});
     }
     return y;
 }
 
 // ------------------------------------------------------------------------------------------------ edge attention
-// The row schedule of one direction and the workspace of its long rows.
+// The row schedule of one direction.
 struct EdgePlan {
     tango_edge_plan p{};
-    Tensor ws;
-    bool present = false;
+    bool present;
+    EdgePlan(const EdgeSchedule &s) : present(s.present) {
+        if (!present) return;
+        p.rows = ptr<int32_t>(s.rows); p.n_long = s.n_long;
+        p.units = ptr<int32_t>(s.units); p.n_units = s.n_units;
+        p.heavy_first = ptr<int32_t>(s.heavy_first); p.n_heavy = s.n_heavy;
+    }
     const tango_edge_plan *get() const { return present ? &p : nullptr; }
-    int64_t bytes() const { return ws.defined() ? ws.numel() : 0; }
+    int64_t workspace(int pass, int heads, int d) const { return tango_edge_attention_workspace_bytes(pass, p.n_units, heads, d); }
     int launches() const { return p.n_heavy > 0 ? 2 : 1; }
 };
-static EdgePlan edge_plan(const EdgeSchedule &s, int pass, int heads, int d, const Tensor &like) {
-    EdgePlan plan;
-    plan.present = s.present;
-    if (!plan.present) return plan;
-    plan.p.rows = ptr<int32_t>(s.rows); plan.p.n_long = s.n_long;
-    if (s.n_heavy == 0) return plan;
-    plan.p.units = ptr<int32_t>(s.units); plan.p.n_units = s.n_units;
-    plan.p.heavy_first = ptr<int32_t>(s.heavy_first); plan.p.n_heavy = s.n_heavy;
-    plan.ws = at::empty({tango_edge_attention_workspace_bytes(pass, s.n_units, heads, d)}, like.options().dtype(at::kByte));
-    return plan;
-}
 static const int32_t *index_ptr(const Direction &d) { return ptr<int32_t>(d.indices.numel() > 0 ? d.indices : d.indptr); }
-static tango_rows8 view(const Rows8 &r) { return {ptr<int8_t>(r.q), ptr<float>(r.scale)}; }
+
+// What the forward pass keeps: the 8-bit operands and the softmax statistics.
+struct Kept8 {
+    Layout l;
+    int64_t q, kv, sq, skv, stats;
+    Kept8(int64_t n, int64_t heads, int64_t d) {
+        const int64_t ld = tango_rows8_ld(heads * d, d);
+        q = l.add(n * ld); kv = l.add(2 * n * ld); sq = l.add(4 * n * heads); skv = l.add(8 * n * heads); stats = l.add(8 * n * heads);
+    }
+    tango_edge_operands operands(const Tensor &t) const {
+        return {part<int8_t>(t, q), part<int8_t>(t, kv), nullptr, part<float>(t, sq), part<float>(t, skv), nullptr};
+    }
+};
 
 struct EdgeAttentionBackward : SavingNode {
     std::string name() const override { return "EdgeAttentionBackward"; }
@@ -171,40 +181,39 @@ struct EdgeAttentionBackward : SavingNode {
     variable_list backward(const variable_list &grads) override {
         const std::vector<Tensor> k = kept();
         if (!grads[0].defined()) return variable_list(3);
-        const Tensor grad = grads[0].to(type);
-        const c10::cuda::CUDAGuard guard(grad.device());
-        const Tensor q8 = k[0].contiguous(), kv8 = k[1].contiguous();
-        const Tensor sq = numbers(k[2]), skv = numbers(k[3]), stats = numbers(k[4]);
-        const int64_t n = g->n_nodes;
-        const auto out = [&] { return at::empty({n, heads, d}, grad.options()); };
+        const Matrix grad = matrix(grads[0].to(type));
+        const c10::cuda::CUDAGuard guard(grad.t.device());
+        const int64_t n = g->n_nodes, ld = tango_rows8_ld((int64_t)heads * d, d);
+        const auto out = [&] { return at::empty({n, heads, d}, grad.t.options()); };
         const Tensor dq = out();
         if (n == 0) return {dq, out(), out()};
-        const Rows8 o8 = pack_all({grad}, d)[0];
+        const Tensor saved = k[0].contiguous();
+        const Kept8 in(n, heads, d);
         const bool sources = needs(1) || needs(2);
-        Tensor record, qo8;       // what the second pass reads of a destination
-        if (sources) {
-            record = at::empty({n, heads, 4}, grad.options().dtype(at::kFloat));
-            qo8 = at::empty_like(kv8);
-        }
-        tango_edge_operands x{ptr<int8_t>(q8), ptr<int8_t>(kv8), ptr<int8_t>(o8.q), ptr<float>(sq), ptr<float>(skv),
-                              ptr<float>(o8.scale)};
-        const int code = type_code(grad);
-        {
-            const Direction &in = g->dir(false);
-            const EdgePlan plan = edge_plan(in.edge_sched, 1, heads, d, grad);
-            check(tango_edge_attention_bwd_dst(ptr<int32_t>(in.indptr), index_ptr(in), n, plan.get(), heads, d, &x, scale,
-                                               ptr<float>(stats), ptr(dq), code, ptr<float>(record), ptr<int8_t>(qo8), ptr(plan.ws),
-                                               plan.bytes(), cuda_stream()), "edge_attention_bwd_dst");
-            count(plan.launches());
-        }
+        const Direction &to = g->dir(false), &from = g->dir(true);
+        const EdgePlan by_dst(to.edge_sched), by_src(from.edge_sched);
+        // the gradient in 8 bits, what the second pass reads of a destination, and the workspace, which the passes share
+        Layout l;
+        const int64_t o = l.add(n * ld), so = l.add(4 * n * heads), record = l.add(sources ? 16 * n * heads : 0),
+                      qo = l.add(sources ? 2 * n * ld : 0), ws_bytes = std::max(by_dst.workspace(1, heads, d), by_src.workspace(2, heads, d)),
+                      ws = l.add(ws_bytes);
+        const Tensor scratch = allocate(l, grad.t);
+        const tango_rows8_job job{ptr(grad.t), grad.ld, part<int8_t>(scratch, o), part<float>(scratch, so), 1, 0};
+        pack(&job, 1, grad, d);
+        tango_edge_operands x = in.operands(saved);
+        x.o = part<int8_t>(scratch, o); x.so = part<float>(scratch, so);
+        const int code = type_code(grad.t);
+        check(tango_edge_attention_bwd_dst(ptr<int32_t>(to.indptr), index_ptr(to), n, by_dst.get(), heads, d, &x, scale,
+                                           part<float>(saved, in.stats), ptr(dq), code, sources ? part<float>(scratch, record) : nullptr,
+                                           sources ? part<int8_t>(scratch, qo) : nullptr, part<void>(scratch, ws), ws_bytes,
+                                           cuda_stream()), "edge_attention_bwd_dst");
+        count(by_dst.launches());
         if (!sources) return {dq, Tensor(), Tensor()};
         const Tensor dk = out(), dv = out();
-        const Direction &from = g->dir(true);
-        const EdgePlan plan = edge_plan(from.edge_sched, 2, heads, d, grad);
-        check(tango_edge_attention_bwd_src(ptr<int32_t>(from.indptr), index_ptr(from), n, plan.get(), heads, d, ptr<int8_t>(kv8),
-                                           ptr<float>(skv), ptr<int8_t>(qo8), ptr<float>(record), ptr(dk), ptr(dv), code, ptr(plan.ws), plan.bytes(), cuda_stream()),
-              "edge_attention_bwd_src");
-        count(plan.launches());
+        check(tango_edge_attention_bwd_src(ptr<int32_t>(from.indptr), index_ptr(from), n, by_src.get(), heads, d, x.kv, x.skv,
+                                           part<int8_t>(scratch, qo), part<float>(scratch, record), ptr(dk), ptr(dv), code,
+                                           part<void>(scratch, ws), ws_bytes, cuda_stream()), "edge_attention_bwd_src");
+        count(by_src.launches());
         return {needs(0) ? dq : Tensor(), needs(1) ? dk : Tensor(), needs(2) ? dv : Tensor()};
     }
 };
@@ -225,33 +234,47 @@ Tensor edge_attention_fn(const GraphPtr &g, const Tensor &q, const Tensor &k, co
     require(g->csc->indptr.device() == q.device(), "graph and features must be on the same GPU");
     require(std::isfinite(scale), "finite scale expected");
     const int heads = (int)q.size(1), d = (int)q.size(2);
-    const bool saves = torch::autograd::compute_requires_grad(q, k, v);
-    Tensor out, stats;
-    std::vector<Rows8> r;
+    const int64_t n = q.size(0);
+    Tensor out, saved;
+    auto node = make_node<EdgeAttentionBackward>(q, k, v);
     {
         const Raw raw;
         const c10::cuda::CUDAGuard guard(q.device());
         out = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
-        r = pack_all({q, k, v}, d, true);
-        if (saves) stats = floats({q.size(0), heads, 2}, q);
-        if (q.size(0) > 0) {
-            const Direction &in = g->dir(false);
-            const EdgePlan plan = edge_plan(in.edge_sched, 0, heads, d, q);
-            const tango_edge_operands x{ptr<int8_t>(r[0].q), ptr<int8_t>(r[1].q), nullptr, ptr<float>(r[0].scale),
-                                        ptr<float>(r[1].scale), nullptr};
-            check(tango_edge_attention(ptr<int32_t>(in.indptr), index_ptr(in), q.size(0), plan.get(), heads, d, &x, (float)scale, ptr(out),
-                                       type_code(q), ptr<float>(stats), ptr(plan.ws), plan.bytes(), cuda_stream()),
-                  "edge_attention");
+        const Direction &in = g->dir(false);
+        const EdgePlan plan(in.edge_sched);
+        Kept8 at(n, heads, d);
+        const int64_t ws_bytes = plan.workspace(0, heads, d);
+        Tensor ws;
+        int64_t ws_at = 0;
+        if (node) ws = at::empty({ws_bytes}, q.options().dtype(at::kByte));
+        else ws_at = at.l.add(ws_bytes);
+        saved = allocate(at.l, q);
+        if (!node) ws = saved;
+        if (n > 0) {
+            const Matrix m[3] = {matrix(q), matrix(k), matrix(v)};
+            const tango_edge_operands x = at.operands(saved);
+            const int64_t run = tango_rows8_run(d);
+            int8_t *kv = part<int8_t>(saved, at.kv);
+            float *skv = part<float>(saved, at.skv);
+            const tango_rows8_job jobs[3] = {{ptr(m[0].t), m[0].ld, part<int8_t>(saved, at.q), part<float>(saved, at.sq), 1, 0},
+                                             {ptr(m[1].t), m[1].ld, kv, skv, 2, 1}, {ptr(m[2].t), m[2].ld, kv + run, skv + 1, 2, 1}};
+            pack(jobs, 3, m[0], d);
+            check(tango_edge_attention(ptr<int32_t>(in.indptr), index_ptr(in), n, plan.get(), heads, d, &x, (float)scale, ptr(out),
+                                       type_code(q), node ? part<float>(saved, at.stats) : nullptr, part<void>(ws, ws_at), ws_bytes,
+                                       cuda_stream()), "edge_attention");
             count(plan.launches());
         }
     }
-    if (auto node = make_node<EdgeAttentionBackward>(q, k, v)) {
+    if (node) {
         node->g = g; node->heads = heads; node->d = d; node->scale = (float)scale; node->type = q.scalar_type();
         torch::autograd::set_history(out, node);
-        node->keep({r[0].q, r[1].q, bytes(r[0].scale), bytes(r[1].scale), bytes(stats)});
+        node->keep({saved});
     }
     return out;
 }
+
+static tango_rows8 view(const Rows8 &r) { return {ptr<int8_t>(r.q), ptr<float>(r.scale)}; }
 
 Tensor edge_attention_rows(const GraphPtr &g, const Tensor &rows_, const Tensor &q, const Rows8 &k, const Rows8 &v, double scale) {
     require_heads(q);

@@ -22,7 +22,7 @@ class Packed8:
     __slots__ = ("codes", "scales", "shape", "group", "dtype")
 
     def __init__(self, codes, scales, shape, group, dtype):
-        self.codes, self.scales, self.shape, self.group, self.dtype = codes, scales, torch.Size(shape), group, dtype
+        self.codes, self.scales, self.shape, self.group, self.dtype = codes, scales, shape, group, dtype
 
     @property
     def device(self):
@@ -44,14 +44,13 @@ class Packed8:
 
 def pack8(x: torch.Tensor, group: int = GROUP) -> Packed8:
     """The 8-bit form of x (fp32, bf16 or fp16, any strides) in groups of `group` columns, 1 to 1024.  Not differentiable."""
-    codes, scales = _native.call(_native.ops.pack8, x.detach(), group)
+    codes, scales = _native.call(_native.ops.pack8, x if not x.requires_grad else x.detach(), group)
     return Packed8(codes, scales, x.shape, group, x.dtype)
 
 
 def unpack8(packed: Packed8, dtype=None) -> torch.Tensor:
     """The values of a packed tensor, by default in the type it had."""
-    like = torch.empty(0, dtype=packed.dtype if dtype is None else dtype)
-    return _native.call(_native.ops.unpack8, packed.codes, packed.scales, list(packed.shape), packed.group, like)
+    return _native.call(_native.ops.unpack8, packed.codes, packed.scales, packed.shape, packed.group, dtype or packed.dtype)
 
 
 _KINDS = {"elu": 0, "gelu": 1, "silu": 2}
