@@ -22,7 +22,7 @@
 namespace tango {
 
 enum { FORWARD = 0, BY_DST = 1, BY_SRC = 2 };
-constexpr int kWarps = 4, kRowWarps = 8;
+constexpr int kWarps = 4, kRowWarps = 4;
 
 struct AttnArgs {
     const int32_t *indptr, *indices;
@@ -533,30 +533,30 @@ struct RowsArgs {
     uint64_t seed, call;
     const unsigned long long *step;
 };
-constexpr int kRowChunk = 1024;   // edges below which a row is not cut
+constexpr int kRowChunk = 256;    // edges below which a row is not cut: eight trips of a block of F = 128
 
 __host__ __device__ inline int row_chunk(int len, int splits) {
     const int c = (len + splits - 1) / splits;
     return c < kRowChunk ? kRowChunk : c;
 }
 
-template <int VB, int P, class T>
-__device__ __forceinline__ Codes<VB> encode_query(const RowsArgs &a, int64_t r, int head, int chunk, bool live, float &s) {
-    const int64_t at = r * a.ldq + (int64_t)head * a.d + chunk * VB;
-    float v[VB], top = 0.f;
+template <int VB, class T>
+__device__ __forceinline__ void load_query(const RowsArgs &a, int64_t r, int head, int chunk, bool live, float (&v)[VB]) {
+    const T *p = static_cast<const T *>(a.q) + r * a.ldq + (int64_t)head * a.d + chunk * VB;
 #pragma unroll
-    for (int i = 0; i < VB / 4; ++i) {
-        load4<T, 1>(static_cast<const T *>(a.q) + at + 4 * i, live ? min(4, a.d - chunk * VB - 4 * i) : 0, v + 4 * i);
+    for (int i = 0; i < VB; i += 4) load4<T, 1>(p + i, live ? min(4, a.d - chunk * VB - i) : 0, v + i);
+}
+template <int VB, int P>
+__device__ __forceinline__ Codes<VB> encode_query(const RowsArgs &a, int64_t r, int head, int chunk, const float (&v)[VB], float &s) {
+    float top = 0.f;
 #pragma unroll
-        for (int k = 4 * i; k < 4 * i + 4; k += 2) top = max_abs3(v[k], v[k + 1], top);
-    }
+    for (int k = 0; k < VB; k += 2) top = max_abs3(v[k], v[k + 1], top);
 #pragma unroll
     for (int o = P / 2; o > 0; o >>= 1) top = max_or_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
     s = group_scale(top);
-    const float inv = group_inverse(s);
     Codes<VB> c;
     if (a.mode == TANGO_ROUND_NEAREST) {
-        encode_nearest<VB / 4>(v, s, inv, c.w);
+        encode_nearest<VB / 4>(v, s, group_inverse(s), c.w);
     } else {
 #pragma unroll
         for (int i = 0; i < VB / 4; ++i)
@@ -567,13 +567,24 @@ __device__ __forceinline__ Codes<VB> encode_query(const RowsArgs &a, int64_t r, 
 }
 
 template <int VB, int P>
-__global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(const __grid_constant__ RowsArgs a) {
-    constexpr int U = InFlight<FORWARD>::U;
+__global__ void __launch_bounds__(kRowWarps * 32, 6) attn_rows_kernel(const __grid_constant__ RowsArgs a) {
+    constexpr int U = 2;
     __shared__ float s_acc[kRowWarps][32 * VB];
     __shared__ float2 s_ml[kRowWarps][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t r = blockIdx.x;
     const int64_t row = __ldg(a.rows + r);
+    const int L = a.hb * P, slots = 32 / L;
+    const int slot = lane / L, in_edge = lane & (L - 1);
+    const int head = blockIdx.z * a.hb + in_edge / P, chunk = in_edge & (P - 1);
+    const bool live = head < a.heads && chunk * VB < a.pitch;
+    const int hd = head < a.heads ? head : a.heads - 1, off = live ? head * a.pitch + chunk * VB : hd * a.pitch;
+    // A short row is a chain of loads (bounds, ids, keys and values) that the query's does not depend on: it is asked for first
+    // and rounded while the first keys are on their way.
+    float query[VB];
+    if (a.type == TANGO_FP32) load_query<VB, float>(a, r, head, chunk, live, query);
+    else if (a.type == TANGO_BF16) load_query<VB, Bf16>(a, r, head, chunk, live, query);
+    else load_query<VB, Fp16>(a, r, head, chunk, live, query);
     const bool known = row >= 0 && row < a.n_nodes;
     const int beg0 = known ? __ldg(a.indptr + row) : 0, end0 = known ? __ldg(a.indptr + row + 1) : 0;
     const int chunk_len = row_chunk(end0 - beg0, a.splits);
@@ -581,24 +592,16 @@ __global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(const __grid_
     if (blockIdx.y > 0 && (int64_t)blockIdx.y * chunk_len >= end0 - beg0) return;
     const int beg = beg0 + blockIdx.y * chunk_len, end = end0 - beg < chunk_len ? end0 : beg + chunk_len;
 
-    const int L = a.hb * P, slots = 32 / L;
-    const int slot = lane / L, in_edge = lane & (L - 1);
-    const int head = blockIdx.z * a.hb + in_edge / P, chunk = in_edge & (P - 1);
-    const bool live = head < a.heads && chunk * VB < a.pitch;
-    const int hd = head < a.heads ? head : a.heads - 1, off = live ? head * a.pitch + chunk * VB : hd * a.pitch;
-    float sa;
-    const Codes<VB> fa = a.type == TANGO_FP32   ? encode_query<VB, P, float>(a, r, head, chunk, live, sa)
-                         : a.type == TANGO_BF16 ? encode_query<VB, P, Bf16>(a, r, head, chunk, live, sa)
-                                                : encode_query<VB, P, Fp16>(a, r, head, chunk, live, sa);
-    sa *= a.qscale;
     Running<VB> run;
     const int stride = slots * U * kRowWarps;
-    for (int j = beg + warp * slots * U; j < end; j += stride) {
-        Codes<VB> ga[U], gb[U];
-        float z[U], sk[U], sv[U];
-        int at[U];
+    int at[U], j = beg + warp * slots * U;
+    Codes<VB> ga[U], gb[U];
+    float sk[U], sv[U];
+    const auto ids = [&](int j) {
 #pragma unroll
         for (int u = 0; u < U; ++u) at[u] = __ldg(a.indices + min(j + u * slots + slot, end - 1));
+    };
+    const auto load = [&] {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             ga[u] = load_codes<VB>(a.k + (int64_t)at[u] * a.ld + off);
@@ -606,12 +609,27 @@ __global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(const __grid_
             sk[u] = __ldg(a.sk + (int64_t)at[u] * a.heads + hd);
             sv[u] = __ldg(a.sv + (int64_t)at[u] * a.heads + hd);
         }
+    };
+    if (j < end) {
+        ids(j);
+        load();
+        ids(j + stride);
+    }
+    float sa;
+    const Codes<VB> fa = encode_query<VB, P>(a, r, head, chunk, query, sa);
+    sa *= a.qscale;
+    while (j < end) {
+        float z[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const float s = dot<VB, P>(fa, ga[u]);
             z[u] = j + u * slots + slot < end ? __fmul_rn(s, __fmul_rn(sk[u], sa)) : -INFINITY;
         }
         softmax_step<VB, U>(run, z, sv, gb);
+        j += stride;
+        if (j >= end) break;
+        load();
+        ids(j + stride);
     }
     for (int o = L; o < 32; o <<= 1) run.merge(o);
     if (slot == 0) {
@@ -801,8 +819,10 @@ extern "C" int tango_edge_attention_bwd_src(const int32_t *indptr, const int32_t
 extern "C" int tango_edge_attention_rows_splits(int64_t n_rows, int64_t longest) {
     if (n_rows < 0 || longest < 0) return TANGO_EINVAL;
     if (n_rows == 0 || longest <= kRowChunk) return 1;
-    const int64_t most = 64, want = ceil_div(longest, kRowChunk);
-    return (int)(want < most ? want : most);
+    // Most of a row's blocks find nothing to do unless it is a long one, and take their turn all the same: 1024 rows of 20 M
+    // edges (62 in the middle, 2021 at most), 4 x 32, take 28 us with one block a row, 19 with 4, 22 with 8, 32 with 16.
+    const int64_t want = ceil_div(longest, kRowChunk), most = 4096 / n_rows < 64 ? 4096 / n_rows : 64;
+    return (int)(want < most ? want : most < 1 ? 1 : most);
 }
 
 extern "C" int64_t tango_edge_attention_rows_workspace_bytes(int64_t n_rows, int splits, int heads, int d) {

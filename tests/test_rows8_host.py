@@ -109,7 +109,8 @@ def test_attention_arguments_are_checked_before_any_launch():
 
     assert rows(n=0) == 0 and rows(n=-1) == -1 and rows(splits=0) == -1 and rows(ld=31) == -1 and rows(ids=None) == -1
     assert rows(splits=4) == -1 and rows(splits=4, ws=0x1000, nbytes=64) == -1 and rows(d=600) == -5
-    assert lib.tango_edge_attention_rows_splits(0, 10 ** 6) == 1 and lib.tango_edge_attention_rows_splits(5, 1024) == 1
+    assert lib.tango_edge_attention_rows_splits(0, 10 ** 6) == 1 and lib.tango_edge_attention_rows_splits(5, 256) == 1
+    assert lib.tango_edge_attention_rows_splits(10 ** 6, 10 ** 6) == 1
     assert 1 < lib.tango_edge_attention_rows_splits(1, 10 ** 6) <= 65535
 
 
