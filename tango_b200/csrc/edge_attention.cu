@@ -14,9 +14,9 @@
 // per edge through L2 together with the instructions that turn codes into floats and add them up.
 //
 // A lane holds VB neighbouring codes of one head (16, less for narrow heads), P lanes a head, L = P * (heads of a block)
-// lanes an edge; the rest of a team of lanes takes further edges, U of them in flight per lane.  A row of more than 48 edges
-// has a warp, a shorter one a part of a warp; the longest ones are cut into units whose partial results are merged by a
-// second launch.
+// lanes an edge, and a warp as many edges side by side (slots) as fit.  None of these has to be a power of two: three heads of
+// 41 are 9 lanes an edge, three edges a warp.  A long row has a warp, a short one the lanes of a slot or a few (a team); the
+// longest ones are cut into units whose partial results are merged by a second launch.
 #include "rows8.cuh"
 
 namespace tango {
@@ -24,11 +24,20 @@ namespace tango {
 enum { FORWARD = 0, BY_DST = 1, BY_SRC = 2 };
 constexpr int kWarps = 4, kRowWarps = 4;
 
+// How a warp is shared out.
+struct Lanes {
+    int hb, l, slots;                  // heads of a block, lanes of an edge, edges side by side
+    int team_slots, teams;             // slots of a short row's team, teams of a warp
+    uint32_t rcp_l, rcp_team;          // 65536 / lanes, rounded up: exact quotients of the 32 lanes
+};
+__device__ __forceinline__ int over(int lane, uint32_t rcp) { return (int)((uint32_t)lane * rcp >> 16); }
+
 struct AttnArgs {
     const int32_t *indptr, *indices;
     const int4 *rows, *units;                       // (row, first slot, end slot, place of a unit in its row)
     int64_t n_units, n_heavy, n_long, n_rows;       // rows: [heavy: by units] [to n_long: a warp] [the rest: a team]
-    int heads, d, pitch, hb, team;                  // hb: heads of a block (a power of two); team: lanes of a short row
+    int heads, d, pitch;
+    Lanes lanes;
     int ld;                                         // bytes of a row of codes
     const int8_t *q, *o, *kv;                       // kv and qo: runs of VB codes of the one and of the other in turn
     int8_t *qo;
@@ -49,7 +58,7 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return y;
 }
 
-__device__ __forceinline__ Pair shuffle2(Pair a, int lanes) { return {__shfl_xor_sync(0xffffffffu, a.v, lanes)}; }
+__device__ __forceinline__ Pair shuffle2(Pair a, int from) { return {__shfl_sync(0xffffffffu, a.v, from)}; }
 
 // VB codes.
 template <int VB> struct Codes { uint32_t w[VB / 4]; };
@@ -100,16 +109,37 @@ __device__ __forceinline__ Codes<VB> codes_if(bool there, const int8_t *p) {
     for (int i = 0; i < VB / 4; ++i) c.w[i] = 0;
     return c;
 }
-// Exact product of two heads, the same number in all their P lanes.
+// Sum over the P lanes of a head (of which this is the one at `chunk`), the same number in all of them.
+template <int P>
+__device__ __forceinline__ int head_sum(int s, int lane, int chunk) {
+    if constexpr ((P & (P - 1)) == 0) {             // heads start on multiples of P
+#pragma unroll
+        for (int o = P / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        return s;
+    } else {
+        int at = chunk;
+        if constexpr (P == 6) {
+            s += __shfl_sync(0xffffffffu, s, at < 3 ? lane + 3 : lane - 3);
+            at = at < 3 ? at : at - 3;
+        } else {
+            static_assert(P == 3, "lanes of a head");
+        }
+        const int right = __shfl_sync(0xffffffffu, s, at == 2 ? lane - 2 : lane + 1);
+        return s + right + __shfl_sync(0xffffffffu, s, at == 0 ? lane + 2 : lane - 1);
+    }
+}
+// Exact product of two heads.  Up to 256 codes the sum is below 2^22 and is added up in the mantissa of 1.5 * 2^23, with which
+// one lane of the head starts (`start`: dot_start).
+constexpr int kMagicBits = 0x4B400000;
 template <int VB, int P>
-__device__ __forceinline__ float dot(const Codes<VB> &a, const Codes<VB> &b) {
-    int s = 0;
+__device__ __forceinline__ int dot_start(int chunk) { return VB * P <= 256 && chunk == 0 ? kMagicBits : 0; }
+template <int VB, int P>
+__device__ __forceinline__ float dot(const Codes<VB> &a, const Codes<VB> &b, int start, int lane, int chunk) {
+    int s = start;
 #pragma unroll
     for (int i = 0; i < VB / 4; ++i) s = __dp4a((int)a.w[i], (int)b.w[i], s);
-#pragma unroll
-    for (int o = P / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    // up to 256 codes the sum is below 2^22 and sits in the mantissa of 1.5 * 2^23
-    if constexpr (VB * P <= 256) return __fsub_rn(__int_as_float(0x4B400000 + s), kRoundMagic);
+    s = head_sum<P>(s, lane, chunk);
+    if constexpr (VB * P <= 256) return __fsub_rn(__int_as_float(s), kRoundMagic);
     else return __int2float_rn(s);
 }
 // acc += by * codes
@@ -186,18 +216,35 @@ template <int VB> struct Running {
 #pragma unroll
         for (int i = 0; i < VB / 2; ++i) acc[i] = mul2(acc[i], cc);
     }
-    // with the same place of the lanes at a distance of `lanes`
-    __device__ __forceinline__ void merge(int lanes) {
-        const float mo = __shfl_xor_sync(0xffffffffu, m, lanes), lo = __shfl_xor_sync(0xffffffffu, l, lanes);
+    // with the same place of another slot, if there is one
+    __device__ __forceinline__ void merge(int from, bool there) {
+        float mo = __shfl_sync(0xffffffffu, m, from), lo = __shfl_sync(0xffffffffu, l, from);
+        if (!there) { mo = kBelow; lo = 0.f; }
         const float top = fmaxf(m, mo);
-        const float c = exp2_fast(m - top), co = exp2_fast(mo - top);
+        const float c = exp2_fast(m - top), co = there ? exp2_fast(mo - top) : 0.f;
         const Pair cc = pair(c, c), cco = pair(co, co);
         m = top;
         l = fmaf(l, c, lo * co);
 #pragma unroll
-        for (int i = 0; i < VB / 2; ++i) acc[i] = fma2(acc[i], cc, mul2(shuffle2(acc[i], lanes), cco));
+        for (int i = 0; i < VB / 2; ++i) {
+            const Pair o = shuffle2(acc[i], from);
+            acc[i] = mul2(acc[i], cc);
+            if (there) acc[i] = fma2(o, cco, acc[i]);
+        }
     }
 };
+
+// The slots of a team meet, the lower half taking over the upper one's until the first has all: f(lane to read, whether it counts).
+template <class F>
+__device__ __forceinline__ void join_slots(int slots, int slot, int lane, int l, F f) {
+    int o = 1;
+    while (o < slots) o <<= 1;
+    for (o >>= 1; o > 0; o >>= 1) {
+        const bool there = slot < o && slot + o < slots;
+        f(there ? lane + o * l : lane, there);
+        slots = o;
+    }
+}
 
 // One step of the forward pass: U edges of a lane; an edge that is not there has z = -inf and so no weight.
 template <int VB, int U>
@@ -226,20 +273,25 @@ __global__ void __launch_bounds__(kWarps * 32, MODE == FORWARD ? 6 : 4) attn_ker
     const int lane = threadIdx.x & 31;
     // ---- what this warp works on
     const int64_t w = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
-    int row = -1, beg = 0, end = 0, team = 32;
-    int64_t unit = -1;
-    int place = 0;
+    int row = -1, beg = 0, end = 0, place = 0, slots = a.lanes.slots, in_team = lane;
+    int64_t unit = -1, at = -1;
     if (w < a.n_units) {
         unit = w;
-        const int4 t = __ldg(a.units + w);
-        row = t.x; beg = t.y; end = t.z; place = t.w;
     } else {
-        int64_t at = w - a.n_units + a.n_heavy;
+        at = w - a.n_units + a.n_heavy;
         if (at >= a.n_long) {
-            team = a.team;
-            at = a.n_long + (at - a.n_long) * (32 / team) + lane / team;
+            const int team = over(lane, a.lanes.rcp_team);
+            slots = a.lanes.team_slots;
+            in_team = lane - team * slots * a.lanes.l;
+            at = team < a.lanes.teams ? a.n_long + (at - a.n_long) * a.lanes.teams + team : a.n_rows;
         }
-        if (at < a.n_rows) {
+    }
+    const int L = a.lanes.l, slot = over(in_team, a.lanes.rcp_l), in_edge = in_team - slot * L;
+    if (slot < slots) {                 // lanes behind the last slot have no row
+        if (unit >= 0) {
+            const int4 t = __ldg(a.units + unit);
+            row = t.x; beg = t.y; end = t.z; place = t.w;
+        } else if (at < a.n_rows) {
             if (a.rows) {
                 const int4 t = __ldg(a.rows + at);
                 row = t.x; beg = t.y; end = t.z;
@@ -248,9 +300,7 @@ __global__ void __launch_bounds__(kWarps * 32, MODE == FORWARD ? 6 : 4) attn_ker
             }
         }
     }
-    const int L = a.hb * P, slots = team / L;
-    const int slot = (lane & (team - 1)) / L, in_edge = lane & (L - 1);
-    const int head = blockIdx.y * a.hb + in_edge / P, chunk = in_edge & (P - 1);
+    const int head = blockIdx.y * a.lanes.hb + in_edge / P, chunk = in_edge % P, start = dot_start<VB, P>(chunk);
     const bool live = head < a.heads && chunk * VB < a.pitch;
     // Lanes without a place in the row read along with one that has (their own operand is 0, their results go nowhere), and
     // slots behind the row's end read its last edge once more without weight: no load and no register waits for a condition.
@@ -284,8 +334,8 @@ __global__ void __launch_bounds__(kWarps * 32, MODE == FORWARD ? 6 : 4) attn_ker
     }
     const int8_t *base = (MODE == BY_SRC ? a.qo : a.kv) + 2 * off;
     const int ld2 = 2 * a.ld;
-    const float2 *skv_base = a.skv + hd;
-    const float4 *rec_base = a.record + hd;
+    const char *scales = MODE == BY_SRC ? reinterpret_cast<const char *>(a.record + hd) : reinterpret_cast<const char *>(a.skv + hd);
+    const int scales_ld = a.heads * (MODE == BY_SRC ? (int)sizeof(float4) : (int)sizeof(float2));
 
     Running<VB> run;                    // forward: the softmax; else acc = the first sum
     Pair acc2[VB / 2];
@@ -311,8 +361,9 @@ __global__ void __launch_bounds__(kWarps * 32, MODE == FORWARD ? 6 : 4) attn_ker
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             load_runs<VB>(base + (int64_t)next[u] * ld2, t.a[u], t.b[u]);
-            if constexpr (MODE == BY_SRC) t.rec[u] = __ldg(rec_base + (int64_t)next[u] * a.heads);
-            else t.kv[u] = __ldg(skv_base + (int64_t)next[u] * a.heads);
+            const char *p = scales + (int64_t)next[u] * scales_ld;
+            if constexpr (MODE == BY_SRC) t.rec[u] = __ldg(reinterpret_cast<const float4 *>(p));
+            else t.kv[u] = __ldg(reinterpret_cast<const float2 *>(p));
         }
     };
     const auto work = [&](const Trip &t, int j) {
@@ -320,7 +371,7 @@ __global__ void __launch_bounds__(kWarps * 32, MODE == FORWARD ? 6 : 4) attn_ker
             float z[U], sv[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const float s = dot<VB, P>(fa, t.a[u]);
+                const float s = dot<VB, P>(fa, t.a[u], start, lane, chunk);
                 z[u] = j + u * slots < end ? __fmul_rn(s, __fmul_rn(t.kv[u].x, sa)) : -INFINITY;
                 sv[u] = t.kv[u].y;
             }
@@ -328,7 +379,7 @@ __global__ void __launch_bounds__(kWarps * 32, MODE == FORWARD ? 6 : 4) attn_ker
         } else if constexpr (MODE == BY_DST) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const float s = dot<VB, P>(fa, t.a[u]), dp = dot<VB, P>(fb, t.b[u]) * t.kv[u].y;
+                const float s = dot<VB, P>(fa, t.a[u], start, lane, chunk), dp = dot<VB, P>(fb, t.b[u], start, lane, chunk) * t.kv[u].y;
                 const float z = j + u * slots < end ? __fmul_rn(s, __fmul_rn(t.kv[u].x, sa)) : -INFINITY;
                 const float p = exp2_fast(z - top) * inv;
                 delta = fmaf(p, dp, delta);
@@ -339,7 +390,7 @@ __global__ void __launch_bounds__(kWarps * 32, MODE == FORWARD ? 6 : 4) attn_ker
             // record of a destination: scale * log2(e) * scale of q, maximum, scale of o / sum, delta / scale of o
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const float s = dot<VB, P>(fa, t.a[u]), dp = dot<VB, P>(fb, t.b[u]) * sb;
+                const float s = dot<VB, P>(fa, t.a[u], start, lane, chunk), dp = dot<VB, P>(fb, t.b[u], start, lane, chunk) * sb;
                 const float z = j + u * slots < end ? __fmul_rn(s, __fmul_rn(sa, t.rec[u].x)) : -INFINITY;
                 const float p = exp2_fast(z - t.rec[u].y) * t.rec[u].z;
                 const float ds = p * (dp - t.rec[u].w) * t.rec[u].x;
@@ -367,19 +418,22 @@ __global__ void __launch_bounds__(kWarps * 32, MODE == FORWARD ? 6 : 4) attn_ker
         }
     }
 
-    // ---- the slots of a team meet
-    for (int o = L; o < team; o <<= 1) {
+    join_slots(slots, slot, lane, L, [&](int from, bool there) {
         if constexpr (MODE == FORWARD) {
-            run.merge(o);
+            run.merge(from, there);
         } else {
-            delta += __shfl_xor_sync(0xffffffffu, delta, o);
+            const float d = __shfl_sync(0xffffffffu, delta, from);
+            if (there) delta += d;
 #pragma unroll
             for (int i = 0; i < VB / 2; ++i) {
-                run.acc[i] = add2(run.acc[i], shuffle2(run.acc[i], o));
-                acc2[i] = add2(acc2[i], shuffle2(acc2[i], o));
+                const Pair x = shuffle2(run.acc[i], from), y = shuffle2(acc2[i], from);
+                if (there) {
+                    run.acc[i] = add2(run.acc[i], x);
+                    acc2[i] = add2(acc2[i], y);
+                }
             }
         }
-    }
+    });
     if (end == beg) {               // a row without edges read along with others, whose NaN is not its own
         run.l = delta = 0.f;
 #pragma unroll
@@ -520,7 +574,8 @@ struct RowsArgs {
     int64_t n_nodes;
     const void *q;
     int64_t ldq;                  // elements between two queries
-    int heads, d, pitch, hb;
+    int heads, d, pitch;
+    Lanes lanes;
     int ld;
     const int8_t *k, *v;
     const float *sk, *sv;
@@ -551,8 +606,11 @@ __device__ __forceinline__ Codes<VB> encode_query(const RowsArgs &a, int64_t r, 
     float top = 0.f;
 #pragma unroll
     for (int k = 0; k < VB; k += 2) top = max_abs3(v[k], v[k + 1], top);
+    const int lane = threadIdx.x & 31, first = lane - chunk;
+    float all = top;
 #pragma unroll
-    for (int o = P / 2; o > 0; o >>= 1) top = max_or_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+    for (int k = 0; k < P; ++k) all = max_or_nan(all, __shfl_sync(0xffffffffu, top, first + k));
+    top = all;
     s = group_scale(top);
     Codes<VB> c;
     if (a.mode == TANGO_ROUND_NEAREST) {
@@ -574,10 +632,10 @@ __global__ void __launch_bounds__(kRowWarps * 32, 6) attn_rows_kernel(const __gr
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t r = blockIdx.x;
     const int64_t row = __ldg(a.rows + r);
-    const int L = a.hb * P, slots = 32 / L;
-    const int slot = lane / L, in_edge = lane & (L - 1);
-    const int head = blockIdx.z * a.hb + in_edge / P, chunk = in_edge & (P - 1);
-    const bool live = head < a.heads && chunk * VB < a.pitch;
+    const int L = a.lanes.l, slots = a.lanes.slots;
+    const int slot = over(lane, a.lanes.rcp_l), in_edge = lane - slot * L;
+    const int head = blockIdx.z * a.lanes.hb + in_edge / P, chunk = in_edge % P, start = dot_start<VB, P>(chunk);
+    const bool live = head < a.heads && chunk * VB < a.pitch, counts = slot < slots;      // lanes behind the last slot do not count
     const int hd = head < a.heads ? head : a.heads - 1, off = live ? head * a.pitch + chunk * VB : hd * a.pitch;
     // A short row is a chain of loads (bounds, ids, keys and values) that the query's does not depend on: it is asked for first
     // and rounded while the first keys are on their way.
@@ -622,8 +680,8 @@ __global__ void __launch_bounds__(kRowWarps * 32, 6) attn_rows_kernel(const __gr
         float z[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const float s = dot<VB, P>(fa, ga[u]);
-            z[u] = j + u * slots + slot < end ? __fmul_rn(s, __fmul_rn(sk[u], sa)) : -INFINITY;
+            const float s = dot<VB, P>(fa, ga[u], start, lane, chunk);
+            z[u] = counts && j + u * slots + slot < end ? __fmul_rn(s, __fmul_rn(sk[u], sa)) : -INFINITY;
         }
         softmax_step<VB, U>(run, z, sv, gb);
         j += stride;
@@ -631,7 +689,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 6) attn_rows_kernel(const __gr
         load();
         ids(j + stride);
     }
-    for (int o = L; o < 32; o <<= 1) run.merge(o);
+    join_slots(slots, slot, lane, L, [&](int from, bool there) { run.merge(from, there); });
     if (slot == 0) {
         s_ml[warp][in_edge] = make_float2(run.m, run.l);
 #pragma unroll
@@ -639,7 +697,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 6) attn_rows_kernel(const __gr
     }
     __syncthreads();
     for (int e = threadIdx.x; e < L * VB; e += kRowWarps * 32) {
-        const int ie = e / VB, hd = blockIdx.z * a.hb + ie / P, i = (ie & (P - 1)) * VB + e % VB;
+        const int ie = e / VB, hd = blockIdx.z * a.lanes.hb + ie / P, i = ie % P * VB + e % VB;
         if (hd >= a.heads || i >= a.d) continue;
         float m = kBelow, l = 0.f, s = 0.f;
 #pragma unroll
@@ -695,15 +753,29 @@ static int with_shape(int d, F f) {
     const std::integral_constant<int, 16> vb{};
     if (d <= 16) return f(vb, std::integral_constant<int, 1>{});
     if (d <= 32) return f(vb, std::integral_constant<int, 2>{});
+    if (d <= 48) return f(vb, std::integral_constant<int, 3>{});
     if (d <= 64) return f(vb, std::integral_constant<int, 4>{});
+    if (d <= 96) return f(vb, std::integral_constant<int, 6>{});
     if (d <= 128) return f(vb, std::integral_constant<int, 8>{});
     if (d <= 256) return f(vb, std::integral_constant<int, 16>{});
     return f(vb, std::integral_constant<int, 32>{});
 }
-static int heads_of_a_block(int heads, int p) {
-    int hb = 1;
-    while (hb < heads && hb * 2 * p <= 32) hb *= 2;
-    return hb;
+// Heads of a block: as many as fit, unless fewer leave clearly fewer lanes idle.  (A head's lanes all have work, so that idle ones
+// are those behind the last slot and those of heads that a last block lacks.)
+static Lanes share_out(int heads, int p) {
+    Lanes best{};
+    double most = 0;
+    for (int hb = heads < 32 / p ? heads : 32 / p; hb >= 1; --hb) {
+        const int l = hb * p, slots = 32 / l, blocks = (heads + hb - 1) / hb;
+        const double busy = (double)heads / (blocks * hb) * (slots * l) / 32;
+        if (busy <= most * 1.1) continue;
+        most = busy;
+        // a short row's team: about eight lanes
+        const int team_slots = l < 8 ? 8 / l : 1;
+        best = {hb, l, slots, team_slots, 32 / (team_slots * l), (uint32_t)(65536 + l - 1) / l,
+                (uint32_t)(65536 + team_slots * l - 1) / (team_slots * l)};
+    }
+    return best;
 }
 static bool known_type(int type) { return type >= TANGO_FP32 && type <= TANGO_FP16; }
 
@@ -728,10 +800,9 @@ static int launch(AttnArgs a, const tango_edge_plan *plan, float *ws, int64_t ws
     a.ws = ws;
     const int rc = with_shape(a.d, [&](auto vb, auto p) -> int {
         constexpr int VB = decltype(vb)::value, P = decltype(p)::value;
-        a.hb = heads_of_a_block(a.heads, P);
-        a.team = a.hb * P > 8 ? a.hb * P : 8;
-        const int64_t warps = a.n_units + (a.n_long - a.n_heavy) + ceil_div(a.n_rows - a.n_long, 32 / a.team);
-        const int64_t blocks = ceil_div(warps, kWarps), by = ceil_div(a.heads, a.hb);
+        a.lanes = share_out(a.heads, P);
+        const int64_t warps = a.n_units + (a.n_long - a.n_heavy) + ceil_div(a.n_rows - a.n_long, a.lanes.teams);
+        const int64_t blocks = ceil_div(warps, kWarps), by = ceil_div(a.heads, a.lanes.hb);
         if (blocks > 0x7fffffffLL || by > 65535) return TANGO_ESIZE;
         attn_kernel<MODE, VB, P><<<dim3((unsigned)blocks, (unsigned)by), kWarps * 32, 0, st>>>(a);
         TANGO_LAUNCH_CHECK();
@@ -854,8 +925,8 @@ extern "C" int tango_edge_attention_rows(const int32_t *indptr, const int32_t *i
     a.mode = mode; a.seed = seed; a.call = call; a.step = reinterpret_cast<const unsigned long long *>(step);
     const int done = with_shape(d, [&](auto vb, auto p) -> int {
         constexpr int VB = decltype(vb)::value, P = decltype(p)::value;
-        a.hb = heads_of_a_block(heads, P);
-        const int64_t bz = ceil_div(heads, a.hb);
+        a.lanes = share_out(heads, P);
+        const int64_t bz = ceil_div(heads, a.lanes.hb);
         if (bz > 65535) return TANGO_ESIZE;
         attn_rows_kernel<VB, P><<<dim3((unsigned)n_rows, (unsigned)splits, (unsigned)bz), kRowWarps * 32, 0, st>>>(a);
         TANGO_LAUNCH_CHECK();
