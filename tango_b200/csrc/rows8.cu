@@ -120,7 +120,102 @@ template <int LPG, int R> struct Tile {
     static constexpr int kElements = kItems * LPG * R * 4;
 };
 
-template <class T, int VL, int LPG, int R, bool ACT>
+// How the elements are reached: in one run, four or two at a time, one at a time, or (two-byte elements of any alignment) in
+// aligned pieces that are shifted into place.
+enum { SHIFTED = 0, SINGLE = 1, PAIRS = 2, WIDE = 4, FLAT = 8 };
+
+// ---- a lane's elements of a group: four neighbours at lane * 4, (lane + LPG) * 4, ..
+// Two-byte elements of any alignment come in the aligned 8-byte pieces that hold them; a lane's four straddle its own piece and
+// the next lane's.  Single accesses of two bytes each took 373 us where these take TIME (169343 x 601 bf16, SiLU, forward).
+template <int LPG>
+__device__ __forceinline__ uint64_t from_lane(uint64_t v, int lane) { return __shfl_sync(0xffffffffu, v, ((threadIdx.x & 31) & ~(LPG - 1)) + lane); }
+
+// n elements at p; [begin, end): the matrix, outside of which nothing is read.
+template <class T, int ACCESS, int LPG, int R>
+__device__ __forceinline__ void load_group(const T *p, int n, const T *begin, const T *end, float (&v)[R * 4]) {
+    const int lane = threadIdx.x % LPG;
+    if constexpr (ACCESS != SHIFTED) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) load4<T, ACCESS>(p + (lane + r * LPG) * 4, n - (lane + r * LPG) * 4, v + 4 * r);
+    } else {
+        const int off = (int)(reinterpret_cast<uintptr_t>(p) & 7), bits = off * 8, pieces = n > 0 ? (n * 2 + off + 7) / 8 : 0;
+        const char *first = reinterpret_cast<const char *>(p) - off;
+        const bool inside = first >= reinterpret_cast<const char *>(begin) && first + pieces * 8 <= reinterpret_cast<const char *>(end);
+        uint64_t w[R + 1];
+#pragma unroll
+        for (int r = 0; r <= R; ++r) {
+            const int k = lane + r * LPG;
+            w[r] = 0;
+            if (r == R && lane > 0) continue;
+            if (k >= pieces) continue;
+            if (inside) {
+                w[r] = __ldg(reinterpret_cast<const unsigned long long *>(first) + k);
+            } else {                    // the matrix begins or ends inside a piece
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int e = k * 4 - off / 2 + i;
+                    if (e >= 0 && e < n) w[r] |= (uint64_t)__ldg(reinterpret_cast<const unsigned short *>(p) + e) << (16 * i);
+                }
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const uint64_t next = from_lane<LPG>(lane == 0 ? w[r + 1] : w[r], (lane + 1) & (LPG - 1));
+            const uint64_t four = bits ? w[r] >> bits | next << (64 - bits) : w[r];
+            const int left = n - (lane + r * LPG) * 4;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                T t;
+                t.bits = i < left ? (uint16_t)(four >> (16 * i)) : (uint16_t)0;
+                v[4 * r + i] = to_float(t);
+            }
+        }
+    }
+}
+template <class T, int ACCESS, int LPG, int R>
+__device__ __forceinline__ void store_group(T *p, int n, const float (&v)[R * 4]) {
+    const int lane = threadIdx.x % LPG;
+    if constexpr (ACCESS != SHIFTED) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) store4<T, ACCESS>(p + (lane + r * LPG) * 4, n - (lane + r * LPG) * 4, v + 4 * r);
+    } else {
+        const int off = (int)(reinterpret_cast<uintptr_t>(p) & 7), bits = off * 8, skip = off / 2;
+        uint64_t *first = reinterpret_cast<uint64_t *>(reinterpret_cast<char *>(p) - off);
+        uint64_t w[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            w[r] = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                T t;
+                from_float(v[4 * r + i], t);
+                w[r] |= (uint64_t)t.bits << (16 * i);
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const uint64_t before = from_lane<LPG>(lane == LPG - 1 ? (r > 0 ? w[r > 0 ? r - 1 : 0] : 0) : w[r], (lane + LPG - 1) & (LPG - 1));
+            const uint64_t piece = bits ? w[r] << bits | before >> (64 - bits) : w[r];
+            const int k = lane + r * LPG, e = k * 4 - skip;          // the piece's first element
+            if (e >= 0 && e + 4 <= n) {
+                first[k] = piece;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (e + i >= 0 && e + i < n) p[e + i].bits = (uint16_t)(piece >> (16 * i));
+            }
+        }
+        if (lane == LPG - 1) {                                        // what the shift pushed out behind the last piece
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int e = (R * LPG - 1) * 4 + i;
+                if (i >= 4 - skip && e < n) p[e].bits = (uint16_t)(w[R - 1] >> (16 * i));
+            }
+        }
+    }
+}
+
+template <class T, int ACCESS, int LPG, int R, bool ACT>
 __global__ void __launch_bounds__(kBlock) rows8_pack_kernel(const __grid_constant__ Rows8Args a) {
     constexpr int U = Tile<LPG, R>::U, NG = Tile<LPG, R>::kGroups;
     const int job = blockIdx.y, lane = threadIdx.x % LPG;
@@ -133,9 +228,7 @@ __global__ void __launch_bounds__(kBlock) rows8_pack_kernel(const __grid_constan
         const int64_t i = first + u * NG;
         w[u] = {0, 0, 0, 0};
         if (i < a.items) w[u] = locate(a, i, a.ldx[job]);
-        const T *p = x + w[u].x + lane * 4;
-#pragma unroll
-        for (int r = 0; r < R; ++r) load4<T, VL>(p + r * LPG * 4, w[u].n - (lane + r * LPG) * 4, v[u] + 4 * r);
+        load_group<T, ACCESS, LPG, R>(x + w[u].x, w[u].n, x, x + (a.rows - 1) * a.ldx[job] + a.cols, v[u]);
     }
     const int run = a.run[job];
 #pragma unroll
@@ -146,9 +239,8 @@ __global__ void __launch_bounds__(kBlock) rows8_pack_kernel(const __grid_constan
 #pragma unroll
         for (int o = LPG / 2; o > 0; o >>= 1) top = max_or_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
         const int64_t i = first + u * NG;
-        if (i >= a.items) continue;
         const bool keep = !ACT || a.q[job];          // an activation without a backward pass keeps nothing
-        if (keep) {
+        if (keep && i < a.items) {
             const float s = group_scale(top), inv = group_inverse(s);
             const int width = code_width(a, w[u]);
             int8_t *q = a.q[job] + (code_place(a, w[u]) << (run > 0));
@@ -169,24 +261,22 @@ __global__ void __launch_bounds__(kBlock) rows8_pack_kernel(const __grid_constan
             }
         }
         if constexpr (ACT) {
-            T *y = static_cast<T *>(a.y) + (w[u].x + w[u].row * (a.ldy - a.ldx[0])) + lane * 4;
             with_act(a.act, [&](auto kind) {
 #pragma unroll
                 for (int k = 0; k < R * 4; ++k) v[u][k] = activate<kind.value>(v[u][k]);
             });
-#pragma unroll
-            for (int r = 0; r < R; ++r) store4<T, VL>(y + r * LPG * 4, w[u].n - (lane + r * LPG) * 4, v[u] + 4 * r);
+            store_group<T, ACCESS, LPG, R>(static_cast<T *>(a.y) + (w[u].x + w[u].row * (a.ldy - a.ldx[0])), w[u].n, v[u]);
         }
     }
 }
 
-template <class T, int VL, int LPG, int R, bool ACT>
+template <class T, int ACCESS, int LPG, int R, bool ACT>
 __global__ void __launch_bounds__(kBlock) rows8_unpack_kernel(const __grid_constant__ Rows8Args a) {
     constexpr int U = Tile<LPG, R>::U, NG = Tile<LPG, R>::kGroups;
     const int lane = threadIdx.x % LPG;
     const int64_t first = (int64_t)blockIdx.x * (NG * U) + threadIdx.x / LPG;
     uint32_t word[U][R];
-    float dy[ACT ? U : 1][R][4], s[U];
+    float dy[ACT ? U : 1][R * 4], s[U];
     Where w[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -199,11 +289,13 @@ __global__ void __launch_bounds__(kBlock) rows8_unpack_kernel(const __grid_const
         for (int r = 0; r < R; ++r) {
             const int e = (lane + r * LPG) * 4;
             word[u][r] = e < w[u].n ? __ldg(reinterpret_cast<const uint32_t *>(q + r * LPG * 4)) : 0u;
-            if constexpr (ACT)
-                load4<T, VL>(static_cast<const T *>(a.x[0]) + (w[u].x + w[u].row * (a.ldx[0] - a.ldy)) + e, w[u].n - e, dy[u][r]);
+        }
+        if constexpr (ACT) {
+            const T *x = static_cast<const T *>(a.x[0]);
+            load_group<T, ACCESS, LPG, R>(x + (w[u].x + w[u].row * (a.ldx[0] - a.ldy)), w[u].n, x, x + (a.rows - 1) * a.ldx[0] + a.cols, dy[u]);
         }
     }
-    float o[U][R][4];
+    float o[U][R * 4];
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -211,25 +303,18 @@ __global__ void __launch_bounds__(kBlock) rows8_unpack_kernel(const __grid_const
             Pair lo, hi;
             decode4(word[u][r], lo, hi);
             const float2 l = both(mul2(lo, pair(s[u], s[u]))), h = both(mul2(hi, pair(s[u], s[u])));
-            o[u][r][0] = l.x; o[u][r][1] = l.y; o[u][r][2] = h.x; o[u][r][3] = h.y;
+            o[u][4 * r] = l.x; o[u][4 * r + 1] = l.y; o[u][4 * r + 2] = h.x; o[u][4 * r + 3] = h.y;
         }
     if constexpr (ACT) {
         with_act(a.act, [&](auto kind) {
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
-                for (int r = 0; r < R; ++r)
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) o[u][r][k] = __fmul_rn(dy[u][r][k], slope_of<kind.value>(o[u][r][k]));
+                for (int k = 0; k < R * 4; ++k) o[u][k] = __fmul_rn(dy[u][k], slope_of<kind.value>(o[u][k]));
         });
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const int e = (lane + r * LPG) * 4;
-            store4<T, VL>(static_cast<T *>(a.y) + w[u].x + e, w[u].n - e, o[u][r]);
-        }
+    for (int u = 0; u < U; ++u) store_group<T, ACCESS, LPG, R>(static_cast<T *>(a.y) + w[u].x, w[u].n, o[u]);
 }
 
 // ---- contiguous matrices whose groups have 4, 8, .. 128 columns and fill their rows: one run of memory in every respect (groups,
@@ -310,206 +395,13 @@ __global__ void __launch_bounds__(kBlock) rows8_flat_kernel(const __grid_constan
     }
 }
 
-// ---- contiguous matrices whose row pitch allows no wide access (601 columns): the items of a block are one run of memory all the
-// same, in the matrix as in the codes, and pass through shared memory in 16-byte pieces, the next ones while a block works on
-// one.  Lanes take single neighbouring elements there.
-__device__ __forceinline__ void copy_async(void *shared, const void *global) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(shared)), "l"(global) : "memory");
-}
-// from[begin .. begin + n) of an array of `total` elements to to[begin % per ..], by whole 16-byte pieces of the array (which its
-// last elements may not fill).
-template <class T>
-__device__ __forceinline__ void copy_in(T *to, const T *from, int64_t begin, int n, int64_t total) {
-    constexpr int per = 16 / sizeof(T);
-    const int lead = (int)(begin & (per - 1));
-    const T *p = from + (begin - lead);
-    const int64_t left = total - (begin - lead);
-    for (int at = threadIdx.x * per; at < lead + n; at += kBlock * per) {
-        if (at + per <= left) {
-            copy_async(to + at, p + at);
-        } else {
-            for (int k = at; k < left; ++k) to[k] = p[k];
-        }
-    }
-}
-template <class T>
-__device__ __forceinline__ void copy_out(T *to, int64_t begin, int n, const T *from) {
-    constexpr int per = 16 / sizeof(T);
-    const int lead = (int)(begin & (per - 1));
-    T *p = to + (begin - lead);
-    const int end = lead + n;
-    for (int at = threadIdx.x * per; at < end; at += kBlock * per) {
-        if (at >= lead && at + per <= end) {
-            *reinterpret_cast<uint4 *>(p + at) = *reinterpret_cast<const uint4 *>(from + at);
-        } else {
-            for (int k = at < lead ? lead : at; k < at + per && k < end; ++k) p[k] = from[k];
-        }
-    }
-}
-
-// The run of a block's items: first element and byte of codes, and how many of each.
-struct Run {
-    int64_t x, q;
-    int n, nq, items;
-};
-__device__ __forceinline__ Run run_of(const Rows8Args &a, int items, int64_t first) {
-    Run r;
-    r.items = a.items - first < items ? (int)(a.items - first) : items;
-    const Where b = locate(a, first, a.cols), e = locate(a, first + r.items - 1, a.cols);
-    r.x = b.x; r.n = (int)(e.x + e.n - b.x);
-    r.q = code_place(a, b); r.nq = (int)(code_place(a, e) + code_width(a, e) - r.q);
-    return r;
-}
-
-// The r-th element of this lane's group: neighbouring lanes, neighbouring elements, and every group of a warp begins at another
-// place (32 elements are one turn of all banks), for groups that start in one bank of shared memory.
-template <int LPG, int R>
-__device__ __forceinline__ int turned(int r) { return ((int)(threadIdx.x % 32) + r * LPG) & (LPG * R * 4 - 1); }
-
-// Shared memory: buffers of elements and of codes, each with room for the pieces that stick out at both ends.
-template <class T, int LPG, int R, bool ACT, bool PACK> struct Staging {
-    static constexpr int kX = (Tile<LPG, R>::kElements + 32 / (int)sizeof(T)) * (int)sizeof(T), kQ = Tile<LPG, R>::kElements + 32;
-    static constexpr int kXs = PACK || ACT ? 2 : 1, kQs = PACK ? 1 : 2;
-    static constexpr int kBytes = kXs * kX + kQs * kQ;
-};
-
-template <class T, int LPG, int R, bool ACT, bool PACK>
-__global__ void __launch_bounds__(kBlock, 4) rows8_staged_kernel(const __grid_constant__ Rows8Args a) {
-    typedef Tile<LPG, R> Shape;
-    typedef Staging<T, LPG, R, ACT, PACK> Room;
-    extern __shared__ __align__(16) char room[];
-    const int job = blockIdx.y, lane = threadIdx.x % LPG;
-    const int64_t tiles = (a.items + Shape::kItems - 1) / Shape::kItems, total = a.rows * a.cols, total_q = a.rows * a.ldq;
-    const auto buffer_x = [&](int64_t t) { return reinterpret_cast<T *>(room + (Room::kXs > 1 ? (t & 1) * Room::kX : 0)); };
-    const auto buffer_q = [&](int64_t t) {
-        return reinterpret_cast<int8_t *>(room + Room::kXs * Room::kX + (Room::kQs > 1 ? (t & 1) * Room::kQ : 0));
-    };
-    const auto fetch = [&](int64_t tile, int64_t t) {
-        Run run{};
-        if (tile < tiles) {
-            run = run_of(a, Shape::kItems, tile * Shape::kItems);
-            if constexpr (PACK || ACT) copy_in(buffer_x(t), static_cast<const T *>(a.x[job]), run.x, run.n, total);
-            if constexpr (!PACK) copy_in(buffer_q(t), a.q[0], run.q, run.nq, total_q);
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        return run;
-    };
-    const bool keep = !PACK || !ACT || a.q[job];
-    Run next = fetch(blockIdx.x, 0);
-    for (int64_t t = 0, tile = blockIdx.x; tile < tiles; ++t, tile += gridDim.x) {
-        const Run run = next;
-        next = fetch(tile + gridDim.x, t + 1);
-        asm volatile("cp.async.wait_group 1;" ::: "memory");
-        __syncthreads();
-        const int64_t first = tile * Shape::kItems;
-        T *s_x = buffer_x(t);
-        int8_t *s_q = buffer_q(t);
-        const int lead = (int)(run.x & (16 / sizeof(T) - 1)), lead_q = (int)(run.q & 15);
-#pragma unroll
-        for (int u = 0; u < Shape::U; ++u) {
-            const int k = threadIdx.x / LPG + u * Shape::kGroups;
-            const bool there = k < run.items;
-            Where w = {0, 0, 0, 0};
-            if (there) w = locate(a, first + k, a.cols);
-            // threads without an item read along with the first one
-            T *x = s_x + lead + (there ? (int)(w.x - run.x) : 0);
-            int8_t *q = s_q + lead_q + (there ? (int)(code_place(a, w) - run.q) : 0);
-            if constexpr (PACK) {
-                // elements behind the item's end are read too (they are in the buffer) and taken for 0
-                float v[R * 4], top = 0.f;
-#pragma unroll
-                for (int r = 0; r < R * 4; ++r) v[r] = to_float(x[turned<LPG, R>(r)]);
-#pragma unroll
-                for (int r = 0; r < R * 4; ++r) v[r] = turned<LPG, R>(r) < w.n ? v[r] : 0.f;
-#pragma unroll
-                for (int r = 0; r < R * 4; r += 2) top = max_abs3(v[r], v[r + 1], top);
-#pragma unroll
-                for (int o = LPG / 2; o > 0; o >>= 1) top = max_or_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
-                if (there && keep) {
-                    const float s = group_scale(top), inv = group_inverse(s);
-                    if (lane == 0) a.scale[job][(first + k) * a.scale_stride[job]] = s;
-                    const int width = code_width(a, w);
-                    if (a.mode == TANGO_ROUND_NEAREST) {
-                        float b[R * 4];
-                        round_nearest<R * 4>(v, s, inv, b);
-#pragma unroll
-                        for (int r = 0; r < R * 4; ++r) {
-                            const int e = turned<LPG, R>(r);
-                            if (e < width) q[e] = inv == 0.f ? (int8_t)0 : (int8_t)__float_as_uint(b[r]);
-                        }
-                    } else {
-#pragma unroll 1
-                        for (int r = 0; r < R * 4; ++r) {
-                            const int e = turned<LPG, R>(r);
-                            if (e < width)
-                                q[e] = e < w.n ? (int8_t)encode_mode(to_float(x[e]), s, a.mode, a.seed, effective_call(a.call + job, a.step),
-                                                                     (uint64_t)w.row * a.cols + (int64_t)w.g * a.group + e)
-                                               : (int8_t)0;
-                        }
-                    }
-                }
-                if constexpr (ACT) {
-                    with_act(a.act, [&](auto kind) {
-#pragma unroll
-                        for (int r = 0; r < R * 4; ++r) v[r] = activate<kind.value>(v[r]);
-                    });
-#pragma unroll
-                    for (int r = 0; r < R * 4; ++r)
-                        if (turned<LPG, R>(r) < w.n) from_float(v[r], x[turned<LPG, R>(r)]);
-                }
-            } else if (there) {
-                const float s = __ldg(a.scale[0] + first + k);
-                float o[R * 4];
-#pragma unroll
-                for (int r = 0; r < R * 4; ++r) o[r] = __fmul_rn((float)q[turned<LPG, R>(r)], s);
-                if constexpr (ACT) {
-                    float dy[R * 4];
-#pragma unroll
-                    for (int r = 0; r < R * 4; ++r) dy[r] = to_float(x[turned<LPG, R>(r)]);
-                    with_act(a.act, [&](auto kind) {
-#pragma unroll
-                        for (int r = 0; r < R * 4; ++r) o[r] = __fmul_rn(dy[r], slope_of<kind.value>(o[r]));
-                    });
-                }
-#pragma unroll
-                for (int r = 0; r < R * 4; ++r)
-                    if (turned<LPG, R>(r) < w.n) from_float(o[r], x[turned<LPG, R>(r)]);
-            }
-        }
-        __syncthreads();
-        if constexpr (PACK) {
-            if (keep) copy_out(a.q[job], run.q, run.nq, s_q);
-        }
-        if constexpr (!PACK || ACT) copy_out(static_cast<T *>(a.y), run.x, run.n, s_x);
-        __syncthreads();          // before the buffers are filled again
-    }
-}
-
-// How the elements are reached: four at a time, the same in one run, one at a time (rows of any pitch), or through shared memory.
-enum { SINGLE = 0, STAGED = 1, WIDE = 2, FLAT = 3 };
-
-static int sm_count() {
-    int device = 0, n = kNumSMs;
-    if (cudaGetDevice(&device) == cudaSuccess) cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device);
-    return n;
-}
-
 template <class T, int ACCESS, bool ACT, bool PACK, int LPG, int R>
 static int launch_kernel(const Rows8Args &a, int jobs, cudaStream_t st) {
     const int64_t blocks = ceil_div(a.items, Tile<LPG, R>::kItems);
     if (blocks > 0x7fffffffLL) return TANGO_ESIZE;
     const dim3 grid((unsigned)blocks, (unsigned)jobs);
-    if constexpr (ACCESS == STAGED) {
-        constexpr int bytes = Staging<T, LPG, R, ACT, PACK>::kBytes, resident = 220 * 1024 / bytes < 4 ? 220 * 1024 / bytes : 4;
-        const auto kernel = rows8_staged_kernel<T, LPG, R, ACT, PACK>;
-        if (bytes > 48 * 1024) TANGO_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-        const int64_t most = (int64_t)sm_count() * resident;
-        kernel<<<dim3((unsigned)(blocks < most ? blocks : most), (unsigned)jobs), kBlock, bytes, st>>>(a);
-    } else if constexpr (PACK) {
-        rows8_pack_kernel<T, ACCESS == WIDE ? 4 : 1, LPG, R, ACT><<<grid, kBlock, 0, st>>>(a);
-    } else {
-        rows8_unpack_kernel<T, ACCESS == WIDE ? 4 : 1, LPG, R, ACT><<<grid, kBlock, 0, st>>>(a);
-    }
+    if constexpr (PACK) rows8_pack_kernel<T, ACCESS, LPG, R, ACT><<<grid, kBlock, 0, st>>>(a);
+    else rows8_unpack_kernel<T, ACCESS, LPG, R, ACT><<<grid, kBlock, 0, st>>>(a);
     TANGO_LAUNCH_CHECK();
     return TANGO_OK;
 }
@@ -551,10 +443,10 @@ template <bool ACT, bool PACK>
 static int launch(const Rows8Args &a, int jobs, int type, int access, cudaStream_t st) {
     const auto go = [&](auto t) {
         typedef decltype(t) T;
-        return access == FLAT     ? launch_flat<T, ACT, PACK>(a, jobs, st)
-               : access == WIDE   ? launch_tile<T, WIDE, ACT, PACK>(a, jobs, st)
-               : access == STAGED ? launch_tile<T, STAGED, ACT, PACK>(a, jobs, st)
-                                  : launch_tile<T, SINGLE, ACT, PACK>(a, jobs, st);
+        if (access == FLAT) return launch_flat<T, ACT, PACK>(a, jobs, st);
+        if (access == WIDE) return launch_tile<T, WIDE, ACT, PACK>(a, jobs, st);
+        if (access == PAIRS) return launch_tile<T, PAIRS, ACT, PACK>(a, jobs, st);
+        return launch_tile<T, sizeof(T) == 2 ? SHIFTED : SINGLE, ACT, PACK>(a, jobs, st);
     };
     if (type == TANGO_FP32) return go(float{});
     if (type == TANGO_BF16) return go(Bf16{});
@@ -582,13 +474,11 @@ static int fill(Rows8Args &a, int64_t rows, int64_t cols, int64_t group, int typ
 // What the matrices (with their leading dimensions) and the codes of a launch allow.
 static int access_of(const Rows8Args &a, int type, std::initializer_list<const void *> matrices, std::initializer_list<int64_t> lds,
                      std::initializer_list<const void *> codes, bool interleaved) {
-    bool wide = a.groups == 1 || a.group % 4 == 0, run = true, pieces = true;
-    for (const void *p : matrices) { wide &= aligned(p, 4 * element_bytes(type)); pieces &= aligned(p, 16); }
-    for (int64_t ld : lds) { wide &= a.rows == 1 || ld % 4 == 0; run &= a.rows == 1 || ld == a.cols; }
-    for (const void *p : codes) pieces &= aligned(p, 16);
+    bool wide = a.groups == 1 || a.group % 4 == 0, pairs = a.groups == 1 || a.group % 2 == 0, run = true;
+    for (const void *p : matrices) { wide &= aligned(p, 4 * element_bytes(type)); pairs &= aligned(p, 2 * element_bytes(type)); }
+    for (int64_t ld : lds) { wide &= a.rows == 1 || ld % 4 == 0; pairs &= a.rows == 1 || ld % 2 == 0; run &= a.rows == 1 || ld == a.cols; }
     if (wide && run && a.cols % a.group == 0 && a.group <= 128 && a.group >= 4 && (a.group & (a.group - 1)) == 0) return FLAT;
-    if (wide) return WIDE;
-    return run && pieces && !interleaved ? STAGED : SINGLE;
+    return wide ? WIDE : pairs ? PAIRS : SINGLE;
 }
 static bool fits_32(int64_t v) { return v < 0x7fffffffLL; }
 
@@ -625,9 +515,6 @@ extern "C" int tango_rows8_pack(const tango_rows8_job *jobs, int n_jobs, int64_t
         const int way = access_of(a, type, {j.x}, {j.ldx}, {j.q}, j.interleaved);
         if (way < access) access = way;
     }
-    // what one of them cannot do is done by none; the staged form asks for more than the wide one
-    for (int k = 0; k < n_jobs && access == STAGED; ++k)
-        if (!aligned(jobs[k].x, 16) || (rows > 1 && jobs[k].ldx != cols) || !aligned(jobs[k].q, 16) || jobs[k].interleaved) access = SINGLE;
     a.mode = mode; a.act = ACT_NONE; a.seed = seed; a.call = call;
     a.step = reinterpret_cast<const unsigned long long *>(step);
     return launch<false, true>(a, n_jobs, type, access, static_cast<cudaStream_t>(stream));
