@@ -519,7 +519,8 @@ typedef struct tango_edge_operands {
 } tango_edge_operands;
 int64_t tango_edge_attention_workspace_bytes(int pass, int64_t n_units, int heads, int d);
 
-/* CSC in, out [rows, heads, d] contiguous of `type`; stats (optional) [rows, heads, 2] fp32: largest z * log2(e), 1 / sum. */
+/* CSC in, out [rows, heads, d] contiguous of `type`; stats (optional) [rows, heads, 2] fp32: m, close to
+ * the largest z * log2(e), and 1 / sum of 2^(z log2(e) - m). */
 int tango_edge_attention(const int32_t *indptr, const int32_t *indices, int64_t n_rows, const tango_edge_plan *plan, int heads, int d,
                          const tango_edge_operands *x, float scale, void *out, int type, float *stats, void *ws, int64_t ws_bytes,
                          tango_stream_t stream);

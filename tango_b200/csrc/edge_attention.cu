@@ -44,7 +44,7 @@ struct AttnArgs {
     const float *sq, *so;                           // scales [rows, heads]
     const float2 *skv;                              // scales of k and v [rows, heads]
     float qscale;                                   // scale * log2(e)
-    float2 *stats;                                  // [rows, heads]: maximum of z * log2(e), 1 / sum
+    float2 *stats;                                  // [rows, heads]: reference of z * log2(e), 1 / sum
     float4 *record;                                 // [rows, heads], BY_DST writes and BY_SRC gathers: see there
     void *out_a, *out_b;
     int type;
@@ -200,9 +200,12 @@ __host__ __device__ inline int64_t partial_floats(int mode, int heads, int64_t l
     return (partial_heads(mode) * heads + 3) / 4 * 4 + partial_sums(mode) * ld;
 }
 
-// A softmax that is being added up: running maximum (of z * log2 e), sum, weighted sums of codes.  Before the first edge the
-// maximum is a number below all scores, so that nothing here has to ask for it.
-constexpr float kBelow = -3.0e38f;
+// A softmax that is being added up: reference (of z * log2 e), sum, weighted sums of codes.  The reference follows the maximum
+// only when a score passes it by kSlack: weights up to 2^kSlack are as exact in fp32 as weights up to 1, and what has been added
+// up is rescaled once or twice a row, where the exact maximum changes in one of a warp's 32 softmaxes in nearly every trip
+// through rows of some hundred edges.  Before the first edge the reference is a number below all scores, so that nothing here
+// has to ask for it.
+constexpr float kBelow = -3.0e38f, kSlack = 8.f;
 template <int VB> struct Running {
     float m = kBelow, l = 0.f;
     Pair acc[VB / 2];
@@ -252,9 +255,11 @@ __device__ __forceinline__ void softmax_step(Running<VB> &r, const float (&z)[U]
     float top = r.m;
 #pragma unroll
     for (int u = 0; u < U; ++u) top = fmaxf(top, z[u]);
-    if (__any_sync(0xffffffffu, top > r.m)) {       // seldom after the first edges of a row
-        r.scale(exp2_fast(r.m - top));
-        r.m = top;
+    const bool passed = top > r.m + kSlack;
+    if (__any_sync(0xffffffffu, passed)) {
+        const float to = passed ? top : r.m;
+        r.scale(exp2_fast(r.m - to));
+        r.m = to;
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -265,10 +270,13 @@ __device__ __forceinline__ void softmax_step(Running<VB> &r, const float (&z)[U]
     }
 }
 
-template <int MODE> struct InFlight { static constexpr int U = 2; };
+// Edges of a slot in one trip and blocks an SM: what is loaded one trip ahead hides the way to L2, against the registers that it
+// takes.  Forward / by destination / by source, us, 20 M edges of 4 x 32: 2, 2, 2 edges with 6, 4, 4 blocks 605 / 755 / 849;
+// 3, 3, 3 with 5, 3, 3 572 / 788 / 886; 4, 4, 4 with 6, 4, 4 609 / 693 / 814; as here 544 / 681 / 790.
+template <int MODE> struct InFlight { static constexpr int U = MODE == FORWARD ? 4 : 3, kBlocks = MODE == FORWARD ? 5 : 4; };
 
 template <int MODE, int VB, int P>
-__global__ void __launch_bounds__(kWarps * 32, MODE == FORWARD ? 6 : 4) attn_kernel(const __grid_constant__ AttnArgs a) {
+__global__ void __launch_bounds__(kWarps * 32, InFlight<MODE>::kBlocks) attn_kernel(const __grid_constant__ AttnArgs a) {
     constexpr int U = InFlight<MODE>::U;
     const int lane = threadIdx.x & 31;
     // ---- what this warp works on
@@ -387,7 +395,7 @@ __global__ void __launch_bounds__(kWarps * 32, MODE == FORWARD ? 6 : 4) attn_ker
                 add_codes_twice<VB>(run.acc, acc2, t.a[u], pair(pdk, pdk), pair(pk, pk));
             }
         } else {
-            // record of a destination: scale * log2(e) * scale of q, maximum, scale of o / sum, delta / scale of o
+            // record of a destination: scale * log2(e) * scale of q, reference, scale of o / sum, delta / scale of o
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const float s = dot<VB, P>(fa, t.a[u], start, lane, chunk), dp = dot<VB, P>(fb, t.b[u], start, lane, chunk) * sb;
