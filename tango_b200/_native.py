@@ -8,6 +8,7 @@ import importlib.machinery
 import importlib.util
 import os
 import sys
+import threading
 
 import torch
 from torch.autograd.function import Function, once_differentiable
@@ -155,10 +156,36 @@ def graph(g):
     return handle
 
 
-def edge_graph(g):
-    """The same with the row schedules of the edge-attention kernels, made at the first call."""
+_edge_lock = threading.Lock()
+
+
+def _add_edge_schedules(g, handle, formats) -> None:
+    from .graph import EdgeSchedule
+    with _edge_lock:
+        for fmt in formats:
+            if not handle.has_edge_schedule(fmt):
+                plan = getattr(g, "_plans", {}).get(fmt)
+                indptr = (g.adj_csc if fmt == "csc" else g.adj_csr)[0]
+                sched = EdgeSchedule(indptr, g.num_edges(), getattr(plan, "row_order", None))
+                if indptr.is_cuda:          # the next call may come on another stream
+                    torch.cuda.current_stream(indptr.device).synchronize()
+                handle.set_edge_schedule(fmt, sched)
+
+
+def edge_graph(g, backward: bool):
+    """The same with the row schedules of the edge-attention kernels, made at the first call that needs them (which therefore
+    cannot be inside a captured CUDA graph)."""
     handle = graph(g)
-    if not handle.has_edge_schedules():
-        from .graph import EdgeSchedule
-        handle.set_edge_schedules(EdgeSchedule(g.adj_csc[0]), EdgeSchedule(g.adj_csr[0]))
+    formats = ("csc", "csr") if backward else ("csc",)
+    if not all(handle.has_edge_schedule(fmt) for fmt in formats):
+        _add_edge_schedules(g, handle, formats)
+    return handle
+
+
+def rows_graph(g):
+    """The same with the length of the longest row, which is found at the first call."""
+    handle = graph(g)
+    if not handle.knows_longest():
+        indptr = g.adj_csc[0]
+        handle.set_longest(int((indptr[1:] - indptr[:-1]).max()) if g.num_nodes() else 0)
     return handle

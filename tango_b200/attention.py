@@ -23,7 +23,8 @@ def edge_attention(g, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: 
     sums are fp32.  The backward pass computes the probabilities anew from the 8-bit tensors and two floats per node and head
     -- all that is kept -- with the incoming gradient rounded to 8 bits in the same way, and takes the rounding as the
     identity, as the other operators of this package do."""
-    return _native.call(_native.ops.edge_attention, _native.edge_graph(g), q, k, v, _scale(q, scale))
+    backward = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
+    return _native.call(_native.ops.edge_attention, _native.edge_graph(g, backward), q, k, v, _scale(q, scale))
 
 
 def edge_attention_rows(g, rows: torch.Tensor, q: torch.Tensor, k8: Packed8, v8: Packed8, scale: Optional[float] = None) -> torch.Tensor:
@@ -36,7 +37,7 @@ def edge_attention_rows(g, rows: torch.Tensor, q: torch.Tensor, k8: Packed8, v8:
         if q.dim() != 3 or tuple(t.shape) != (g.num_nodes(), *q.shape[1:]) or t.group != q.shape[2]:
             raise ValueError(f"edge_attention_rows: {name} must be pack8(x, {q.shape[-1]}) of an x [{g.num_nodes()}, "
                              f"{', '.join(map(str, q.shape[1:]))}], not of {tuple(t.shape)} in groups of {t.group}")
-    return _native.call(_native.ops.edge_attention_rows, _native.edge_graph(g), rows, q, k8.codes, k8.scales, v8.codes, v8.scales,
+    return _native.call(_native.ops.edge_attention_rows, _native.rows_graph(g), rows, q, k8.codes, k8.scales, v8.codes, v8.scales,
                         _scale(q, scale))
 
 

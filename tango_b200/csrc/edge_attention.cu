@@ -800,7 +800,8 @@ static int launch(AttnArgs a, const tango_edge_plan *plan, float *ws, int64_t ws
         a.rows = reinterpret_cast<const int4 *>(plan->rows);
         a.units = reinterpret_cast<const int4 *>(plan->units);
         a.n_units = plan->n_units; a.n_heavy = plan->n_heavy; a.n_long = plan->n_long;
-        if (!plan->rows || a.n_units < 0 || a.n_heavy < 0 || a.n_long < a.n_heavy || a.n_long > a.n_rows) return TANGO_EINVAL;
+        if (!plan->rows || a.n_heavy < 0 || a.n_units < a.n_heavy || a.n_long < a.n_heavy || a.n_long > a.n_rows) return TANGO_EINVAL;
+        if (a.n_heavy == 0 && a.n_units > 0) return TANGO_EINVAL;
         if (a.n_heavy > 0 && (!plan->units || !plan->heavy_first || !ws || ws_bytes < a.n_units * partial_floats(MODE, a.heads, a.ld) * 4))
             return TANGO_EINVAL;
         if (!aligned(plan->rows, 16) || !aligned(plan->units, 16) || !aligned(ws, 16)) return TANGO_EALIGN;

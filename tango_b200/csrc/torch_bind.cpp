@@ -63,7 +63,6 @@ static EdgeSchedule edge_schedule(const py::object &s) {
     out.n_long = s.attr("n_long").cast<int64_t>();
     out.n_units = s.attr("n_units").cast<int64_t>();
     out.n_heavy = s.attr("n_heavy").cast<int64_t>();
-    out.longest = s.attr("longest").cast<int64_t>();
     out.present = true;
     return out;
 }
@@ -90,11 +89,12 @@ PYBIND11_MODULE(_torch_ops, m) {
             g->csc = std::move(csc); g->csr = std::move(csr); g->src = std::move(src); g->dst = std::move(dst); g->n_nodes = n;
             return g;
         }))
-        .def("has_edge_schedules", [](const Graph &g) { return g.csc->edge_sched.present && g.csr->edge_sched.present; })
-        .def("set_edge_schedules", [](Graph &g, const py::object &csc, const py::object &csr) {
-            g.csc->edge_sched = edge_schedule(csc);
-            g.csr->edge_sched = edge_schedule(csr);
-        });
+        .def("has_edge_schedule", [](const Graph &g, const std::string &fmt) { return g.dir(fmt == "csr").edge_sched.present; })
+        .def("set_edge_schedule", [](Graph &g, const std::string &fmt, const py::object &s) {
+            (fmt == "csr" ? g.csr : g.csc)->edge_sched = edge_schedule(s);
+        })
+        .def("knows_longest", [](const Graph &g) { return g.longest >= 0; })
+        .def("set_longest", [](Graph &g, int64_t n) { g.longest = n; });
 
     m.def("set_rounding", [](int gemm, int quantize, uint64_t seed) {
         settings().mode_gemm = gemm; settings().mode_quantize = quantize; settings().seed = seed;

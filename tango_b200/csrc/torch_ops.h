@@ -60,7 +60,7 @@ struct Schedule {
 // The row schedule of the edge-attention kernels (tango_b200.graph.EdgeSchedule).
 struct EdgeSchedule {
     Tensor rows, units, heavy_first;
-    int64_t n_long = 0, n_units = 0, n_heavy = 0, longest = 0;
+    int64_t n_long = 0, n_units = 0, n_heavy = 0;
     bool present = false;
 };
 
@@ -78,7 +78,7 @@ struct Direction {
 struct Graph {
     std::shared_ptr<Direction> csc, csr;
     Tensor src, dst;
-    int64_t n_nodes = 0;
+    int64_t n_nodes = 0, longest = -1;   // longest: slots of the longest CSC row, where that is known
     const Direction &dir(bool reverse) const { return reverse ? *csr : *csc; }
     int64_t n_edges() const { return src.numel(); }
 };

@@ -232,7 +232,7 @@ Tensor edge_attention_fn(const GraphPtr &g, const Tensor &q, const Tensor &k, co
     }
     require(q.size(0) == g->n_nodes, "one row of q, k and v per node expected");
     require(g->csc->indptr.device() == q.device(), "graph and features must be on the same GPU");
-    require(std::isfinite(scale), "finite scale expected");
+    require(std::isfinite((float)scale), "finite scale expected");
     const int heads = (int)q.size(1), d = (int)q.size(2);
     const int64_t n = q.size(0);
     Tensor out, saved;
@@ -289,7 +289,7 @@ Tensor edge_attention_rows(const GraphPtr &g, const Tensor &rows_, const Tensor 
         require(t->q.dim() == 2 && t->q.size(0) == n && t->q.size(1) == tango_rows8_ld(heads * d, d) && t->scale.numel() == n * heads,
                 "keys and values packed with one row per node and one group per head expected");
     }
-    require(std::isfinite(scale), "finite scale expected");
+    require(std::isfinite((float)scale), "finite scale expected");
     const Raw raw;
     const c10::cuda::CUDAGuard guard(q.device());
     const Tensor out = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
@@ -297,7 +297,7 @@ Tensor edge_attention_rows(const GraphPtr &g, const Tensor &rows_, const Tensor 
     const Tensor rows = rows_.to(at::kLong).contiguous();
     const Matrix qm = matrix(q);
     const Direction &in = g->dir(false);
-    const int splits = tango_edge_attention_rows_splits(r, in.edge_sched.present ? in.edge_sched.longest : g->n_edges());
+    const int splits = tango_edge_attention_rows_splits(r, g->longest >= 0 ? g->longest : g->n_edges());
     const int64_t bytes = tango_edge_attention_rows_workspace_bytes(r, splits, (int)heads, (int)d);
     if (bytes < 0) check((int)bytes, "edge_attention_rows");
     const Tensor ws = at::empty({bytes}, q.options().dtype(at::kByte));

@@ -348,30 +348,38 @@ class EdgeSchedule:
     48 (head of the row order first, so that the walk of the longest is hidden), on 1.2 M edges 160 to 200 us against 96 with
     up to 160.  Units keep the longest walk short on small graphs (128 edges) and their partial results few on large ones."""
 
-    def __init__(self, indptr: torch.Tensor):
-        ip = indptr.long()
-        length = ip[1:] - ip[:-1]
+    def __init__(self, indptr: torch.Tensor, nnz: Optional[int] = None, order: Optional[torch.Tensor] = None):
+        """nnz and order (the rows by decreasing length, SpmmSchedule.row_order) where they are known already."""
+        length = indptr[1:] - indptr[:-1]
         n, dev = length.numel(), indptr.device
-        order = torch.argsort(length, descending=True, stable=True)
-        nnz = int(ip[-1]) if n else 0
+        if order is None:
+            order = torch.argsort(length, descending=True, stable=True)
+        order = order.to(torch.int32)
+        if nnz is None:
+            nnz = int(indptr[-1]) if n else 0
         team = min(512, max(48, nnz // 8192))
         unit = 128
         while unit < 1024 and unit * 16384 < nnz:
             unit *= 2
         self.threshold = 2 * unit
-        self.rows = torch.stack([order, ip[:-1][order], ip[1:][order], torch.zeros_like(order)], 1).to(torch.int32).contiguous()
-        counts = torch.stack([(length > team).sum(), (length > self.threshold).sum(),
-                              length.max() if n else torch.zeros((), dtype=torch.int64, device=dev)]).tolist()
-        self.n_heavy, self.longest = counts[1], counts[2]
-        self.n_long = max(counts[0], self.n_heavy)
-        heavy = order[:self.n_heavy]
-        n_units = (length[heavy] + unit - 1) // unit
+        self.rows = torch.stack([order, indptr[:-1][order], indptr[1:][order], torch.zeros_like(order)], 1)
+        self.n_long = self.n_heavy = self.longest = self.n_units = 0
+        if n:
+            ranked = torch.neg(length[order])          # ascending
+            n_long, n_heavy = torch.searchsorted(ranked, torch.tensor([-team, -self.threshold], device=dev, dtype=ranked.dtype)).tolist()
+            self.longest, self.n_heavy, self.n_long = -int(ranked[0]), n_heavy, max(n_long, n_heavy)
+        if self.n_heavy == 0:
+            self.heavy_first = torch.zeros(1, dtype=torch.int32, device=dev)
+            self.units = torch.zeros((0, 4), dtype=torch.int32, device=dev)
+            return
+        heavy = self.rows[:self.n_heavy].long()
+        n_units = (heavy[:, 2] - heavy[:, 1] + unit - 1) // unit
         last = torch.cumsum(n_units, 0)
         self.heavy_first = torch.cat([torch.zeros(1, dtype=torch.int64, device=dev), last]).to(torch.int32)
         of = torch.repeat_interleave(torch.arange(self.n_heavy, device=dev), n_units)
         place = torch.arange(of.numel(), device=dev) - (last - n_units)[of]
-        begin = ip[heavy[of]] + place * unit
-        self.units = torch.stack([heavy[of], begin, torch.minimum(begin + unit, ip[heavy[of] + 1]), place], 1).to(torch.int32).contiguous()
+        begin = heavy[of, 1] + place * unit
+        self.units = torch.stack([heavy[of, 0], begin, torch.minimum(begin + unit, heavy[of, 2]), place], 1).to(torch.int32).contiguous()
         self.n_units = int(self.units.shape[0])
 
 

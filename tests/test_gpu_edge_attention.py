@@ -265,8 +265,9 @@ def test_refusals(cuda):
                 (q.flatten(1), k.flatten(1), v.flatten(1))):
         with pytest.raises(AssertionError):
             T.edge_attention(g, *bad)
-    with pytest.raises(AssertionError, match="finite"):
-        T.edge_attention(g, q, k, v, math.inf)
+    for scale in (math.inf, math.nan, 1e300):
+        with pytest.raises(AssertionError, match="finite"):
+            T.edge_attention(g, q, k, v, scale)
     k8, v8 = T.pack8(k, 8), T.pack8(v, 8)
     ids = torch.tensor([1, 2], device="cuda")
     for rows, t in ((ids.float(), q[:2]), (ids[:1], q[:2]), (ids.cpu(), q[:2]), (ids.view(2, 1), q[:2])):
@@ -360,6 +361,69 @@ def test_streams_and_captured_graphs(cuda):
             graph.replay()
             for a, b in zip(outs, run(g, *new)):
                 assert torch.equal(a, b)
+
+
+def test_first_calls_on_two_streams_and_from_two_threads(cuda):
+    """The row schedules are made by whoever comes first; a call on another stream right behind it finds them whole."""
+    import threading
+    import tango_b200 as T
+    want, graphs = None, [make_graph("hubs") for _ in range(3)]
+    tensors = case(graphs[0], 4, 16)
+    want = run(graphs[0], *tensors)
+    g = graphs[1]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    res = [None, None]
+    for i, s in enumerate(streams):
+        with torch.cuda.stream(s):
+            res[i] = run(g, *tensors)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for r in res for a, b in zip(r, want))
+    g, res = graphs[2], [None, None]
+
+    def work(i):
+        with torch.cuda.stream(streams[i]):
+            res[i] = run(g, *tensors)
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert all(torch.equal(a, b) for r in res for a, b in zip(r, want))
+
+
+def test_offsets_beyond_32_bits(cuda):
+    """Codes, outputs and gradients of more than 2^32 bytes: rows at the far end of the tensors."""
+    import tango_b200 as T
+    from tango_b200.graph import Graph
+    n, h, d = 4_300_000, 8, 64          # 2.2e9 elements a tensor, 4.4e9 bytes of interleaved codes
+    if torch.cuda.mem_get_info()[0] < 100 << 30:
+        pytest.skip("needs 100 GB")
+    ends = torch.tensor([n - 1, n - 2, 5, n - 7, 3, n // 2], device="cuda")
+    src, dst = ends.repeat(6), ends.repeat_interleave(6)
+    g = Graph(src, dst, n)
+    small = Graph(torch.arange(6, device="cuda").repeat(6), torch.arange(6, device="cuda").repeat_interleave(6), 6)
+    parts = [randn(i, 6, h, d, dtype=torch.bfloat16) for i in range(4)]
+    want = run(small, *parts)
+    big = []
+    for p in parts:
+        t = torch.zeros(n, h, d, dtype=torch.bfloat16, device="cuda")
+        t[ends] = p
+        big.append(t)
+    leaves = [t.requires_grad_() for t in big[:3]]
+    out = T.edge_attention(g, *leaves)
+    got = [out.detach()[ends]]
+    grads = torch.autograd.grad(out, leaves, big[3])
+    got += [t[ends] for t in grads]
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    del out, grads
+    k8, v8 = T.pack8(big[1], d), T.pack8(big[2], d)
+    with torch.no_grad():
+        rows = T.edge_attention_rows(g, ends, parts[0], k8, v8)
+    check([rows], [want[0].double()], [want[0].double().abs() * 2.0 ** -7 + 1e-3], torch.bfloat16)
+    assert torch.equal(k8.unpack()[ends], T.pack8(parts[1], d).unpack())
 
 
 def test_stochastic_rounding_draws_anew(cuda):

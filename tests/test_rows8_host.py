@@ -87,6 +87,8 @@ def test_attention_arguments_are_checked_before_any_launch():
     assert forward(plan=_ref(plan)) == -1 and forward(plan=_ref(plan), ws=0x1000, nbytes=16) == -1
     assert forward(plan=_ref(_Plan(0x10, 0, 0x20, 3, 0x40, 1)), ws=0x1000, nbytes=1 << 20) == -1
     assert forward(plan=_ref(_Plan(0x10, 5, 0x20, 0, 0x40, 0))) == -1
+    assert forward(plan=_ref(_Plan(0x10, 2, 0x20, 3, 0x40, 0))) == -1        # units of no row
+    assert forward(plan=_ref(_Plan(0x10, 2, 0x20, 1, 0x40, 2)), ws=0x1000, nbytes=1 << 20) == -1
     assert forward(plan=_ref(_Plan(None, 2, None, 0, None, 0))) == -1 and forward(plan=_ref(_Plan(0x18, 2, None, 0, None, 0))) == -2
     def by_dst(x=x(), stats=0x4000, record=0x4000, qo=0x6000):
         return lib.tango_edge_attention_bwd_dst(0x100, 0x200, 4, None, 2, 16, x, 1.0, stats, 0x3000, 0, record, qo, None, 0, None)
@@ -176,6 +178,8 @@ def test_units_cover_every_long_row_once(scale):
     indptr = torch.zeros(lengths.numel() + 1, dtype=torch.int32)
     indptr[1:] = lengths.cumsum(0)
     s = EdgeSchedule(indptr)
+    same = EdgeSchedule(indptr, int(indptr[-1]), torch.argsort(lengths, descending=True, stable=True).int())
+    assert torch.equal(s.rows, same.rows) and torch.equal(s.units, same.units) and s.n_long == same.n_long
     assert s.longest == 3000 * scale
     rows = s.rows.long()
     length = rows[:, 2] - rows[:, 1]
