@@ -31,6 +31,7 @@ struct Rows8Args {
     int64_t ldq;
     FastDiv by_groups;
     int wide;                     // 2^31 groups or more
+    int jobs;                     // matrices: blocks take them in turn, so that the runs of interleaved ones meet in L2
     int mode, act;
     uint64_t seed, call;
     const unsigned long long *step;
@@ -226,9 +227,9 @@ __device__ __forceinline__ void store_group(T *p, int n, const float (&v)[R * 4]
 template <class T, int ACCESS, int LPG, int R, bool ACT>
 __global__ void __launch_bounds__(kBlock) rows8_pack_kernel(const __grid_constant__ Rows8Args a) {
     constexpr int U = Tile<LPG, R>::U, NG = Tile<LPG, R>::kGroups;
-    const int job = blockIdx.y, lane = threadIdx.x % LPG;
+    const int job = blockIdx.x % a.jobs, lane = threadIdx.x % LPG;
     const T *x = static_cast<const T *>(a.x[job]);
-    const int64_t first = (int64_t)blockIdx.x * (NG * U) + threadIdx.x / LPG;
+    const int64_t first = (int64_t)(blockIdx.x / a.jobs) * (NG * U) + threadIdx.x / LPG;
     float v[U][R * 4];
     Where w[U];
 #pragma unroll
@@ -330,8 +331,8 @@ __global__ void __launch_bounds__(kBlock) rows8_unpack_kernel(const __grid_const
 template <class T, int GL, bool ACT, bool PACK>
 __global__ void __launch_bounds__(kBlock) rows8_flat_kernel(const __grid_constant__ Rows8Args a) {
     constexpr int R = 4;                        // GL: lanes of a group
-    const int job = blockIdx.y;
-    const int64_t total = a.rows * a.cols, at = ((int64_t)blockIdx.x * kBlock * R + (threadIdx.x & ~31) * R + (threadIdx.x & 31)) * 4;
+    const int job = blockIdx.x % a.jobs;
+    const int64_t total = a.rows * a.cols, at = ((int64_t)(blockIdx.x / a.jobs) * kBlock * R + (threadIdx.x & ~31) * R + (threadIdx.x & 31)) * 4;
     float v[R * 4];
     uint32_t word[R];
     float s[R];
@@ -405,9 +406,9 @@ __global__ void __launch_bounds__(kBlock) rows8_flat_kernel(const __grid_constan
 
 template <class T, int ACCESS, bool ACT, bool PACK, int LPG, int R>
 static int launch_kernel(const Rows8Args &a, int jobs, cudaStream_t st) {
-    const int64_t blocks = ceil_div(a.items, Tile<LPG, R>::kItems);
+    const int64_t blocks = ceil_div(a.items, Tile<LPG, R>::kItems) * jobs;
     if (blocks > 0x7fffffffLL) return TANGO_ESIZE;
-    const dim3 grid((unsigned)blocks, (unsigned)jobs);
+    const unsigned grid = (unsigned)blocks;
     if constexpr (PACK) rows8_pack_kernel<T, ACCESS, LPG, R, ACT><<<grid, kBlock, 0, st>>>(a);
     else rows8_unpack_kernel<T, ACCESS, LPG, R, ACT><<<grid, kBlock, 0, st>>>(a);
     TANGO_LAUNCH_CHECK();
@@ -416,9 +417,9 @@ static int launch_kernel(const Rows8Args &a, int jobs, cudaStream_t st) {
 
 template <class T, bool ACT, bool PACK, int GL>
 static int launch_flat(const Rows8Args &a, int jobs, cudaStream_t st) {
-    const int64_t blocks = ceil_div(a.rows * a.cols, kBlock * 16);
+    const int64_t blocks = ceil_div(a.rows * a.cols, kBlock * 16) * jobs;
     if (blocks > 0x7fffffffLL) return TANGO_ESIZE;
-    rows8_flat_kernel<T, GL, ACT, PACK><<<dim3((unsigned)blocks, (unsigned)jobs), kBlock, 0, st>>>(a);
+    rows8_flat_kernel<T, GL, ACT, PACK><<<(unsigned)blocks, kBlock, 0, st>>>(a);
     TANGO_LAUNCH_CHECK();
     return TANGO_OK;
 }
@@ -448,7 +449,8 @@ static int launch_tile(const Rows8Args &a, int jobs, cudaStream_t st) {
 }
 
 template <bool ACT, bool PACK>
-static int launch(const Rows8Args &a, int jobs, int type, int access, cudaStream_t st) {
+static int launch(Rows8Args a, int jobs, int type, int access, cudaStream_t st) {
+    a.jobs = jobs;
     const auto go = [&](auto t) {
         typedef decltype(t) T;
         if (access == FLAT) return launch_flat<T, ACT, PACK>(a, jobs, st);
