@@ -349,13 +349,21 @@ __global__ void __launch_bounds__(kBlock) rows8_flat_kernel(const __grid_constan
     if constexpr (PACK) {
         const bool keep = !ACT || a.q[job];
         if (keep) {
+            float top[R];
 #pragma unroll
             for (int r = 0; r < R; ++r) {
-                float top = max_abs3(v[4 * r], v[4 * r + 1], 0.f);
-                top = max_abs3(v[4 * r + 2], v[4 * r + 3], top);
+                top[r] = max_abs3(max_abs3(v[4 * r], v[4 * r + 1], v[4 * r + 2]), v[4 * r + 3], 0.f);
 #pragma unroll
-                for (int o = GL / 2; o > 0; o >>= 1) top = max_or_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
-                s[r] = group_scale(top);
+                for (int o = GL / 2; o > 0; o >>= 1) top[r] = max_or_nan(top[r], __shfl_xor_sync(0xffffffffu, top[r], o));
+            }
+            if constexpr (GL >= 4) {        // four lanes of a group divide for one of its four pieces each
+                const int k = threadIdx.x & 3;
+                const float mine = group_scale(k < 2 ? (k == 0 ? top[0] : top[1]) : (k == 2 ? top[2] : top[3]));
+#pragma unroll
+                for (int r = 0; r < R; ++r) s[r] = __shfl_sync(0xffffffffu, mine, (threadIdx.x & 28) | r);
+            } else {
+#pragma unroll
+                for (int r = 0; r < R; ++r) s[r] = group_scale(top[r]);
             }
             if (a.mode == TANGO_ROUND_NEAREST) {
 #pragma unroll
