@@ -596,7 +596,7 @@ struct RowsArgs {
     uint64_t seed, call;
     const unsigned long long *step;
 };
-constexpr int kRowChunk = 256;    // edges below which a row is not cut: eight trips of a block of F = 128
+constexpr int kRowChunk = 256;    // edges below which a row is not cut: four trips of a block of F = 128
 
 __host__ __device__ inline int row_chunk(int len, int splits) {
     const int c = (len + splits - 1) / splits;
@@ -633,8 +633,8 @@ __device__ __forceinline__ Codes<VB> encode_query(const RowsArgs &a, int64_t r, 
 }
 
 template <int VB, int P>
-__global__ void __launch_bounds__(kRowWarps * 32, 6) attn_rows_kernel(const __grid_constant__ RowsArgs a) {
-    constexpr int U = 2;
+__global__ void __launch_bounds__(kRowWarps * 32, 5) attn_rows_kernel(const __grid_constant__ RowsArgs a) {
+    constexpr int U = 4;
     __shared__ float s_acc[kRowWarps][32 * VB];
     __shared__ float2 s_ml[kRowWarps][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -900,7 +900,7 @@ extern "C" int tango_edge_attention_rows_splits(int64_t n_rows, int64_t longest)
     if (n_rows < 0 || longest < 0) return TANGO_EINVAL;
     if (n_rows == 0 || longest <= kRowChunk) return 1;
     // Most of a row's blocks find nothing to do unless it is a long one, and take their turn all the same: 1024 rows of 20 M
-    // edges (62 in the middle, 2021 at most), 4 x 32, take 28 us with one block a row, 19 with 4, 22 with 8, 32 with 16.
+    // edges (62 in the middle, 2021 at most), 4 x 32, take 39 us with one block a row, 26 with 4, 28 with 8 (from HBM).
     const int64_t want = ceil_div(longest, kRowChunk), most = 4096 / n_rows < 64 ? 4096 / n_rows : 64;
     return (int)(want < most ? want : most < 1 ? 1 : most);
 }

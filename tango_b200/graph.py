@@ -361,7 +361,8 @@ class EdgeSchedule:
         unit = 128
         while unit < 1024 and unit * 16384 < nnz:
             unit *= 2
-        self.threshold = 2 * unit
+        # a row below it is one warp's; on large graphs a longer walk is hidden, and fewer rows have parts to merge
+        self.threshold = 2 * unit if unit < 1024 else 4 * unit
         self.rows = torch.stack([order, indptr[:-1][order], indptr[1:][order], torch.zeros_like(order)], 1)
         self.n_long = self.n_heavy = self.longest = self.n_units = 0
         if n:
