@@ -10,8 +10,22 @@
 // are the same ones).  delta is not needed beforehand: dq = scale * (sum p dp k - delta sum p k), so one walk
 // gathers delta and both sums, and what the forward pass has to keep is the 8-bit rows and two floats per row and head.
 //
-// Sums are fp32, in one order per row length and shape (no atomics).  What bounds these kernels is the gather of 2 F bytes
-// per edge through L2 together with the instructions that turn codes into floats and add them up.
+// Sums are fp32, in one order per row length and schedule (no atomics).
+//
+// What bounds these kernels is the gather through L1 and L2: an edge brings 2 F bytes of codes and 8 H bytes of scales (16 H by
+// source), 5.8 GB for 20 M edges of 4 x 32.  On 232,965 nodes they take 535 us forward, 669 by destination and 785 by source (10.8,
+// 8.6 and 8.2 TB/s of gathered bytes; 20 to 30 % of the sectors miss L2, whose near half holds no table of 60 MB), on 114.6 M edges
+// of 4 x 16 1361 us forward (13.5 TB/s, issue slots two thirds busy).  Without the weighted sums (leaving out the conversion and
+// addition of v) the forward passes would take 527 and 1254 us where they took 615 and 1537: their arithmetic is mostly hidden, and
+// matrix instructions for it would buy little.
+//   * k and v (in the backward pass q and the gradient, which the pass by destination lays out for the one by source) lie in turns
+//     of one lane's codes, so that a 32-byte load brings both: 20 M edges 631 -> 603 us forward, by source 913 -> 861.
+//   * The loads of a lane's next edges are issued before the present ones are worked on (InFlight), and none depends on a
+//     condition: slots behind a row's end read its last edge again, without weight.
+//   * Codes become floats by placing the biased byte in the mantissa of 2^23, two at a time in packed fp32 arithmetic; dot products
+//     of codes are exact in integers.
+//   * Persistent warps that share out the short rows and fetch the next row's bounds early lost to the hardware's order of blocks
+//     (603 -> 713 us at best: unequal rows), cache hints on outputs, indices and the table changed nothing.
 //
 // A lane holds VB neighbouring codes of one head (16, less for narrow heads), P lanes a head, L = P * (heads of a block)
 // lanes an edge, and a warp as many edges side by side (slots) as fit.  None of these has to be a power of two: three heads of

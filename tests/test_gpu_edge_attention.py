@@ -363,6 +363,31 @@ def test_streams_and_captured_graphs(cuda):
                 assert torch.equal(a, b)
 
 
+def test_captured_backward_beside_a_living_graph_of_the_same_leaves(cuda):
+    import tango_b200 as T
+    g = make_graph("hubs")
+    q, k, v, o = case(g, 2, 16)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    want = run(g, q, k, v, o)[1:]
+    side = torch.cuda.Stream()          # (on the default stream PyTorch refuses to capture beside it, whatever the operator)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        alive = T.edge_attention(g, *leaves)
+        alive.backward(o, retain_graph=True)
+        for t in leaves:
+            t.grad.zero_()              # the captured pass adds to these
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        T.edge_attention(g, *leaves).backward(o)
+    for n in (1, 2):
+        graph.replay()
+        assert all(torch.equal(t.grad, n * b) for t, b in zip(leaves, want))
+    alive.backward(o)
+    torch.cuda.synchronize()
+    assert all(torch.equal(t.grad, 3 * b) or torch.allclose(t.grad, 3 * b, rtol=1e-6) for t, b in zip(leaves, want))
+
+
 def test_first_calls_on_two_streams_and_from_two_threads(cuda):
     """The row schedules are made by whoever comes first; a call on another stream right behind it finds them whole."""
     import threading
