@@ -132,13 +132,13 @@ template <int LPG, int R> struct Tile {
     static constexpr int kElements = kItems * LPG * R * 4;
 };
 
-// How the elements are reached: in one run, four or two at a time, one at a time, or (two-byte elements of any alignment) in
-// aligned pieces that are shifted into place.
-enum { SHIFTED = 0, SINGLE = 1, PAIRS = 2, WIDE = 4, FLAT = 8 };
+// How the elements are reached: in aligned pieces of four that are shifted into place (rows of any pitch), four at a time, or in one
+// run.
+enum { SHIFTED = 0, WIDE = 4, FLAT = 8 };
 
 // ---- a lane's elements of a group: four neighbours at lane * 4, (lane + LPG) * 4, ..
-// Two-byte elements of any alignment come in the aligned 8-byte pieces that hold them; a lane's four straddle its own piece and
-// the next lane's.  Single accesses of two bytes each took 373 us where these take 258 (169343 x 601 bf16, SiLU, forward).
+// In rows of any pitch they come in the aligned pieces of four (16 or 8 bytes) that hold them: a lane's four straddle its own piece
+// and the next lane's, and go out likewise.  Single accesses took 373 us where these take 260 (169343 x 601 bf16, SiLU, forward).
 template <int LPG>
 __device__ __forceinline__ uint64_t from_lane(uint64_t v, int lane) { return __shfl_sync(0xffffffffu, v, ((threadIdx.x & 31) & ~(LPG - 1)) + lane); }
 
@@ -146,9 +146,52 @@ __device__ __forceinline__ uint64_t from_lane(uint64_t v, int lane) { return __s
 template <class T, int ACCESS, int LPG, int R>
 __device__ __forceinline__ void load_group(const T *p, int n, const T *begin, const T *end, float (&v)[R * 4]) {
     const int lane = threadIdx.x % LPG;
-    if constexpr (ACCESS != SHIFTED) {
+    if constexpr (ACCESS == WIDE) {
 #pragma unroll
-        for (int r = 0; r < R; ++r) load4<T, ACCESS>(p + (lane + r * LPG) * 4, n - (lane + r * LPG) * 4, v + 4 * r);
+        for (int r = 0; r < R; ++r) load4<T, WIDE>(p + (lane + r * LPG) * 4, n - (lane + r * LPG) * 4, v + 4 * r);
+    } else if constexpr (sizeof(T) == 4) {
+        const int skip = (int)(reinterpret_cast<uintptr_t>(p) >> 2 & 3), pieces = n > 0 ? (n + skip + 3) / 4 : 0;
+        const float *first = reinterpret_cast<const float *>(p) - skip;
+        const bool inside = first >= reinterpret_cast<const float *>(begin) && first + pieces * 4 <= reinterpret_cast<const float *>(end);
+        const int from = ((threadIdx.x & 31) & ~(LPG - 1)) + ((lane + 1) & (LPG - 1));
+        float w[R + 1][4];
+#pragma unroll
+        for (int r = 0; r <= R; ++r) {
+            const int k = lane + r * LPG;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[r][i] = 0.f;
+            if (r == R && lane > 0) continue;
+            if (k >= pieces) continue;
+            if (inside) {
+                const float4 t = __ldg(reinterpret_cast<const float4 *>(first) + k);
+                w[r][0] = t.x; w[r][1] = t.y; w[r][2] = t.z; w[r][3] = t.w;
+            } else {                    // the matrix begins or ends inside a piece
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int e = k * 4 - skip + i;
+                    if (e >= 0 && e < n) w[r][i] = to_float(p[e]);
+                }
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            float all[7];          // this lane's piece, and the first three elements of the next lane's
+#pragma unroll
+            for (int i = 0; i < 4; ++i) all[i] = w[r][i];
+#pragma unroll
+            for (int i = 0; i < 3; ++i) all[4 + i] = __shfl_sync(0xffffffffu, lane == 0 ? w[r + 1][i] : w[r][i], from);
+            const int left = n - (lane + r * LPG) * 4;
+            float half[6];
+#pragma unroll
+            for (int i = 0; i < 6; ++i) half[i] = skip & 1 ? all[i + 1] : all[i];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[4 * r + i] = skip & 2 ? half[i + 2] : half[i];
+            if (left < 4) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (i >= left) v[4 * r + i] = 0.f;
+            }
+        }
     } else {
         const int off = (int)(reinterpret_cast<uintptr_t>(p) & 7), bits = off * 8, pieces = n > 0 ? (n * 2 + off + 7) / 8 : 0;
         const char *first = reinterpret_cast<const char *>(p) - off;
@@ -189,9 +232,44 @@ __device__ __forceinline__ void load_group(const T *p, int n, const T *begin, co
 template <class T, int ACCESS, int LPG, int R>
 __device__ __forceinline__ void store_group(T *p, int n, const float (&v)[R * 4]) {
     const int lane = threadIdx.x % LPG;
-    if constexpr (ACCESS != SHIFTED) {
+    if constexpr (ACCESS == WIDE) {
 #pragma unroll
-        for (int r = 0; r < R; ++r) store4<T, ACCESS>(p + (lane + r * LPG) * 4, n - (lane + r * LPG) * 4, v + 4 * r);
+        for (int r = 0; r < R; ++r) store4<T, WIDE>(p + (lane + r * LPG) * 4, n - (lane + r * LPG) * 4, v + 4 * r);
+    } else if constexpr (sizeof(T) == 4) {
+        // the same for four-byte elements, by whole elements: with accesses of 4 bytes unpacking 232965 x 601 took 355 us, 139 so
+        const int skip = (int)(reinterpret_cast<uintptr_t>(p) >> 2 & 3), from = ((threadIdx.x & 31) & ~(LPG - 1)) + ((lane + LPG - 1) & (LPG - 1));
+        float *first = reinterpret_cast<float *>(p) - skip;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            float all[7];          // the last three elements of the lane before, and this one's
+#pragma unroll
+            for (int i = 1; i < 4; ++i) {
+                const float mine = lane == LPG - 1 ? (r > 0 ? v[r > 0 ? 4 * r - 4 + i : 0] : 0.f) : v[4 * r + i];
+                all[i - 1] = __shfl_sync(0xffffffffu, mine, from);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) all[3 + i] = v[4 * r + i];
+            float half[6], piece[4];
+#pragma unroll
+            for (int i = 0; i < 6; ++i) half[i] = skip & 1 ? all[i] : all[i + 1];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) piece[i] = skip & 2 ? half[i] : half[i + 2];
+            const int k = lane + r * LPG, e = k * 4 - skip;
+            if (e >= 0 && e + 4 <= n) {
+                reinterpret_cast<float4 *>(first)[k] = make_float4(piece[0], piece[1], piece[2], piece[3]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (e + i >= 0 && e + i < n) from_float(piece[i], p[e + i]);
+            }
+        }
+        if (lane == LPG - 1) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int e = (R * LPG - 1) * 4 + i;
+                if (i >= 4 - skip && e < n) from_float(v[4 * R - 4 + i], p[e]);
+            }
+        }
     } else {
         const int off = (int)(reinterpret_cast<uintptr_t>(p) & 7), bits = off * 8, skip = off / 2;
         uint64_t *first = reinterpret_cast<uint64_t *>(reinterpret_cast<char *>(p) - off);
@@ -229,59 +307,81 @@ __device__ __forceinline__ void store_group(T *p, int n, const float (&v)[R * 4]
     }
 }
 
+template <int ACCESS> constexpr bool kAhead = ACCESS != SHIFTED;
+constexpr int kAheadBlocks = 16;        // blocks an SM of the kernels that take several tiles
+
 template <class T, int ACCESS, int LPG, int R, bool ACT>
 __global__ void __launch_bounds__(kBlock) rows8_pack_kernel(const __grid_constant__ Rows8Args a) {
     constexpr int U = Tile<LPG, R>::U, NG = Tile<LPG, R>::kGroups;
     const int job = blockIdx.x % a.jobs, lane = threadIdx.x % LPG;
     const T *x = static_cast<const T *>(a.x[job]);
-    const int64_t first = (int64_t)(blockIdx.x / a.jobs) * (NG * U) + threadIdx.x / LPG;
-    float v[U][R * 4];
-    Where w[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const int64_t i = first + u * NG;
-        w[u] = {0, 0, 0, 0};
-        if (i < a.items) w[u] = locate(a, i, a.ldx[job]);
-        load_group<T, ACCESS, LPG, R>(x + w[u].x, w[u].n, x, x + (a.rows - 1) * a.ldx[job] + a.cols, v[u]);
-    }
     const int run = a.run[job];
+    float ahead[U][R * 4];
+    Where to_come[U];
+    const auto fetch = [&](int64_t tile) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        float top = 0.f;
+        for (int u = 0; u < U; ++u) {
+            const int64_t i = tile * (NG * U) + threadIdx.x / LPG + u * NG;
+            to_come[u] = {0, 0, 0, 0};
+            if (i < a.items) to_come[u] = locate(a, i, a.ldx[job]);
+            load_group<T, ACCESS, LPG, R>(x + to_come[u].x, to_come[u].n, x, x + (a.rows - 1) * a.ldx[job] + a.cols, ahead[u]);
+        }
+    };
+    // Where registers allow, a block takes several tiles and has the next one's loads under way: 100000 x 500 in groups of 100
+    // 78 -> 67 us.  (With the shifts of odd rows it lost: 232965 x 602 166 -> 179.)
+    int64_t tile = blockIdx.x / a.jobs;
+    const int64_t tiles = (a.items + NG * U - 1) / (NG * U), apart = gridDim.x / a.jobs;
+    fetch(tile);
+    do {
+        const int64_t first = tile * (NG * U) + threadIdx.x / LPG;
+        float v[U][R * 4];
+        Where w[U];
 #pragma unroll
-        for (int k = 0; k < R * 4; k += 2) top = max_abs3(v[u][k], v[u][k + 1], top);
+        for (int u = 0; u < U; ++u) {
+            w[u] = to_come[u];
 #pragma unroll
-        for (int o = LPG / 2; o > 0; o >>= 1) top = max_or_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const int64_t i = first + u * NG;
-        const bool keep = !ACT || a.q[job];          // an activation without a backward pass keeps nothing
-        if (keep && i < a.items) {
-            const float s = group_scale(top), inv = group_inverse(s);
-            const int width = code_width(a, w[u]);
-            int8_t *q = a.q[job] + (code_place(a, w[u]) << (run > 0));
-            if (lane == 0) a.scale[job][i * a.scale_stride[job]] = s;
-            uint32_t word[R];
-            if (a.mode == TANGO_ROUND_NEAREST) {
-                encode_nearest<R>(v[u], s, inv, word);
-            } else {
+            for (int k = 0; k < R * 4; ++k) v[u][k] = ahead[u][k];
+        }
+        tile += apart;
+        if (kAhead<ACCESS> && tile < tiles) fetch(tile);
 #pragma unroll
-                for (int r = 0; r < R; ++r)
-                    word[r] = encode4_mode(v[u] + 4 * r, s, a.mode, a.seed, effective_call(a.call + job, a.step),
-                                           (uint64_t)w[u].row * a.cols + (int64_t)w[u].g * a.group + (lane + r * LPG) * 4);
+        for (int u = 0; u < U; ++u) {
+            float top = 0.f;
+#pragma unroll
+            for (int k = 0; k < R * 4; k += 2) top = max_abs3(v[u][k], v[u][k + 1], top);
+#pragma unroll
+            for (int o = LPG / 2; o > 0; o >>= 1) top = max_or_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+            const int64_t i = first + u * NG;
+            const bool keep = !ACT || a.q[job];          // an activation without a backward pass keeps nothing
+            if (keep && i < a.items) {
+                const float s = group_scale(top), inv = group_inverse(s);
+                const int width = code_width(a, w[u]);
+                int8_t *q = a.q[job] + (code_place(a, w[u]) << (run > 0));
+                if (lane == 0) a.scale[job][i * a.scale_stride[job]] = s;
+                uint32_t word[R];
+                if (a.mode == TANGO_ROUND_NEAREST) {
+                    encode_nearest<R>(v[u], s, inv, word);
+                } else {
+#pragma unroll
+                    for (int r = 0; r < R; ++r)
+                        word[r] = encode4_mode(v[u] + 4 * r, s, a.mode, a.seed, effective_call(a.call + job, a.step),
+                                               (uint64_t)w[u].row * a.cols + (int64_t)w[u].g * a.group + (lane + r * LPG) * 4);
+                }
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    const int e = (lane + r * LPG) * 4;
+                    if (e < width) *reinterpret_cast<uint32_t *>(q + (run ? ((e & -run) << 1 | (e & (run - 1))) : e)) = word[r];
+                }
             }
+            if constexpr (ACT) {
+                with_act(a.act, [&](auto kind) {
 #pragma unroll
-            for (int r = 0; r < R; ++r) {
-                const int e = (lane + r * LPG) * 4;
-                if (e < width) *reinterpret_cast<uint32_t *>(q + (run ? ((e & -run) << 1 | (e & (run - 1))) : e)) = word[r];
+                    for (int k = 0; k < R * 4; ++k) v[u][k] = activate<kind.value>(v[u][k]);
+                });
+                store_group<T, ACCESS, LPG, R>(static_cast<T *>(a.y) + (w[u].x + w[u].row * (a.ldy - a.ldx[0])), w[u].n, v[u]);
             }
         }
-        if constexpr (ACT) {
-            with_act(a.act, [&](auto kind) {
-#pragma unroll
-                for (int k = 0; k < R * 4; ++k) v[u][k] = activate<kind.value>(v[u][k]);
-            });
-            store_group<T, ACCESS, LPG, R>(static_cast<T *>(a.y) + (w[u].x + w[u].row * (a.ldy - a.ldx[0])), w[u].n, v[u]);
-        }
-    }
+    } while (kAhead<ACCESS> && tile < tiles);
 }
 
 template <class T, int ACCESS, int LPG, int R, bool ACT>
@@ -419,7 +519,9 @@ __global__ void __launch_bounds__(kBlock) rows8_flat_kernel(const __grid_constan
 
 template <class T, int ACCESS, bool ACT, bool PACK, int LPG, int R>
 static int launch_kernel(const Rows8Args &a, int jobs, cudaStream_t st) {
-    const int64_t blocks = ceil_div(a.items, Tile<LPG, R>::kItems) * jobs;
+    int64_t blocks = ceil_div(a.items, Tile<LPG, R>::kItems);
+    if (PACK && kAhead<ACCESS> && blocks > kNumSMs * kAheadBlocks) blocks = kNumSMs * kAheadBlocks;
+    blocks *= jobs;
     if (blocks > 0x7fffffffLL) return TANGO_ESIZE;
     const unsigned grid = (unsigned)blocks;
     if constexpr (PACK) rows8_pack_kernel<T, ACCESS, LPG, R, ACT><<<grid, kBlock, 0, st>>>(a);
@@ -468,8 +570,7 @@ static int launch(Rows8Args a, int jobs, int type, int access, cudaStream_t st) 
         typedef decltype(t) T;
         if (access == FLAT) return launch_flat<T, ACT, PACK>(a, jobs, st);
         if (access == WIDE) return launch_tile<T, WIDE, ACT, PACK>(a, jobs, st);
-        if (access == PAIRS) return launch_tile<T, PAIRS, ACT, PACK>(a, jobs, st);
-        return launch_tile<T, sizeof(T) == 2 ? SHIFTED : SINGLE, ACT, PACK>(a, jobs, st);
+        return launch_tile<T, SHIFTED, ACT, PACK>(a, jobs, st);
     };
     if (type == TANGO_FP32) return go(float{});
     if (type == TANGO_BF16) return go(Bf16{});
@@ -494,14 +595,13 @@ static int fill(Rows8Args &a, int64_t rows, int64_t cols, int64_t group, int typ
     return TANGO_OK;
 }
 
-// What the matrices (with their leading dimensions) and the codes of a launch allow.
-static int access_of(const Rows8Args &a, int type, std::initializer_list<const void *> matrices, std::initializer_list<int64_t> lds,
-                     std::initializer_list<const void *> codes, bool interleaved) {
-    bool wide = a.groups == 1 || a.group % 4 == 0, pairs = a.groups == 1 || a.group % 2 == 0, run = true;
-    for (const void *p : matrices) { wide &= aligned(p, 4 * element_bytes(type)); pairs &= aligned(p, 2 * element_bytes(type)); }
-    for (int64_t ld : lds) { wide &= a.rows == 1 || ld % 4 == 0; pairs &= a.rows == 1 || ld % 2 == 0; run &= a.rows == 1 || ld == a.cols; }
+// What the matrices of a launch, with their leading dimensions, allow.
+static int access_of(const Rows8Args &a, int type, std::initializer_list<const void *> matrices, std::initializer_list<int64_t> lds) {
+    bool wide = a.groups == 1 || a.group % 4 == 0, run = true;
+    for (const void *p : matrices) wide &= aligned(p, 4 * element_bytes(type));
+    for (int64_t ld : lds) { wide &= a.rows == 1 || ld % 4 == 0; run &= a.rows == 1 || ld == a.cols; }
     if (wide && run && a.cols % a.group == 0 && a.group <= 128 && a.group >= 4 && (a.group & (a.group - 1)) == 0) return FLAT;
-    return wide ? WIDE : pairs ? PAIRS : SINGLE;
+    return wide ? WIDE : SHIFTED;
 }
 static bool fits_32(int64_t v) { return v < 0x7fffffffLL; }
 
@@ -535,7 +635,7 @@ extern "C" int tango_rows8_pack(const tango_rows8_job *jobs, int n_jobs, int64_t
         a.scale_stride[k] = j.scale_stride;
         a.run[k] = j.interleaved ? (int)tango_rows8_run(group) : 0;
         a.wide |= !fits_32(j.ldx);
-        const int way = access_of(a, type, {j.x}, {j.ldx}, {j.q}, j.interleaved);
+        const int way = access_of(a, type, {j.x}, {j.ldx});
         if (way < access) access = way;
     }
     a.mode = mode; a.act = ACT_NONE; a.seed = seed; a.call = call;
@@ -552,7 +652,7 @@ extern "C" int tango_rows8_unpack(const int8_t *q, const float *scales, int64_t 
     if (!aligned(out, element_bytes(type)) || !aligned(q, 4)) return TANGO_EALIGN;
     a.q[0] = const_cast<int8_t *>(q); a.scale[0] = const_cast<float *>(scales); a.y = out; a.ldy = ldo; a.act = ACT_NONE;
     a.wide |= !fits_32(ldo);
-    return launch<false, false>(a, 1, type, access_of(a, type, {out}, {ldo}, {q}, false), static_cast<cudaStream_t>(stream));
+    return launch<false, false>(a, 1, type, access_of(a, type, {out}, {ldo}), static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int tango_act8_forward(int act, const tango_rows8_job *job, int64_t rows, int64_t cols, int64_t group, int type, void *y,
@@ -567,7 +667,7 @@ extern "C" int tango_act8_forward(int act, const tango_rows8_job *job, int64_t r
     a.wide |= !fits_32(job->ldx) || !fits_32(ldy);
     a.mode = mode; a.act = act; a.seed = seed; a.call = call;
     a.step = reinterpret_cast<const unsigned long long *>(step);
-    return launch<true, true>(a, 1, type, access_of(a, type, {job->x, y}, {job->ldx, ldy}, {job->q}, false), static_cast<cudaStream_t>(stream));
+    return launch<true, true>(a, 1, type, access_of(a, type, {job->x, y}, {job->ldx, ldy}), static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int tango_act8_backward(int act, const int8_t *q, const float *scales, int64_t rows, int64_t cols, int64_t group, int type,
@@ -581,5 +681,5 @@ extern "C" int tango_act8_backward(int act, const int8_t *q, const float *scales
     a.q[0] = const_cast<int8_t *>(q); a.scale[0] = const_cast<float *>(scales);
     a.x[0] = dy; a.ldx[0] = lddy; a.y = dx; a.ldy = lddx; a.act = act;
     a.wide |= !fits_32(lddy) || !fits_32(lddx);
-    return launch<true, false>(a, 1, type, access_of(a, type, {dy, dx}, {lddy, lddx}, {q}, false), static_cast<cudaStream_t>(stream));
+    return launch<true, false>(a, 1, type, access_of(a, type, {dy, dx}, {lddy, lddx}), static_cast<cudaStream_t>(stream));
 }
