@@ -9,8 +9,8 @@
 // contiguous over the lanes), so that x is read once and stays in registers.  Measured, GB/s of those bytes:
 //   contiguous groups of 4, 8, .. 128 columns: GELU of 232965 x 256 forward 100 us (5.4 TB/s), backward 79 (6.8, dy partly in L2);
 //     three matrices of 23 M elements, one launch, 94 us (3.7): 25 instructions an element keep the issue slots three quarters busy
-//   602 columns, fp32 in pairs: pack 217 us (3.2), unpack 163 (4.3): 8-byte accesses, half a sector each
-//   601 columns, bf16, SiLU: forward 262 us (1.9), backward 187 (2.7): the shifts into place are a third of 60 instructions an element
+//   602 columns, fp32, shifted into place: pack 171 us (4.1), unpack 125 (5.6); pairs of elements, half a sector each, took 217, 163
+//   601 columns, bf16, SiLU: forward 231 us (2.2), backward 188 (2.7): the shifts into place are a third of 60 instructions an element
 // An earlier form with four elements a lane and 32 lanes a group took 408, 215 and 406 us where the first of each pair stands.
 #include "rows8.cuh"
 
@@ -33,6 +33,7 @@ struct Rows8Args {
     int64_t ldy;
     int64_t rows, cols, items;    // items = rows * groups
     int32_t group, groups, pitch; // bytes between the codes of two groups
+    int32_t tile;                 // codes that the lanes of a group have to cover
     int64_t ldq;
     FastDiv by_groups;
     int wide;                     // 2^31 groups or more
@@ -138,7 +139,7 @@ enum { SHIFTED = 0, WIDE = 4, FLAT = 8 };
 
 // ---- a lane's elements of a group: four neighbours at lane * 4, (lane + LPG) * 4, ..
 // In rows of any pitch they come in the aligned pieces of four (16 or 8 bytes) that hold them: a lane's four straddle its own piece
-// and the next lane's, and go out likewise.  Single accesses took 373 us where these take 260 (169343 x 601 bf16, SiLU, forward).
+// and the next lane's, and go out likewise.  Single accesses took 373 us where these take 231 (169343 x 601 bf16, SiLU, forward).
 template <int LPG>
 __device__ __forceinline__ uint64_t from_lane(uint64_t v, int lane) { return __shfl_sync(0xffffffffu, v, ((threadIdx.x & 31) & ~(LPG - 1)) + lane); }
 
@@ -552,14 +553,14 @@ static int launch_flat(const Rows8Args &a, int jobs, cudaStream_t st) {
 
 template <class T, int ACCESS, bool ACT, bool PACK>
 static int launch_tile(const Rows8Args &a, int jobs, cudaStream_t st) {
-    if (a.group <= 4) return launch_kernel<T, ACCESS, ACT, PACK, 1, 1>(a, jobs, st);
-    if (a.group <= 8) return launch_kernel<T, ACCESS, ACT, PACK, 1, 2>(a, jobs, st);
-    if (a.group <= 16) return launch_kernel<T, ACCESS, ACT, PACK, 1, 4>(a, jobs, st);
-    if (a.group <= 32) return launch_kernel<T, ACCESS, ACT, PACK, 2, 4>(a, jobs, st);
-    if (a.group <= 64) return launch_kernel<T, ACCESS, ACT, PACK, 4, 4>(a, jobs, st);
-    if (a.group <= 128) return launch_kernel<T, ACCESS, ACT, PACK, 8, 4>(a, jobs, st);
-    if (a.group <= 256) return launch_kernel<T, ACCESS, ACT, PACK, 16, 4>(a, jobs, st);
-    if (a.group <= 512) return launch_kernel<T, ACCESS, ACT, PACK, 32, 4>(a, jobs, st);
+    if (a.tile <= 4) return launch_kernel<T, ACCESS, ACT, PACK, 1, 1>(a, jobs, st);
+    if (a.tile <= 8) return launch_kernel<T, ACCESS, ACT, PACK, 1, 2>(a, jobs, st);
+    if (a.tile <= 16) return launch_kernel<T, ACCESS, ACT, PACK, 1, 4>(a, jobs, st);
+    if (a.tile <= 32) return launch_kernel<T, ACCESS, ACT, PACK, 2, 4>(a, jobs, st);
+    if (a.tile <= 64) return launch_kernel<T, ACCESS, ACT, PACK, 4, 4>(a, jobs, st);
+    if (a.tile <= 128) return launch_kernel<T, ACCESS, ACT, PACK, 8, 4>(a, jobs, st);
+    if (a.tile <= 256) return launch_kernel<T, ACCESS, ACT, PACK, 16, 4>(a, jobs, st);
+    if (a.tile <= 512) return launch_kernel<T, ACCESS, ACT, PACK, 32, 4>(a, jobs, st);
     return launch_kernel<T, ACCESS, ACT, PACK, 32, 8>(a, jobs, st);
 }
 
@@ -590,6 +591,10 @@ static int fill(Rows8Args &a, int64_t rows, int64_t cols, int64_t group, int typ
     a.items = rows * groups;
     a.pitch = (int32_t)tango_rows8_pitch(group);
     a.ldq = tango_rows8_ld(cols, group);
+    // a row of one group is shared out by its own length: 19717 x 64 in groups of up to 128, packed with
+    // ELU, 9.5 -> 7.0 us
+    a.tile = (int32_t)(groups == 1 && a.ldq < group ? a.ldq : group);
+    if (groups == 1 && a.ldq == cols) a.group = (int32_t)cols;
     a.wide = !fits_32(a.items) || !fits_32(cols);
     a.by_groups = fast_div(groups);
     return TANGO_OK;
@@ -597,7 +602,7 @@ static int fill(Rows8Args &a, int64_t rows, int64_t cols, int64_t group, int typ
 
 // What the matrices of a launch, with their leading dimensions, allow.
 static int access_of(const Rows8Args &a, int type, std::initializer_list<const void *> matrices, std::initializer_list<int64_t> lds) {
-    bool wide = a.groups == 1 || a.group % 4 == 0, run = true;
+    bool wide = a.groups == 1 || a.group % 4 == 0, run = a.ldq == a.cols;
     for (const void *p : matrices) wide &= aligned(p, 4 * element_bytes(type));
     for (int64_t ld : lds) { wide &= a.rows == 1 || ld % 4 == 0; run &= a.rows == 1 || ld == a.cols; }
     if (wide && run && a.cols % a.group == 0 && a.group <= 128 && a.group >= 4 && (a.group & (a.group - 1)) == 0) return FLAT;

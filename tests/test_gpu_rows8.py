@@ -48,7 +48,8 @@ def codes_of(p, rows, cols):
 
 
 SHAPES = [(1, 1, 1), (1, 7, 4), (3, 5, 8), (2, 16, 16), (33, 31, 8), (257, 100, 128), (129, 602, 128), (65, 601, 64), (40, 300, 100),
-          (19, 257, 256), (7, 3000, 1024), (5, 1500, 700), (70000, 8, 8), (1, 40000, 32), (1000, 41, 41), (9, 130, 33)]
+          (19, 257, 256), (7, 3000, 1024), (5, 1500, 700), (70000, 8, 8), (1, 40000, 32), (1000, 41, 41), (9, 130, 33), (300, 64, 128), (77, 16, 1024),
+          (50, 4, 128), (31, 9, 64), (40, 48, 1000), (64, 128, 128), (10, 512, 64), (999, 8, 4)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
