@@ -142,6 +142,30 @@ __device__ __forceinline__ void from_float(float v, float &o) { o = v; }
 __device__ __forceinline__ void from_float(float v, Bf16 &o) { asm("cvt.rn.bf16.f32 %0, %1;" : "=h"(o.bits) : "f"(v)); }
 __device__ __forceinline__ void from_float(float v, Fp16 &o) { asm("cvt.rn.f16.f32 %0, %1;" : "=h"(o.bits) : "f"(v)); }
 
+// Two neighbouring elements in a word.
+template <class T> __device__ __forceinline__ void unpack2(uint32_t w, float &lo, float &hi) {
+    T a, b;
+    a.bits = (uint16_t)w;
+    b.bits = (uint16_t)(w >> 16);
+    lo = to_float(a);
+    hi = to_float(b);
+}
+template <> __device__ __forceinline__ void unpack2<Bf16>(uint32_t w, float &lo, float &hi) {
+    lo = __uint_as_float(w << 16);
+    hi = __uint_as_float(w & 0xffff0000u);
+}
+template <class T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pack2<Bf16>(float lo, float hi) {
+    uint32_t w;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(hi), "f"(lo));
+    return w;
+}
+template <> __device__ __forceinline__ uint32_t pack2<Fp16>(float lo, float hi) {
+    uint32_t w;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(hi), "f"(lo));
+    return w;
+}
+
 // VL elements at once, p aligned to them.
 template <int BYTES> struct Word;
 template <> struct Word<2> { typedef uint16_t T; };
