@@ -640,7 +640,7 @@ __device__ __forceinline__ Codes<VB> encode_query(const RowsArgs &a, int64_t r, 
     } else {
 #pragma unroll
         for (int i = 0; i < VB / 4; ++i)
-            c.w[i] = encode4_mode(v + 4 * i, s, a.mode, a.seed, effective_call(a.call, a.step),
+            c.w[i] = encode4_mode(four(v + 4 * i), s, a.mode, a.seed, effective_call(a.call, a.step),
                                   (uint64_t)r * a.heads * a.d + head * a.d + chunk * VB + 4 * i);
     }
     return c;

@@ -39,6 +39,7 @@ struct Rows8Args {
     int wide;                     // 2^31 groups or more
     int jobs;                     // matrices: blocks take them in turn, so that the runs of interleaved ones meet in L2
     int mode, act;
+    int over;                     // input and output lie differently on the boundaries of four elements
     uint64_t seed, call;
     const unsigned long long *step;
 };
@@ -133,14 +134,38 @@ template <int LPG, int R> struct Tile {
     static constexpr int kElements = kItems * LPG * R * 4;
 };
 
-// How the elements are reached: in aligned pieces of four that are shifted into place (rows of any pitch), four at a time, or in one
-// run.
-enum { SHIFTED = 0, WIDE = 4, FLAT = 8 };
+// How the elements are reached: in the aligned pieces of four that hold them (rows of any pitch), four at a time, or in one run.
+enum { TURNED = 0, WIDE = 4, FLAT = 8 };
 
-// ---- a lane's elements of a group: four neighbours at lane * 4, (lane + LPG) * 4, ..
-// In rows of any pitch they come in the aligned pieces of four (16 or 8 bytes) that hold them: a lane's four straddle its own piece
-// and the next lane's, and go out likewise.  Single accesses took 373 us where these take 231 (169343 x 601 bf16, SiLU, forward).
-//
+// ---- a lane's elements of a group: slots of four neighbours at lane * 4, (lane + LPG) * 4, ..
+// In rows of any pitch a group starts `skip` elements behind a boundary of 16 (8) bytes, and slot k takes the aligned piece k: the
+// elements 4 k - skip + i.  The `skip` places that this leaves free in slot 0 take the last elements of a full group, which lie in
+// a piece of their own, so that the group is turned by `skip` within its slots and fills as many as before.  Loads, the maximum,
+// the activation and stores do not mind; only the codes are turned back, in one exchange of words.  169343 x 601 bf16, SiLU,
+// forward: TIME us; with the elements shifted into place 216, with single accesses 373.
+template <int LPG, int R> constexpr int kSlots = LPG * R * 4;
+template <class T, int ACCESS> __device__ __forceinline__ int skip_of(const T *p) {
+    return ACCESS == TURNED ? (int)(reinterpret_cast<uintptr_t>(p) / sizeof(T) & 3) : 0;
+}
+// Element in place i of slot k.
+template <int LPG, int R> __device__ __forceinline__ int element(int k, int i, int skip) {
+    const int e = k * 4 - skip + i;
+    return e < 0 ? e + kSlots<LPG, R> : e;
+}
+__device__ __forceinline__ void load_piece(const float *p, float *v) {
+    const float4 t = __ldg(reinterpret_cast<const float4 *>(p));
+    v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
+}
+template <class T> __device__ __forceinline__ void load_piece(const T *p, float *v) {
+    const uint2 t = __ldg(reinterpret_cast<const uint2 *>(p));
+    unpack2<T>(t.x, v[0], v[1]);
+    unpack2<T>(t.y, v[2], v[3]);
+}
+__device__ __forceinline__ void store_piece(float *p, const float *v) { *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]); }
+template <class T> __device__ __forceinline__ void store_piece(T *p, const float *v) {
+    *reinterpret_cast<uint2 *>(p) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
+}
+
 // n elements at p; [begin, end): the matrix, outside of which nothing is read.
 template <class T, int ACCESS, int LPG, int R>
 __device__ __forceinline__ void load_group(const T *p, int n, const T *begin, const T *end, float (&v)[R * 4]) {
@@ -148,92 +173,38 @@ __device__ __forceinline__ void load_group(const T *p, int n, const T *begin, co
     if constexpr (ACCESS == WIDE) {
 #pragma unroll
         for (int r = 0; r < R; ++r) load4<T, WIDE>(p + (lane + r * LPG) * 4, n - (lane + r * LPG) * 4, v + 4 * r);
-    } else if constexpr (sizeof(T) == 4) {
-        const int skip = (int)(reinterpret_cast<uintptr_t>(p) >> 2 & 3), pieces = n > 0 ? (n + skip + 3) / 4 : 0;
-        const float *first = reinterpret_cast<const float *>(p) - skip;
-        const bool inside = first >= reinterpret_cast<const float *>(begin) && first + pieces * 4 <= reinterpret_cast<const float *>(end);
-        const int from = ((threadIdx.x & 31) & ~(LPG - 1)) + ((lane + 1) & (LPG - 1));
-        float w[R + 1][4];
-#pragma unroll
-        for (int r = 0; r <= R; ++r)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) w[r][i] = 0.f;
-        if (inside) {
-#pragma unroll
-            for (int r = 0; r <= R; ++r) {
-                const int k = lane + r * LPG;
-                if (k < pieces && (r < R || lane == 0)) {
-                    const float4 t = __ldg(reinterpret_cast<const float4 *>(first) + k);
-                    w[r][0] = t.x; w[r][1] = t.y; w[r][2] = t.z; w[r][3] = t.w;
-                }
-            }
-        } else {                        // the matrix begins or ends inside a piece
-#pragma unroll
-            for (int r = 0; r <= R; ++r)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int e = (lane + r * LPG) * 4 - skip + i;
-                    if (e >= 0 && e < n && (r < R || lane == 0)) w[r][i] = to_float(p[e]);
-                }
-        }
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            float all[7];          // this lane's piece, and the first three elements of the next lane's
-#pragma unroll
-            for (int i = 0; i < 4; ++i) all[i] = w[r][i];
-#pragma unroll
-            for (int i = 0; i < 3; ++i) all[4 + i] = __shfl_sync(0xffffffffu, lane == 0 ? w[r + 1][i] : w[r][i], from);
-            const int left = n - (lane + r * LPG) * 4;
-            float half[6];
-#pragma unroll
-            for (int i = 0; i < 6; ++i) half[i] = skip & 1 ? all[i + 1] : all[i];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[4 * r + i] = skip & 2 ? half[i + 2] : half[i];
-            if (left < 4) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (i >= left) v[4 * r + i] = 0.f;
-            }
-        }
     } else {
-        // by words of two elements, then by one: 32-bit selections throughout
-        const int off = (int)(reinterpret_cast<uintptr_t>(p) & 7), pieces = n > 0 ? (n * 2 + off + 7) / 8 : 0;
-        const char *first = reinterpret_cast<const char *>(p) - off;
-        const bool inside = first >= reinterpret_cast<const char *>(begin) && first + pieces * 8 <= reinterpret_cast<const char *>(end);
-        const uint32_t halves = off & 2 ? 0x5432u : 0x3210u;
-        const int from = ((threadIdx.x & 31) & ~(LPG - 1)) + ((lane + 1) & (LPG - 1));
-        uint2 w[R + 1];
+        const int skip = skip_of<T, ACCESS>(p), pieces = n > 0 ? (n + skip + 3) / 4 : 0;
+        const T *first = p - skip;
 #pragma unroll
-        for (int r = 0; r <= R; ++r) w[r] = make_uint2(0u, 0u);
-        if (inside) {
+        for (int k = 0; k < R * 4; ++k) v[k] = 0.f;
+        if (first >= begin && first + pieces * 4 <= end) {
+            float last[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int r = 0; r <= R; ++r) {
+            for (int r = 0; r < R; ++r)
+                if (lane + r * LPG < pieces) load_piece(first + (lane + r * LPG) * 4, v + 4 * r);
+            if (lane == 0 && LPG * R < pieces) load_piece(first + kSlots<LPG, R>, last);
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
                 const int k = lane + r * LPG;
-                if (k < pieces && (r < R || lane == 0)) w[r] = __ldg(reinterpret_cast<const uint2 *>(first) + k);
+                if (r == 0 && lane == 0) {
+#pragma unroll
+                    for (int i = 0; i < 3; ++i) v[i] = i < skip ? last[i] : v[i];
+                }
+                if ((r == 0 && lane == 0) || k * 4 - skip + 4 > n) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (element<LPG, R>(k, i, skip) >= n) v[4 * r + i] = 0.f;
+                }
             }
         } else {                        // the matrix begins or ends inside a piece
 #pragma unroll
-            for (int r = 0; r <= R; ++r)
+            for (int r = 0; r < R; ++r)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int e = (lane + r * LPG) * 4 - off / 2 + i;
-                    if (e >= 0 && e < n && (r < R || lane == 0))
-                        (i < 2 ? w[r].x : w[r].y) |= (uint32_t)__ldg(reinterpret_cast<const unsigned short *>(p) + e) << (16 * (i & 1));
+                    const int e = element<LPG, R>(lane + r * LPG, i, skip);
+                    if (e < n) v[4 * r + i] = to_float(p[e]);
                 }
-        }
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const uint32_t n0 = __shfl_sync(0xffffffffu, lane == 0 ? w[r + 1].x : w[r].x, from);
-            const uint32_t n1 = __shfl_sync(0xffffffffu, lane == 0 ? w[r + 1].y : w[r].y, from);
-            const uint32_t a0 = off & 4 ? w[r].y : w[r].x, a1 = off & 4 ? n0 : w[r].y, a2 = off & 4 ? n1 : n0;
-            uint32_t lo = __byte_perm(a0, a1, halves), hi = __byte_perm(a1, a2, halves);
-            const int left = n - (lane + r * LPG) * 4;
-            if (left < 4) {
-                hi = left == 3 ? hi & 0xffffu : 0u;
-                lo = left >= 2 ? lo : left == 1 ? lo & 0xffffu : 0u;
-            }
-            unpack2<T>(lo, v[4 * r], v[4 * r + 1]);
-            unpack2<T>(hi, v[4 * r + 2], v[4 * r + 3]);
         }
     }
 }
@@ -243,75 +214,69 @@ __device__ __forceinline__ void store_group(T *p, int n, const float (&v)[R * 4]
     if constexpr (ACCESS == WIDE) {
 #pragma unroll
         for (int r = 0; r < R; ++r) store4<T, WIDE>(p + (lane + r * LPG) * 4, n - (lane + r * LPG) * 4, v + 4 * r);
-    } else if constexpr (sizeof(T) == 4) {
-        // the same for four-byte elements, by whole elements: with accesses of 4 bytes unpacking 232965 x 601 took 355 us, 139 so
-        const int skip = (int)(reinterpret_cast<uintptr_t>(p) >> 2 & 3), from = ((threadIdx.x & 31) & ~(LPG - 1)) + ((lane + LPG - 1) & (LPG - 1));
-        float *first = reinterpret_cast<float *>(p) - skip;
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            float all[7];          // the last three elements of the lane before, and this one's
-#pragma unroll
-            for (int i = 1; i < 4; ++i) {
-                const float mine = lane == LPG - 1 ? (r > 0 ? v[r > 0 ? 4 * r - 4 + i : 0] : 0.f) : v[4 * r + i];
-                all[i - 1] = __shfl_sync(0xffffffffu, mine, from);
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) all[3 + i] = v[4 * r + i];
-            float half[6], piece[4];
-#pragma unroll
-            for (int i = 0; i < 6; ++i) half[i] = skip & 1 ? all[i] : all[i + 1];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) piece[i] = skip & 2 ? half[i] : half[i + 2];
-            const int k = lane + r * LPG, e = k * 4 - skip;
-            if (e >= 0 && e + 4 <= n) {
-                reinterpret_cast<float4 *>(first)[k] = make_float4(piece[0], piece[1], piece[2], piece[3]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (e + i >= 0 && e + i < n) from_float(piece[i], p[e + i]);
-            }
-        }
-        if (lane == LPG - 1) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int e = (R * LPG - 1) * 4 + i;
-                if (i >= 4 - skip && e < n) from_float(v[4 * R - 4 + i], p[e]);
-            }
-        }
     } else {
-        const int off = (int)(reinterpret_cast<uintptr_t>(p) & 7), skip = off / 2;
-        const uint32_t halves = off & 2 ? 0x5432u : 0x7654u;
-        const int from = ((threadIdx.x & 31) & ~(LPG - 1)) + ((lane + LPG - 1) & (LPG - 1));
-        uint2 *first = reinterpret_cast<uint2 *>(reinterpret_cast<char *>(p) - off);
-        uint2 w[R];
-#pragma unroll
-        for (int r = 0; r < R; ++r) w[r] = make_uint2(pack2<T>(v[4 * r], v[4 * r + 1]), pack2<T>(v[4 * r + 2], v[4 * r + 3]));
+        const int skip = skip_of<T, ACCESS>(p);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            const uint2 out = lane == LPG - 1 ? (r > 0 ? w[r > 0 ? r - 1 : 0] : make_uint2(0u, 0u)) : w[r];
-            const uint32_t b0 = __shfl_sync(0xffffffffu, out.x, from), b1 = __shfl_sync(0xffffffffu, out.y, from);
-            const uint32_t c0 = off & 4 ? b0 : b1, c1 = off & 4 ? b1 : w[r].x, c2 = off & 4 ? w[r].x : w[r].y;
-            const uint2 piece = make_uint2(__byte_perm(c0, c1, halves), __byte_perm(c1, c2, halves));
-            const int k = lane + r * LPG, e = k * 4 - skip;          // the piece's first element
+            const int e = (lane + r * LPG) * 4 - skip;
             if (e >= 0 && e + 4 <= n) {
-                first[k] = piece;
-            } else {
+                store_piece(p + e, v + 4 * r);
+            } else if (e < n) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (e + i >= 0 && e + i < n) p[e + i].bits = (uint16_t)((i < 2 ? piece.x : piece.y) >> (16 * (i & 1)));
-            }
-        }
-        if (lane == LPG - 1) {                                        // what the shift pushed out behind the last piece
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int e = (R * LPG - 1) * 4 + i;
-                if (i >= 4 - skip && e < n) p[e].bits = (uint16_t)((i < 2 ? w[R - 1].x : w[R - 1].y) >> (16 * (i & 1)));
+                for (int i = 0; i < 4; ++i) {
+                    const int at = element<LPG, R>(lane + r * LPG, i, skip);
+                    if (at < n) from_float(v[4 * r + i], p[at]);
+                }
             }
         }
     }
 }
+// The lane (of a group's LPG) before or after this one, as a lane of the warp.
+template <int LPG> __device__ __forceinline__ int neighbour(int by) {
+    return ((threadIdx.x & 31) & ~(LPG - 1)) + ((threadIdx.x + by) & (LPG - 1));
+}
+// Codes of the slots, turned, to the words of the codes in order, and back.
+template <int LPG, int R> __device__ __forceinline__ void turn_back(uint32_t (&word)[R], int skip) {
+    const bool wraps = threadIdx.x % LPG == 0;
+    uint32_t next[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) next[r] = __shfl_sync(0xffffffffu, wraps ? word[(r + 1) % R] : word[r], neighbour<LPG>(1));
+#pragma unroll
+    for (int r = 0; r < R; ++r) word[r] = __byte_perm(word[r], next[r], 0x3210 + 0x1111 * skip);
+}
+template <int LPG, int R> __device__ __forceinline__ void turn(uint32_t (&word)[R], int skip) {
+    const bool wraps = threadIdx.x % LPG == LPG - 1;
+    uint32_t before[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) before[r] = __shfl_sync(0xffffffffu, wraps ? word[(r + R - 1) % R] : word[r], neighbour<LPG>(LPG - 1));
+#pragma unroll
+    for (int r = 0; r < R; ++r) word[r] = __byte_perm(before[r], word[r], 0x7654 - 0x1111 * skip);
+}
+// Elements turned by `from` to elements turned by `to`, for an output that lies otherwise on its boundaries than the input.
+template <int LPG, int R> __device__ __forceinline__ void turn_over(float (&v)[R * 4], int from, int to) {
+    const bool first = threadIdx.x % LPG == 0, last = threadIdx.x % LPG == LPG - 1;
+    float w[R * 4];
+#pragma unroll
+    for (int k = 0; k < R * 4; ++k) {               // back by a slot, so that what is left is a turn forward
+        const float before = __shfl_sync(0xffffffffu, last ? v[(k + 4 * R - 4) % (4 * R)] : v[k], neighbour<LPG>(LPG - 1));
+        w[k] = from < to ? before : v[k];
+    }
+    const int by = from - to & 3;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        float all[7], half[6];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) all[i] = w[4 * r + i];
+#pragma unroll
+        for (int i = 0; i < 3; ++i) all[4 + i] = __shfl_sync(0xffffffffu, first ? w[(4 * r + 4) % (4 * R) + i] : w[4 * r + i], neighbour<LPG>(1));
+#pragma unroll
+        for (int i = 0; i < 6; ++i) half[i] = by & 1 ? all[i + 1 < 7 ? i + 1 : 6] : all[i];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[4 * r + i] = by & 2 ? half[i + 2] : half[i];
+    }
+}
 
-template <int ACCESS> constexpr bool kAhead = ACCESS != SHIFTED;
+template <int ACCESS> constexpr bool kAhead = ACCESS != TURNED;
 constexpr int kAheadBlocks = 16;        // blocks an SM of the kernels that take several tiles
 
 template <class T, int ACCESS, int LPG, int R, bool ACT>
@@ -357,24 +322,27 @@ __global__ void __launch_bounds__(kBlock) rows8_pack_kernel(const __grid_constan
             for (int o = LPG / 2; o > 0; o >>= 1) top = max_or_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
             const int64_t i = first + u * NG;
             const bool keep = !ACT || a.q[job];          // an activation without a backward pass keeps nothing
-            if (keep && i < a.items) {
+            const int skip = skip_of<T, ACCESS>(x + w[u].x);
+            if (keep) {
                 const float s = group_scale(top), inv = group_inverse(s);
                 const int width = code_width(a, w[u]);
                 int8_t *q = a.q[job] + (code_place(a, w[u]) << (run > 0));
-                if (lane == 0) a.scale[job][i * a.scale_stride[job]] = s;
+                if (lane == 0 && i < a.items) a.scale[job][i * a.scale_stride[job]] = s;
                 uint32_t word[R];
                 if (a.mode == TANGO_ROUND_NEAREST) {
                     encode_nearest<R>(v[u], s, inv, word);
                 } else {
 #pragma unroll
                     for (int r = 0; r < R; ++r)
-                        word[r] = encode4_mode(v[u] + 4 * r, s, a.mode, a.seed, effective_call(a.call + job, a.step),
-                                               (uint64_t)w[u].row * a.cols + (int64_t)w[u].g * a.group + (lane + r * LPG) * 4);
+                        word[r] = encode4_mode(four(v[u] + 4 * r), s, a.mode, a.seed, effective_call(a.call + job, a.step),
+                                               (uint64_t)w[u].row * a.cols + (int64_t)w[u].g * a.group + (lane + r * LPG) * 4 - skip,
+                                               lane + r == 0 ? skip : 0, kSlots<LPG, R>);
                 }
+                if constexpr (ACCESS == TURNED) turn_back<LPG, R>(word, skip);
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
                     const int e = (lane + r * LPG) * 4;
-                    if (e < width) *reinterpret_cast<uint32_t *>(q + (run ? ((e & -run) << 1 | (e & (run - 1))) : e)) = word[r];
+                    if (e < width && i < a.items) *reinterpret_cast<uint32_t *>(q + (run ? ((e & -run) << 1 | (e & (run - 1))) : e)) = word[r];
                 }
             }
             if constexpr (ACT) {
@@ -382,7 +350,9 @@ __global__ void __launch_bounds__(kBlock) rows8_pack_kernel(const __grid_constan
 #pragma unroll
                     for (int k = 0; k < R * 4; ++k) v[u][k] = activate<kind.value>(v[u][k]);
                 });
-                store_group<T, ACCESS, LPG, R>(static_cast<T *>(a.y) + (w[u].x + w[u].row * (a.ldy - a.ldx[0])), w[u].n, v[u]);
+                T *y = static_cast<T *>(a.y) + (w[u].x + w[u].row * (a.ldy - a.ldx[0]));
+                if (ACCESS == TURNED && a.over) turn_over<LPG, R>(v[u], skip, skip_of<T, ACCESS>(y));
+                store_group<T, ACCESS, LPG, R>(y, w[u].n, v[u]);
             }
         }
     } while (kAhead<ACCESS> && tile < tiles);
@@ -414,8 +384,12 @@ __global__ void __launch_bounds__(kBlock) rows8_unpack_kernel(const __grid_const
         }
     }
     float o[U][R * 4];
+    int skip[U], skip_out[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+    for (int u = 0; u < U; ++u) {
+        skip[u] = skip_out[u] = skip_of<T, ACCESS>(static_cast<T *>(a.y) + w[u].x);
+        if (ACT) skip[u] = skip_of<T, ACCESS>(static_cast<const T *>(a.x[0]) + (w[u].x + w[u].row * (a.ldx[0] - a.ldy)));
+        if constexpr (ACCESS == TURNED) turn<LPG, R>(word[u], skip[u]);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             Pair lo, hi;
@@ -423,6 +397,7 @@ __global__ void __launch_bounds__(kBlock) rows8_unpack_kernel(const __grid_const
             const float2 l = both(mul2(lo, pair(s[u], s[u]))), h = both(mul2(hi, pair(s[u], s[u])));
             o[u][4 * r] = l.x; o[u][4 * r + 1] = l.y; o[u][4 * r + 2] = h.x; o[u][4 * r + 3] = h.y;
         }
+    }
     if constexpr (ACT) {
         with_act(a.act, [&](auto kind) {
 #pragma unroll
@@ -432,7 +407,10 @@ __global__ void __launch_bounds__(kBlock) rows8_unpack_kernel(const __grid_const
         });
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u) store_group<T, ACCESS, LPG, R>(static_cast<T *>(a.y) + w[u].x, w[u].n, o[u]);
+    for (int u = 0; u < U; ++u) {
+        if (ACT && ACCESS == TURNED && a.over) turn_over<LPG, R>(o[u], skip[u], skip_out[u]);
+        store_group<T, ACCESS, LPG, R>(static_cast<T *>(a.y) + w[u].x, w[u].n, o[u]);
+    }
 }
 
 // ---- contiguous matrices whose groups have 4, 8, .. 128 columns and fill their rows: one run of memory in every respect (groups,
@@ -480,7 +458,7 @@ __global__ void __launch_bounds__(kBlock) rows8_flat_kernel(const __grid_constan
             } else {
 #pragma unroll
                 for (int r = 0; r < R; ++r)
-                    word[r] = encode4_mode(v + 4 * r, s[r], a.mode, a.seed, effective_call(a.call + job, a.step), at + r * 128);
+                    word[r] = encode4_mode(four(v + 4 * r), s[r], a.mode, a.seed, effective_call(a.call + job, a.step), at + r * 128);
             }
             const int run = a.run[job];
 #pragma unroll
@@ -574,7 +552,7 @@ static int launch(Rows8Args a, int jobs, int type, int access, cudaStream_t st) 
         typedef decltype(t) T;
         if (access == FLAT) return launch_flat<T, ACT, PACK>(a, jobs, st);
         if (access == WIDE) return launch_tile<T, WIDE, ACT, PACK>(a, jobs, st);
-        return launch_tile<T, SHIFTED, ACT, PACK>(a, jobs, st);
+        return launch_tile<T, TURNED, ACT, PACK>(a, jobs, st);
     };
     if (type == TANGO_FP32) return go(float{});
     if (type == TANGO_BF16) return go(Bf16{});
@@ -609,7 +587,11 @@ static int access_of(const Rows8Args &a, int type, std::initializer_list<const v
     for (const void *p : matrices) wide &= aligned(p, 4 * element_bytes(type));
     for (int64_t ld : lds) { wide &= a.rows == 1 || ld % 4 == 0; run &= a.rows == 1 || ld == a.cols; }
     if (wide && run && a.cols % a.group == 0 && a.group <= 128 && a.group >= 4 && (a.group & (a.group - 1)) == 0) return FLAT;
-    return wide ? WIDE : SHIFTED;
+    return wide ? WIDE : TURNED;
+}
+static int lie_apart(const Rows8Args &a, int type) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a.x[0]), y = reinterpret_cast<uintptr_t>(a.y), e = (uintptr_t)element_bytes(type);
+    return (x / e & 3) != (y / e & 3) || (a.rows > 1 && (a.ldx[0] - a.ldy) % 4 != 0);
 }
 static bool fits_32(int64_t v) { return v < 0x7fffffffLL; }
 
@@ -673,6 +655,7 @@ extern "C" int tango_act8_forward(int act, const tango_rows8_job *job, int64_t r
     if (!aligned(job->x, element_bytes(type)) || !aligned(y, element_bytes(type)) || !aligned(job->q, 4)) return TANGO_EALIGN;
     a.x[0] = job->x; a.ldx[0] = job->ldx; a.q[0] = job->q; a.scale[0] = job->scales; a.scale_stride[0] = job->scale_stride; a.y = y; a.ldy = ldy;
     a.wide |= !fits_32(job->ldx) || !fits_32(ldy);
+    a.over = lie_apart(a, type);
     a.mode = mode; a.act = act; a.seed = seed; a.call = call;
     a.step = reinterpret_cast<const unsigned long long *>(step);
     return launch<true, true>(a, 1, type, access_of(a, type, {job->x, y}, {job->ldx, ldy}), static_cast<cudaStream_t>(stream));
@@ -689,5 +672,6 @@ extern "C" int tango_act8_backward(int act, const int8_t *q, const float *scales
     a.q[0] = const_cast<int8_t *>(q); a.scale[0] = const_cast<float *>(scales);
     a.x[0] = dy; a.ldx[0] = lddy; a.y = dx; a.ldy = lddx; a.act = act;
     a.wide |= !fits_32(lddy) || !fits_32(lddx);
+    a.over = lie_apart(a, type);
     return launch<true, false>(a, 1, type, access_of(a, type, {dy, dx}, {lddy, lddx}), static_cast<cudaStream_t>(stream));
 }

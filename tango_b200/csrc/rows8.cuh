@@ -64,19 +64,30 @@ __device__ __forceinline__ float group_inverse(float s) { return s > 0.f ? __fdi
 template <int N>
 __device__ __forceinline__ void round_nearest(const float *x, float s, float inv, float *b) {
     const Pair by = pair(inv, inv), magic = pair(kRoundMagic, kRoundMagic), minus = pair(-1.f, -1.f);
-    float far = 0.f;
+    float far[N / 4], farthest = 0.f;
 #pragma unroll
-    for (int k = 0; k < N; k += 2) {
-        const Pair v = pair(x[k], x[k + 1]), c = fma2(v, by, magic);
-        const float2 d = both(fma2(v, by, fma2(c, minus, magic))), f = both(c);
-        far = max_abs3(d.x, d.y, far);
-        b[k] = f.x; b[k + 1] = f.y;
+    for (int k = 0; k < N; k += 4) {
+        float d[4];
+#pragma unroll
+        for (int j = 0; j < 4; j += 2) {
+            const Pair v = pair(x[k + j], x[k + j + 1]), c = fma2(v, by, magic);
+            const float2 e = both(fma2(v, by, fma2(c, minus, magic))), f = both(c);
+            d[j] = e.x; d[j + 1] = e.y;
+            b[k + j] = f.x; b[k + j + 1] = f.y;
+        }
+        far[k / 4] = max_abs3(max_abs3(d[0], d[1], d[2]), d[3], 0.f);
+        farthest = k == 0 ? far[0] : max_or_nan(farthest, far[k / 4]);
     }
-    if (far > 0.4999f) {
+    if (farthest > 0.4999f) {
+        const float half = 0.5f * s, below = __int_as_float(__float_as_int(half) - 1);     // of an odd code a half is enough
 #pragma unroll
-        for (int k = 0; k < N; ++k) {
-            const float rest = fmaf(__fsub_rn(kRoundMagic, b[k]), s, x[k]), twice = 2.f * fabsf(rest);
-            if (twice > s || (twice == s && (__float_as_int(b[k]) & 1))) b[k] = __fadd_rn(b[k], rest > 0.f ? 1.f : -1.f);
+        for (int k = 0; k < N; k += 4) {
+            if (N > 4 && !(far[k / 4] > 0.4999f)) continue;
+#pragma unroll
+            for (int j = k; j < k + 4; ++j) {
+                const float rest = fmaf(__fsub_rn(kRoundMagic, b[j]), s, x[j]);
+                if (fabsf(rest) > (__float_as_int(b[j]) & 1 ? below : half)) b[j] = __fadd_rn(b[j], copysignf(1.f, rest));
+            }
         }
     }
 }
@@ -92,16 +103,21 @@ __device__ __forceinline__ void encode_nearest(const float *x, float s, float in
     }
 }
 
-// The other rounding modes: truncation, and the seeded stochastic stream keyed by the elements' flat indices.
-static __device__ __noinline__ uint32_t encode4_mode(const float *x, float s, int mode, uint64_t seed, uint64_t call, uint64_t flat) {
+__device__ __forceinline__ float4 four(const float *x) { return make_float4(x[0], x[1], x[2], x[3]); }
+
+// The other rounding modes: truncation, and the seeded stochastic stream keyed by the elements' flat indices: flat + i, and
+// `behind` more for the first `turned`.
+static __device__ __noinline__ uint32_t encode4_mode(float4 four, float s, int mode, uint64_t seed, uint64_t call, uint64_t flat,
+                                                   int turned = 0, int behind = 0) {
     if (!(s > 0.f)) return 0u;
+    const float x[4] = {four.x, four.y, four.z, four.w};       // by value: an address would keep the caller's values in memory
     const Philox ph{(uint32_t)seed, (uint32_t)(seed >> 32)};
     uint64_t blk = ~0ull;
     uint4 rnd = make_uint4(0, 0, 0, 0);
     uint32_t word = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const float u = mode == TANGO_ROUND_STOCHASTIC ? sr_uniform(ph, flat + i, call, blk, rnd) : 0.f;
+        const float u = mode == TANGO_ROUND_STOCHASTIC ? sr_uniform(ph, flat + i + (i < turned ? behind : 0), call, blk, rnd) : 0.f;
         word |= (uint32_t)(uint8_t)round_to_i8(__fdiv_rn(x[i], s), mode, u) << (8 * i);
     }
     return word;
