@@ -9,8 +9,8 @@
 // contiguous over the lanes), so that x is read once and stays in registers.  Measured, GB/s of those bytes:
 //   contiguous groups of 4, 8, .. 128 columns: GELU of 232965 x 256 forward 100 us (5.4 TB/s), backward 79 (6.8, dy partly in L2);
 //     three matrices of 23 M elements, one launch, 94 us (3.7): 25 instructions an element keep the issue slots three quarters busy
-//   602 columns, fp32, shifted into place: pack 171 us (4.1), unpack 125 (5.6); pairs of elements, half a sector each, took 217, 163
-//   601 columns, bf16, SiLU: forward 231 us (2.2), backward 188 (2.7): the shifts into place are a third of 60 instructions an element
+//   602 columns, fp32: pack 152 us (4.6: 28 instructions an element), unpack 111 (6.3); pairs of elements, half a sector, 217 and 163
+//   601 columns, bf16, SiLU: forward 174 us (2.9), backward 146 (3.5): the arithmetic pipe is 70 % busy, with 40 instructions an element
 // An earlier form with four elements a lane and 32 lanes a group took 408, 215 and 406 us where the first of each pair stands.
 #include "rows8.cuh"
 
@@ -142,7 +142,7 @@ enum { TURNED = 0, WIDE = 4, FLAT = 8 };
 // elements 4 k - skip + i.  The `skip` places that this leaves free in slot 0 take the last elements of a full group, which lie in
 // a piece of their own, so that the group is turned by `skip` within its slots and fills as many as before.  Loads, the maximum,
 // the activation and stores do not mind; only the codes are turned back, in one exchange of words.  169343 x 601 bf16, SiLU,
-// forward: TIME us; with the elements shifted into place 216, with single accesses 373.
+// forward: 174 us; with the elements shifted into place 216, with single accesses 373.
 template <int LPG, int R> constexpr int kSlots = LPG * R * 4;
 template <class T, int ACCESS> __device__ __forceinline__ int skip_of(const T *p) {
     return ACCESS == TURNED ? (int)(reinterpret_cast<uintptr_t>(p) / sizeof(T) & 3) : 0;
@@ -186,15 +186,13 @@ __device__ __forceinline__ void load_group(const T *p, int n, const T *begin, co
             if (lane == 0 && LPG * R < pieces) load_piece(first + kSlots<LPG, R>, last);
 #pragma unroll
             for (int r = 0; r < R; ++r) {
-                const int k = lane + r * LPG;
+                const int left = n + skip - (lane + r * LPG) * 4;
                 if (r == 0 && lane == 0) {
 #pragma unroll
-                    for (int i = 0; i < 3; ++i) v[i] = i < skip ? last[i] : v[i];
-                }
-                if ((r == 0 && lane == 0) || k * 4 - skip + 4 > n) {
+                    for (int i = 0; i < 4; ++i) v[i] = element<LPG, R>(0, i, skip) < n ? (i < skip ? last[i] : v[i]) : 0.f;
+                } else if (left < 4) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (element<LPG, R>(k, i, skip) >= n) v[4 * r + i] = 0.f;
+                    for (int i = 0; i < 4; ++i) v[4 * r + i] = i < left ? v[4 * r + i] : 0.f;
                 }
             }
         } else {                        // the matrix begins or ends inside a piece
@@ -221,12 +219,16 @@ __device__ __forceinline__ void store_group(T *p, int n, const float (&v)[R * 4]
             const int e = (lane + r * LPG) * 4 - skip;
             if (e >= 0 && e + 4 <= n) {
                 store_piece(p + e, v + 4 * r);
-            } else if (e < n) {
+            } else if (r == 0 && e < 0) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int at = element<LPG, R>(lane + r * LPG, i, skip);
-                    if (at < n) from_float(v[4 * r + i], p[at]);
+                    const int at = element<LPG, R>(0, i, skip);
+                    if (at < n) from_float(v[i], p[at]);
                 }
+            } else if (e < n) {
+#pragma unroll
+                for (int i = 0; i < 3; ++i)
+                    if (e + i < n) from_float(v[4 * r + i], p[e + i]);
             }
         }
     }
@@ -279,8 +281,9 @@ template <int LPG, int R> __device__ __forceinline__ void turn_over(float (&v)[R
 template <int ACCESS> constexpr bool kAhead = ACCESS != TURNED;
 constexpr int kAheadBlocks = 16;        // blocks an SM of the kernels that take several tiles
 
+// Five blocks an SM where registers hold that: 232965 x 602 fp32 162 -> 152 us, bf16 SiLU of 169343 x 601 177 -> 174 (six: 153, 219).
 template <class T, int ACCESS, int LPG, int R, bool ACT>
-__global__ void __launch_bounds__(kBlock) rows8_pack_kernel(const __grid_constant__ Rows8Args a) {
+__global__ void __launch_bounds__(kBlock, ACCESS == TURNED && R <= 4 ? 5 : 1) rows8_pack_kernel(const __grid_constant__ Rows8Args a) {
     constexpr int U = Tile<LPG, R>::U, NG = Tile<LPG, R>::kGroups;
     const int job = blockIdx.x % a.jobs, lane = threadIdx.x % LPG;
     const T *x = static_cast<const T *>(a.x[job]);
@@ -297,7 +300,7 @@ __global__ void __launch_bounds__(kBlock) rows8_pack_kernel(const __grid_constan
         }
     };
     // Where registers allow, a block takes several tiles and has the next one's loads under way: 100000 x 500 in groups of 100
-    // 78 -> 67 us.  (With the shifts of odd rows it lost: 232965 x 602 166 -> 179.)
+    // 78 -> 67 us.  (In turned rows it lost: 232965 x 602 166 -> 203.)
     int64_t tile = blockIdx.x / a.jobs;
     const int64_t tiles = (a.items + NG * U - 1) / (NG * U), apart = gridDim.x / a.jobs;
     fetch(tile);

@@ -139,6 +139,42 @@ def test_refusals(cuda):
         T.unpack8(T.Packed8(p.codes.cpu(), p.scales.cpu(), (4, 16), 16, torch.float32))
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,cols,group", [(37, 41, 41), (50, 130, 64), (9, 601, 128), (21, 16, 16), (40, 3, 8), (11, 700, 700), (1, 67, 32),
+                                             (64, 12, 4), (5, 1030, 1024)])
+def test_where_a_row_begins_changes_nothing(cuda, rows, cols, group, dtype):
+    # the same values behind every offset and at every pitch, in every rounding mode: the same bits as of a contiguous matrix
+    import tango_b200 as T
+    from tango_b200 import config, kernels
+    x = torch.randn(rows, cols, device="cuda").to(dtype)
+    dy = torch.randn(rows, cols, device="cuda").to(dtype)
+
+    def all_of(x, dy):
+        got = []
+        for mode in ("reference", "trunc", "stochastic"):
+            config.set_rounding(mode, seed=3)
+            kernels.set_call_counter(0)
+            p = T.pack8(x, group)
+            leaf = x.detach().requires_grad_()
+            y = T.activation8(leaf, "silu", group)
+            g, = torch.autograd.grad(y, leaf, dy)
+            got += [p.codes, p.scales, p.unpack(), y.detach(), g]
+        return got
+    try:
+        want = all_of(x, dy)
+        for before in range(4):
+            for behind in range(4):
+                wide = torch.full((rows, before + cols + behind), float("nan"), device="cuda", dtype=dtype)
+                at = wide[:, before:before + cols]
+                at.copy_(x)
+                other = torch.full((rows, 1 + cols + behind), float("inf"), device="cuda", dtype=dtype)[:, 1:1 + cols]
+                other.copy_(dy)
+                for a, b in zip(all_of(at, other), want):
+                    assert torch.equal(a, b)
+    finally:
+        config.set_rounding("reference")
+
+
 @pytest.mark.parametrize("mode", ["trunc", "stochastic"])
 def test_rounding_modes(cuda, mode):
     import tango_b200 as T
