@@ -59,8 +59,9 @@ __device__ __forceinline__ float group_inverse(float s) { return s > 0.f ? __fdi
 
 // N codes: x / s exactly rounded, ties to even.  x * inv is within 127 * 2^-21 of the quotient, which decides all but the values
 // that close to a border between two codes.  For those x - q * s is exact in one fused operation (a multiple of half an ulp of
-// s, at most about s / 2), and its double is compared with s.  One question for all N (232965 x 602 fp32: 213 us; one for every
-// four values 248).  The codes come as floats whose bits hold them in the low byte.
+// s, at most about s / 2) and is compared with s / 2, exact too.  One question for all N (232965 x 602 fp32: 213 us; one for every
+// four values 248), then, for the few, one for every four: bf16 quotients meet borders often (max / 2 lies on one), 205 -> 183 us
+// with SiLU of 169343 x 601.  The codes come as floats whose bits hold them in the low byte.
 template <int N>
 __device__ __forceinline__ void round_nearest(const float *x, float s, float inv, float *b) {
     const Pair by = pair(inv, inv), magic = pair(kRoundMagic, kRoundMagic), minus = pair(-1.f, -1.f);
