@@ -276,7 +276,10 @@ Tensor edge_attention_fn(const GraphPtr &g, const Tensor &q, const Tensor &k, co
 
 static tango_rows8 view(const Rows8 &r) { return {ptr<int8_t>(r.q), ptr<float>(r.scale)}; }
 
-Tensor edge_attention_rows(const GraphPtr &g, const Tensor &rows_, const Tensor &q, const Rows8 &k, const Rows8 &v, double scale) {
+Tensor edge_attention_rows(const GraphPtr &g, const Tensor &rows_, const Tensor &q, const Rows8 &k_, const Rows8 &v_, double scale) {
+    // the kernel takes bare pointers: nothing but int8 codes and fp32 scales, dense, reaches it
+    for (const Rows8 *t : {&k_, &v_})
+        require(t->q.scalar_type() == at::kChar && t->scale.scalar_type() == at::kFloat, "keys and values of int8 codes and fp32 scales expected");
     require_heads(q);
     require_matrix(q);
     require(!torch::autograd::compute_requires_grad(q), "edge_attention_rows has no gradient: call it under torch.no_grad()");
@@ -284,14 +287,16 @@ Tensor edge_attention_rows(const GraphPtr &g, const Tensor &rows_, const Tensor 
             "one int32 or int64 node id per query expected");
     require(g->csc->indptr.device() == q.device() && rows_.device() == q.device(), "graph, rows and queries must be on the same GPU");
     const int64_t heads = q.size(1), d = q.size(2), r = q.size(0), n = g->n_nodes;
-    for (const Rows8 *t : {&k, &v}) {
+    for (const Rows8 *t : {&k_, &v_}) {
         require(t->q.device() == q.device() && t->scale.device() == q.device(), "keys and values must be on the GPU of the queries");
-        require(t->q.dim() == 2 && t->q.size(0) == n && t->q.size(1) == tango_rows8_ld(heads * d, d) && t->scale.numel() == n * heads,
+        require(t->q.dim() == 2 && t->q.size(0) == n && t->q.size(1) == tango_rows8_ld(heads * d, d) && t->scale.dim() == 2 &&
+                    t->scale.size(0) == n && t->scale.size(1) == heads,
                 "keys and values packed with one row per node and one group per head expected");
     }
     require(std::isfinite((float)scale), "finite scale expected");
     const Raw raw;
     const c10::cuda::CUDAGuard guard(q.device());
+    const Rows8 k{k_.q.contiguous(), k_.scale.contiguous()}, v{v_.q.contiguous(), v_.scale.contiguous()};
     const Tensor out = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
     if (r == 0) return out;
     const Tensor rows = rows_.to(at::kLong).contiguous();

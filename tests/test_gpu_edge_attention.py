@@ -281,6 +281,33 @@ def test_refusals(cuda):
         T.edge_attention_rows(g, ids, q[:2], k8.to("cpu"), v8)
 
 
+@pytest.mark.parametrize("h,d", [(2, 8), (3, 41), (1, 3)])
+def test_keys_and_values_that_are_not_dense(cuda, h, d):
+    """Packed rows of several layers kept in one array, and scales the other way round: the same bits as from dense ones."""
+    import tango_b200 as T
+    g = make_graph("sparse")
+    n = g.num_nodes()
+    q, k, v, _ = case(g, h, d)
+    k8, v8 = T.pack8(k, d), T.pack8(v, d)
+    ids = torch.tensor([1, 2, n - 1, 2], device="cuda")
+    want = T.edge_attention_rows(g, ids, q[ids], k8, v8)
+    codes = torch.stack([v8.codes, k8.codes, k8.codes + 1, v8.codes], 1)          # [N, layers, ld]
+    scales = torch.stack([v8.scales, k8.scales, 2 * k8.scales, v8.scales], 1)
+
+    def layer(i, scales=scales):
+        return T.Packed8(codes[:, i], scales[:, i], (n, h, d), d, torch.float32)
+
+    assert not layer(1).codes.is_contiguous()
+    assert torch.equal(T.edge_attention_rows(g, ids, q[ids], layer(1), layer(3)), want)
+    assert torch.equal(T.edge_attention_rows(g, ids, q[ids], layer(1), v8), want)
+    turned = T.Packed8(k8.codes, k8.scales.t().contiguous().t(), (n, h, d), d, torch.float32)
+    assert torch.equal(T.edge_attention_rows(g, ids, q[ids], turned, v8), want)
+    for s in (k8.scales.t().contiguous(), k8.scales.flatten(), k8.scales[:1]):    # as many numbers, or fewer, in another shape
+        if s.shape != k8.scales.shape:
+            with pytest.raises(AssertionError, match="one group per head"):
+                T.edge_attention_rows(g, ids, q[ids], T.Packed8(k8.codes, s, (n, h, d), d, torch.float32), v8)
+
+
 @pytest.mark.parametrize("h,d,dtype", [(1, 3, torch.float32), (8, 8, torch.float16), (4, 32, torch.float32), (3, 41, torch.bfloat16),
                                        (2, 300, torch.float32), (33, 8, torch.float32)])
 @pytest.mark.parametrize("kind", ["pair", "classes", "hubs"])

@@ -153,6 +153,21 @@ def test_refusals_before_any_launch():
         T.edge_attention_rows(g, torch.tensor([1]), q[:1], good, good)
 
 
+def test_packed_operands_of_another_type_are_refused_before_any_launch():
+    """Bare pointers go to the kernel: scales of a half type would be read as fp32, twice as far as their buffer reaches."""
+    import tango_b200 as T
+    g = _graph()
+    q = torch.randn(3, 2, 8)
+    codes, scales = torch.zeros(20, 16, dtype=torch.int8), torch.ones(20, 2)
+    good = T.Packed8(codes, scales, (20, 2, 8), 8, torch.float32)
+    for c, s in ((codes, scales.bfloat16()), (codes, scales.half()), (codes, scales.double()), (codes.to(torch.uint8), scales),
+                 (codes.float(), scales)):
+        bad = T.Packed8(c, s, (20, 2, 8), 8, torch.float32)
+        for k8, v8 in ((good, bad), (bad, good)):
+            with pytest.raises(AssertionError, match="int8 codes and fp32 scales"):
+                T.edge_attention_rows(g, torch.tensor([1, 2, 3]), q, k8, v8)
+
+
 def test_activations_that_have_an_8_bit_form():
     import torch.nn as nn
     import torch.nn.functional as F
