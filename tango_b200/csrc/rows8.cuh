@@ -59,7 +59,8 @@ __device__ __forceinline__ float group_inverse(float s) { return s > 0.f ? __fdi
 
 // N codes: x / s exactly rounded, ties to even.  x * inv is within 127 * 2^-21 of the quotient, which decides all but the values
 // that close to a border between two codes.  For those x - q * s is exact in one fused operation (a multiple of half an ulp of
-// s, at most about s / 2) and is compared with s / 2, exact too.  One question for all N (232965 x 602 fp32: 213 us; one for every
+// s, at most about s / 2) and is doubled, exact too, to be compared with s (half of s is not exact for the smallest normal scales,
+// where it is a subnormal number).  One question for all N (232965 x 602 fp32: 213 us; one for every
 // four values 248), then, for the few, one for every four: bf16 quotients meet borders often (max / 2 lies on one), 205 -> 183 us
 // with SiLU of 169343 x 601.  The codes come as floats whose bits hold them in the low byte.
 template <int N>
@@ -80,14 +81,14 @@ __device__ __forceinline__ void round_nearest(const float *x, float s, float inv
         farthest = k == 0 ? far[0] : max_or_nan(farthest, far[k / 4]);
     }
     if (farthest > 0.4999f) {
-        const float half = 0.5f * s, below = __int_as_float(__float_as_int(half) - 1);     // of an odd code a half is enough
+        const float below = __int_as_float(__float_as_int(s) - 1);      // of an odd code a half is enough
 #pragma unroll
         for (int k = 0; k < N; k += 4) {
             if (N > 4 && !(far[k / 4] > 0.4999f)) continue;
 #pragma unroll
             for (int j = k; j < k + 4; ++j) {
                 const float rest = fmaf(__fsub_rn(kRoundMagic, b[j]), s, x[j]);
-                if (fabsf(rest) > (__float_as_int(b[j]) & 1 ? below : half)) b[j] = __fadd_rn(b[j], copysignf(1.f, rest));
+                if (fabsf(rest + rest) > (__float_as_int(b[j]) & 1 ? below : s)) b[j] = __fadd_rn(b[j], copysignf(1.f, rest));
             }
         }
     }

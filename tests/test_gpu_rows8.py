@@ -90,6 +90,26 @@ def test_borders_between_codes(cuda):
     assert torch.equal(got.double(), codes) and torch.equal(p.scales, scales)
 
 
+def test_borders_between_codes_of_the_smallest_scales(cuda):
+    """The same for scales of the lowest normal binades: half of such a scale may lie between two subnormal numbers."""
+    import tango_b200 as T
+    rng = np.random.default_rng(2)
+    rows = []
+    for exponent in (-126, -126, -126, -125, -124):
+        for _ in range(200):
+            s = float(np.float32(rng.uniform(1, 2) * 2.0 ** exponent))
+            m = np.float32(127 * s)
+            s = float(m / np.float32(127))
+            h = ((rng.integers(-126, 126, 41) + 0.5) * s).astype(np.float32)
+            rows.append(np.concatenate([[m], h, np.nextafter(h, np.float32(np.inf)), np.nextafter(h, np.float32(-np.inf))]))
+    x = torch.from_numpy(np.stack(rows).astype(np.float32)).cuda()
+    codes, scales, _ = reference(x, 124)
+    assert bool((scales >= 2.0 ** -126).all())
+    p = T.pack8(x, 124)
+    got, _ = codes_of(p, *x.shape)
+    assert torch.equal(p.scales, scales) and torch.equal(got.double(), codes)
+
+
 def test_groups_without_numbers_and_without_size(cuda):
     import tango_b200 as T
     x = torch.randn(6, 64, device="cuda")

@@ -254,3 +254,31 @@ def test_exact_rounding_in_32_bits():
         for xi, qi in zip(x.tolist(), q.tolist()):
             assert round(Fraction(xi) / Fraction(float(s))) == qi, (xi, float(s))
     assert math.isclose(float(s) * 127, float(m), rel_tol=1e-6)
+
+
+def test_exact_rounding_of_the_smallest_scales():
+    """The same in the arithmetic of the kernel alone -- every operation rounded to fp32 -- for scales from the smallest normal
+    number on, whose half may lie between two subnormal numbers: the remainder, doubled, against the scale and, for an odd code,
+    against the number below it."""
+    from fractions import Fraction
+    import numpy as np
+    f32 = np.float32
+    rng = np.random.default_rng(4)
+
+    def rounded(x, s, q):
+        rest = (x.astype(np.float64) - q.astype(np.float64) * float(s)).astype(f32)     # one fused operation
+        twice = np.abs(rest + rest)
+        assert twice.dtype == f32
+        limit = np.where(q.astype(np.int64) % 2 != 0, np.nextafter(s, f32(0)), s).astype(f32)
+        return q + np.where(twice > limit, np.sign(rest), f32(0))
+
+    for exponent in (-126, -126, -126, -125, -124, -120, 0, 100):
+        for _ in range(40):
+            s = f32(rng.uniform(1, 2) * 2.0 ** exponent)
+            k = np.arange(-126, 126)
+            x = ((k + 0.5) * float(s)).astype(f32)
+            x = np.concatenate([x, np.nextafter(x, f32(np.inf)), np.nextafter(x, f32(-np.inf))])
+            exact = [round(Fraction(float(a)) / Fraction(float(s))) for a in x]
+            for side in (np.floor, np.ceil):             # whichever code the approximate quotient led to
+                got = rounded(x, s, side(x.astype(np.float64) / float(s)).astype(f32))
+                assert got.tolist() == exact, float(s)
