@@ -372,10 +372,11 @@ __global__ void __launch_bounds__(kWarps * 32, InFlight<MODE>::kBlocks) attn_ker
         float4 rec[U];
     };
     const int stride = slots * U;
-    const int trips = (int)__reduce_max_sync(0xffffffffu, (unsigned)((end - beg + stride - 1) / stride));
-    const int last = end > beg ? end - 1 : 0;
+    // slots are counted without a sign: the trips ahead reach some hundred slots past a row's end, beyond 2^31 on the largest graphs
+    const int trips = (int)__reduce_max_sync(0xffffffffu, ((unsigned)(end - beg) + stride - 1) / stride);
+    const unsigned last = end > beg ? end - 1 : 0, behind = end;
     int next[U];
-    const auto ids = [&](int j) {
+    const auto ids = [&](unsigned j) {
 #pragma unroll
         for (int u = 0; u < U; ++u) next[u] = __ldg(a.indices + min(j + u * slots, last));
     };
@@ -388,13 +389,13 @@ __global__ void __launch_bounds__(kWarps * 32, InFlight<MODE>::kBlocks) attn_ker
             else t.kv[u] = __ldg(reinterpret_cast<const float2 *>(p));
         }
     };
-    const auto work = [&](const Trip &t, int j) {
+    const auto work = [&](const Trip &t, unsigned j) {
         if constexpr (MODE == FORWARD) {
             float z[U], sv[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const float s = dot<VB, P>(fa, t.a[u], start, lane, chunk);
-                z[u] = j + u * slots < end ? __fmul_rn(s, __fmul_rn(t.kv[u].x, sa)) : -INFINITY;
+                z[u] = j + u * slots < behind ? __fmul_rn(s, __fmul_rn(t.kv[u].x, sa)) : -INFINITY;
                 sv[u] = t.kv[u].y;
             }
             softmax_step<VB, U>(run, z, sv, t.b);
@@ -402,7 +403,7 @@ __global__ void __launch_bounds__(kWarps * 32, InFlight<MODE>::kBlocks) attn_ker
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const float s = dot<VB, P>(fa, t.a[u], start, lane, chunk), dp = dot<VB, P>(fb, t.b[u], start, lane, chunk) * t.kv[u].y;
-                const float z = j + u * slots < end ? __fmul_rn(s, __fmul_rn(t.kv[u].x, sa)) : -INFINITY;
+                const float z = j + u * slots < behind ? __fmul_rn(s, __fmul_rn(t.kv[u].x, sa)) : -INFINITY;
                 const float p = exp2_fast(z - top) * inv;
                 delta = fmaf(p, dp, delta);
                 const float pk = p * t.kv[u].x, pdk = pk * dp;
@@ -413,7 +414,7 @@ __global__ void __launch_bounds__(kWarps * 32, InFlight<MODE>::kBlocks) attn_ker
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const float s = dot<VB, P>(fa, t.a[u], start, lane, chunk), dp = dot<VB, P>(fb, t.b[u], start, lane, chunk) * sb;
-                const float z = j + u * slots < end ? __fmul_rn(s, __fmul_rn(sa, t.rec[u].x)) : -INFINITY;
+                const float z = j + u * slots < behind ? __fmul_rn(s, __fmul_rn(sa, t.rec[u].x)) : -INFINITY;
                 const float p = exp2_fast(z - t.rec[u].y) * t.rec[u].z;
                 const float ds = p * (dp - t.rec[u].w) * t.rec[u].x;
                 add_codes<VB>(run.acc, t.a[u], pair(ds, ds));
@@ -423,7 +424,7 @@ __global__ void __launch_bounds__(kWarps * 32, InFlight<MODE>::kBlocks) attn_ker
     };
     if (trips > 0) {
         Trip even, odd;
-        int j = beg + slot;
+        unsigned j = beg + slot;
         ids(j);
         load(even);
         ids(j + stride);
@@ -613,7 +614,7 @@ struct RowsArgs {
 constexpr int kRowChunk = 256;    // edges below which a row is not cut: four trips of a block of F = 128
 
 __host__ __device__ inline int row_chunk(int len, int splits) {
-    const int c = (len + splits - 1) / splits;
+    const int c = (int)(((unsigned)len + splits - 1) / splits);
     return c < kRowChunk ? kRowChunk : c;
 }
 
@@ -674,12 +675,14 @@ __global__ void __launch_bounds__(kRowWarps * 32, 5) attn_rows_kernel(const __gr
 
     Running<VB> run;
     const int stride = slots * U * kRowWarps;
-    int at[U], j = beg + warp * slots * U;
+    unsigned j = beg + warp * slots * U;            // without a sign, as in attn_kernel
+    const unsigned behind = end;
+    int at[U];
     Codes<VB> ga[U], gb[U];
     float sk[U], sv[U];
-    const auto ids = [&](int j) {
+    const auto ids = [&](unsigned j) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) at[u] = __ldg(a.indices + min(j + u * slots + slot, end - 1));
+        for (int u = 0; u < U; ++u) at[u] = __ldg(a.indices + min(j + u * slots + slot, behind - 1));
     };
     const auto load = [&] {
 #pragma unroll
@@ -690,7 +693,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 5) attn_rows_kernel(const __gr
             sv[u] = __ldg(a.sv + (int64_t)at[u] * a.heads + hd);
         }
     };
-    if (j < end) {
+    if (j < behind) {
         ids(j);
         load();
         ids(j + stride);
@@ -698,16 +701,16 @@ __global__ void __launch_bounds__(kRowWarps * 32, 5) attn_rows_kernel(const __gr
     float sa;
     const Codes<VB> fa = encode_query<VB, P>(a, r, head, chunk, query, sa);
     sa *= a.qscale;
-    while (j < end) {
+    while (j < behind) {
         float z[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const float s = dot<VB, P>(fa, ga[u], start, lane, chunk);
-            z[u] = counts && j + u * slots + slot < end ? __fmul_rn(s, __fmul_rn(sk[u], sa)) : -INFINITY;
+            z[u] = counts && j + u * slots + slot < behind ? __fmul_rn(s, __fmul_rn(sk[u], sa)) : -INFINITY;
         }
         softmax_step<VB, U>(run, z, sv, gb);
         j += stride;
-        if (j >= end) break;
+        if (j >= behind) break;
         load();
         ids(j + stride);
     }
@@ -747,7 +750,7 @@ __global__ void __launch_bounds__(256) attn_rows_merge_kernel(const __grid_const
     if (row < 0 || row >= a.n_nodes) return;
     const int len = __ldg(a.indptr + row + 1) - __ldg(a.indptr + row), chunk_len = row_chunk(len, a.splits);
     if (len <= chunk_len) return;
-    const int n = (len + chunk_len - 1) / chunk_len, per_head = (2 * a.heads + 3) / 4 * 4;
+    const int n = (int)(((unsigned)len + chunk_len - 1) / chunk_len), per_head = (2 * a.heads + 3) / 4 * 4;
     const int64_t step = partial_floats(FORWARD, a.heads, a.ld);
     const float *ws = a.ws + r * a.splits * step;
     for (int e = threadIdx.x; e < a.ld; e += blockDim.x) {

@@ -478,6 +478,51 @@ def test_offsets_beyond_32_bits(cuda):
     assert torch.equal(k8.unpack()[ends], T.pack8(parts[1], d).unpack())
 
 
+@pytest.mark.parametrize("end", ["long", "middle", "short"])
+def test_slots_at_the_end_of_32_bits(cuda, end):
+    """Rows whose slots end at 2^31 - 1, the last of them of each of the kernels' classes: the same bits as of a graph whose slots
+    begin at 0.  (The graph is symmetric, so that one array of 2^31 - 1 ids serves both directions.)"""
+    import tango_b200 as T
+    if torch.cuda.mem_get_info()[0] < 20 << 30:
+        pytest.skip("needs 20 GB")
+    n = 90
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    times = (torch.rand(n, n, device="cuda", generator=gen) < 0.05).int()          # rows of about nine edges,
+    times[0], times[1, 2:] = 8, 1                                                  # one of some 700 and one of some 100
+    times = torch.maximum(times, times.t())
+    order = torch.arange(n, device="cuda").roll({"long": -1, "middle": -2, "short": 0}[end])     # the last of the new order: 0, 1, n - 1
+    times = times[order][:, order]
+    near = torch.repeat_interleave(torch.arange(n, device="cuda").repeat(n), times.flatten()).int()
+    indptr = torch.cat([torch.zeros(1, device="cuda", dtype=torch.int64), times.sum(1).cumsum(0)])
+    e, most = near.numel(), 2 ** 31 - 1
+    far = torch.zeros(most, dtype=torch.int32, device="cuda")
+    far[most - e:] = near
+
+    class Slots:
+        def __init__(self, indptr, ids):
+            self.adj_csc = self.adj_csr = (indptr.int(), ids, None)
+            self.coo = near, near
+            self._identity = {"csc": True, "csr": True}
+            self._native = None
+
+        def num_nodes(self):
+            return n
+
+        def num_edges(self):
+            return e
+
+    at_0, at_end = Slots(indptr, near), Slots(indptr + (most - e), far)
+    assert int(at_end.adj_csc[0][-1]) == most
+    for h, d in ((1, 3), (4, 32), (3, 41)):
+        q, k, v, o = case(at_0, h, d)
+        want = run(at_0, q, k, v, o)
+        assert all(torch.equal(a, b) for a, b in zip(run(at_end, q, k, v, o), want))
+        k8, v8 = T.pack8(k, d), T.pack8(v, d)
+        for ids in (torch.arange(n, device="cuda"), torch.tensor([n - 1], device="cuda")):
+            rows = T.edge_attention_rows(at_end, ids, q[ids], k8, v8)
+            assert torch.equal(rows, T.edge_attention_rows(at_0, ids, q[ids], k8, v8))
+
+
 def test_stochastic_rounding_draws_anew(cuda):
     import tango_b200 as T
     from tango_b200 import config, kernels
