@@ -217,9 +217,14 @@ __host__ __device__ inline int64_t partial_floats(int mode, int heads, int64_t l
 // A softmax that is being added up: reference (of z * log2 e), sum, weighted sums of codes.  The reference follows the maximum
 // only when a score passes it by kSlack: weights up to 2^kSlack are as exact in fp32 as weights up to 1, and what has been added
 // up is rescaled once or twice a row, where the exact maximum changes in one of a warp's 32 softmaxes in nearly every trip
-// through rows of some hundred edges.  Before the first edge the reference is a number below all scores, so that nothing here
-// has to ask for it.
-constexpr float kBelow = -3.0e38f, kSlack = 8.f;
+// through rows of some hundred edges.  Before the first edge the reference is the lowest number, no score but one of minus
+// infinity is below it, so that nothing here has to ask for it.  A row whose scores have all passed the lowest number has the sum
+// 0 and no softmax: NaN, as a row with a score above the highest number.
+constexpr float kBelow = -3.402823466e38f, kSlack = 8.f;
+__device__ __forceinline__ float softmax_inverse(float l, bool edges) {
+    if (l == 0.f) return edges ? __int_as_float(0x7fffffff) : 0.f;
+    return __fdiv_rn(1.f, l);
+}
 template <int VB> struct Running {
     float m = kBelow, l = 0.f;
     Pair acc[VB / 2];
@@ -480,7 +485,7 @@ __global__ void __launch_bounds__(kWarps * 32, InFlight<MODE>::kBlocks) attn_ker
     const int64_t out = rh * a.d;
     const int e = chunk * VB;
     if constexpr (MODE == FORWARD) {
-        const float by = run.l == 0.f ? 0.f : __fdiv_rn(1.f, run.l);
+        const float by = softmax_inverse(run.l, end > beg);
         store_typed<VB>(a.out_a, out, a.type, e, a.d, run.acc, by);
         if (chunk == 0 && a.stats) a.stats[rh] = make_float2(run.l == 0.f ? 0.f : run.m, by);
     } else if constexpr (MODE == BY_DST) {
@@ -519,7 +524,8 @@ constexpr int kMergeThreads = 512;
 template <int MODE>
 __global__ void __launch_bounds__(kMergeThreads) attn_merge_kernel(const __grid_constant__ MergeArgs a) {
     __shared__ float s_x[kMergeThreads], s_y[kMergeThreads], s_z[kMergeThreads];
-    const int64_t row = __ldg(&a.rows[blockIdx.x].x);
+    const int4 heavy = __ldg(a.rows + blockIdx.x);
+    const int64_t row = heavy.x;
     const int first = __ldg(a.heavy_first + blockIdx.x), n = __ldg(a.heavy_first + blockIdx.x + 1) - first;
     const int64_t step = partial_floats(MODE, a.heads, a.ld);
     const float *ws = a.ws + (int64_t)first * step;
@@ -571,7 +577,7 @@ __global__ void __launch_bounds__(kMergeThreads) attn_merge_kernel(const __grid_
                 }
             }
             if constexpr (MODE == FORWARD) {
-                const float by = z == 0.f ? 0.f : __fdiv_rn(1.f, z);
+                const float by = softmax_inverse(z, heavy.z > heavy.y);
                 store_one(a.out_a, out, a.type, x * by);
                 if (i == 0 && a.stats) a.stats[rh] = make_float2(z == 0.f ? 0.f : m, by);
             } else if constexpr (MODE == BY_DST) {
@@ -735,7 +741,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 5) attn_rows_kernel(const __gr
             s = fmaf(s_acc[w][e], c, s);
         }
         if (whole) {
-            const float by = !known ? __int_as_float(0x7fffffff) : l == 0.f ? 0.f : __fdiv_rn(1.f, l);
+            const float by = known ? softmax_inverse(l, end0 > beg0) : __int_as_float(0x7fffffff);
             store_one(a.out, (r * a.heads + hd) * a.d + i, a.type, s * by);
         } else {
             float *ws = a.ws + (r * a.splits + blockIdx.y) * partial_floats(FORWARD, a.heads, a.ld);
@@ -763,7 +769,7 @@ __global__ void __launch_bounds__(256) attn_rows_merge_kernel(const __grid_const
             l = fmaf(ws[u * step + 2 * head + 1], c, l);
             s = fmaf(ws[u * step + per_head + e], c, s);
         }
-        store_one(a.out, (r * a.heads + head) * a.d + i, a.type, s * (l == 0.f ? 0.f : __fdiv_rn(1.f, l)));
+        store_one(a.out, (r * a.heads + head) * a.d + i, a.type, s * softmax_inverse(l, true));
     }
 }
 

@@ -215,6 +215,29 @@ def test_rows_with_infinities_and_nan_stay_apart(cuda):
     assert got[0][int(dst[0]), 0].isnan().all() and torch.equal(got[0][rest], clean[0][rest]) and torch.equal(got[1][rest], clean[1][rest])
 
 
+@pytest.mark.parametrize("times", [1, 100, 700])
+def test_scores_at_and_beyond_the_lowest_number(cuda, times):
+    """Rows of a part of a warp, of a warp, and cut into units: a score close to the lowest number takes part like any other;
+    one beyond it weighs nothing beside a finite one; a row of nothing else has no softmax, NaN in place of zeros."""
+    import tango_b200 as T
+    from tango_b200.graph import Graph
+    pairs = [(1, 0), (1, 2), (3, 2), (4, 5), (4, 6), (3, 6), (4, 7), (1, 7)]
+    src, dst = (torch.tensor(t, device="cuda").repeat(times) for t in zip(*pairs))
+    g = T.graph_preprocess(Graph(src, dst, 9), hub_block=0)
+    q = torch.ones(9, 1, 1, device="cuda")
+    k, v = torch.zeros_like(q), torch.arange(9.0, device="cuda").view(9, 1, 1)
+    k[1], k[4] = -2.2e38, -3e38              # times log2(e): -3.17e38 and minus infinity
+    want = torch.tensor([1.0, 0, 3, 0, 0, math.nan, 3, 1, 0], device="cuda").view(9, 1, 1)
+    out, dq, dk, dv = run(g, q, k, v, torch.ones_like(v), 1.0)
+    bound = (2 * 4 * times + 32) * E * want.abs()       # equal weights: the sums of their row and one quotient
+    assert torch.equal(out.isnan(), want.isnan()) and bool(((out - want).abs() <= bound)[~want.isnan()].all())
+    assert dq[5].isnan().all() and not dq[[0, 1, 2, 3, 4, 6, 7, 8]].isnan().any()
+    with torch.no_grad():
+        assert torch.equal(T.edge_attention(g, q, k, v, 1.0).nan_to_num(-1), out.nan_to_num(-1))
+    rows = T.edge_attention_rows(g, torch.arange(9, device="cuda"), q, T.pack8(k, 1), T.pack8(v, 1), 1.0)
+    assert torch.equal(rows.isnan(), want.isnan()) and bool(((rows - want).abs() <= bound)[~want.isnan()].all())
+
+
 def test_graph_that_was_not_preprocessed_and_strided_operands(cuda):
     import tango_b200 as T
     from tango_b200.graph import Graph
