@@ -294,6 +294,8 @@ class HGT(nn.Module):
     and v have a scale per node and head instead of one per tensor.  `keys_values` and `forward_rows` serve such a layer to a
     few nodes at a time."""
 
+    _fused = False      # also of a layer from a file of an earlier version, which has no such attribute
+
     def __init__(self, in_dim, out_dim, n_heads, dropout=0.2, use_norm=False, fused=False):
         super().__init__()
         self._fused = fused

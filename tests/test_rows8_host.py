@@ -185,6 +185,17 @@ def test_activations_that_have_an_8_bit_form():
         GAT(None, 2, 8, 4, 3, [2, 1], activation=F.relu, checkpoint="int8")
 
 
+def test_transformer_layers_of_earlier_files_run_the_chain():
+    """A layer that was saved whole before the fused form existed has no attribute that says so."""
+    import pickle
+    from tango_b200.gnn import HGT
+    layer = HGT(8, 16, 2)
+    layer.__dict__.pop("_fused")
+    old = pickle.loads(pickle.dumps(layer))
+    assert "_fused" not in old.__dict__ and old._fused is False
+    assert HGT(8, 16, 2, fused=True)._fused and pickle.loads(pickle.dumps(HGT(8, 16, 2, fused=True)))._fused
+
+
 @pytest.mark.parametrize("scale", [1, 3000])
 def test_units_cover_every_long_row_once(scale):
     """Also with enough edges for the limits to grow (lengths alone: the schedule reads nothing else)."""
