@@ -289,8 +289,9 @@ Tensor edge_attention_rows(const GraphPtr &g, const Tensor &rows_, const Tensor 
     const int64_t heads = q.size(1), d = q.size(2), r = q.size(0), n = g->n_nodes;
     for (const Rows8 *t : {&k_, &v_}) {
         require(t->q.device() == q.device() && t->scale.device() == q.device(), "keys and values must be on the GPU of the queries");
-        require(t->q.dim() == 2 && t->q.size(0) == n && t->q.size(1) == tango_rows8_ld(heads * d, d) && t->scale.dim() == 2 &&
-                    t->scale.size(0) == n && t->scale.size(1) == heads,
+        // (pack8 of a tensor without rows has no columns either)
+        require(t->q.dim() == 2 && t->q.size(0) == n && t->scale.dim() == 2 && t->scale.size(0) == n &&
+                    (n == 0 || (t->q.size(1) == tango_rows8_ld(heads * d, d) && t->scale.size(1) == heads)),
                 "keys and values packed with one row per node and one group per head expected");
     }
     require(std::isfinite((float)scale), "finite scale expected");

@@ -377,6 +377,18 @@ def test_few_rows_of_a_long_hub_and_unknown_ids(cuda):
     assert torch.equal(T.edge_attention_rows(g, at, wide[known][:, 30:94].unflatten(1, (2, 32)), k8, v8), got[known])
 
 
+def test_graph_without_nodes(cuda):
+    import tango_b200 as T
+    from tango_b200.graph import Graph
+    none = torch.zeros(0, dtype=torch.int64, device="cuda")
+    g = Graph(none, none, 0)
+    x = torch.zeros(0, 2, 8, device="cuda")
+    assert all(t.shape == (0, 2, 8) for t in run(g, x, x, x, x))
+    k8, v8 = T.pack8(x, 8), T.pack8(x, 8)
+    assert T.edge_attention_rows(g, none, x, k8, v8).shape == (0, 2, 8)
+    assert T.edge_attention_rows(g, torch.tensor([0, -1], device="cuda"), torch.ones(2, 2, 8, device="cuda"), k8, v8).isnan().all()
+
+
 def test_streams_and_captured_graphs(cuda):
     """A run on a side stream, and two captured training passes replayed in turn with new inputs."""
     import tango_b200 as T
