@@ -334,8 +334,10 @@ class HGT(nn.Module):
     def forward_rows(self, g, rows, h_rows, k8, v8):
         """The layer's output for the nodes `rows` alone, from their features h_rows and what `keys_values` gave.  As `forward`
         with fused=True, except that the projections of h_rows find their int8 scales in these rows alone."""
-        q = self.q_linear(h_rows).view(-1, self.n_heads, self.d_k)
-        return self.a_linear(edge_attention_rows(g, rows, q, k8, v8, 1.0 / self.sqrt_dk).view(-1, self.out_dim))
+        # the int8 products take one row at least
+        q = self.q_linear(h_rows) if len(h_rows) else h_rows.new_empty((0, self.out_dim))
+        out = edge_attention_rows(g, rows, q.view(-1, self.n_heads, self.d_k), k8, v8, 1.0 / self.sqrt_dk).view(-1, self.out_dim)
+        return self.a_linear(out) if len(h_rows) else out
 
 
 # ---------------------------------------------------------------------------------------------------- link prediction

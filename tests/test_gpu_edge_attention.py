@@ -389,6 +389,17 @@ def test_graph_without_nodes(cuda):
     assert T.edge_attention_rows(g, torch.tensor([0, -1], device="cuda"), torch.ones(2, 2, 8, device="cuda"), k8, v8).isnan().all()
 
 
+def test_transformer_layer_asked_for_no_rows(cuda):
+    from tango_b200.gnn import HGT
+    g = make_graph("sparse")
+    layer = HGT(12, 16, 2, fused=True).cuda()
+    x = torch.randn(g.num_nodes(), 12, device="cuda")
+    kept = layer.keys_values(x)
+    ids = torch.zeros(0, dtype=torch.int64, device="cuda")
+    got = layer.forward_rows(g, ids, x[ids], *kept)
+    assert got.shape == (0, 16) and got.dtype == torch.float32
+
+
 def test_streams_and_captured_graphs(cuda):
     """A run on a side stream, and two captured training passes replayed in turn with new inputs."""
     import tango_b200 as T
