@@ -589,6 +589,109 @@ def test_stochastic_rounding_draws_anew(cuda):
         assert float((x - w).norm() / w.norm()) < 0.1
 
 
+# ------------------------------------------------------------------------------------------------ bounds of every row's own
+# As above, but with what a value itself depends on: c = 16 (|z|max of the row + 1) + 2 depth + 32, where depth is the most terms that
+# meet one after another in a sum.  A row of up to 256 edges: that many.  A longer one on graphs of this size is cut into units of
+# 128, which meet one by one; the slots of a warp (32 at most) before them.  Sources add their own depth to their destinations' c.
+def depth_of(n):
+    return torch.where(n <= 256, n, 128 + 32 + n // 128 + 1)
+
+
+def own_bounds(g, q, k, v, o, scale, depth_of=depth_of):
+    src, dst = (t.long() for t in g.edges())
+    n, h, d = q.shape
+    dev = q.device
+
+    def total(at, t):
+        return torch.zeros(n, *t.shape[1:], device=dev, dtype=torch.float64).index_add(0, at, t)
+
+    z = (q[dst] * k[src]).sum(-1) * scale
+    top = torch.full((n, h), -math.inf, device=dev, dtype=torch.float64).scatter_reduce(0, dst[:, None].expand(-1, h), z, "amax")
+    zmax = torch.zeros(n, h, device=dev, dtype=torch.float64).scatter_reduce(0, dst[:, None].expand(-1, h), z.abs(), "amax")
+    p = torch.exp(z - top[dst])
+    p = p / total(dst, p)[dst]
+    into, out_of = (depth_of(torch.bincount(t, minlength=n)).double()[:, None, None] for t in (dst, src))
+    c = 16 * (zmax.unsqueeze(-1) + 1) + 2 * into + 32
+    adp = (o[dst].abs() * v[src].abs()).sum(-1)
+
+    def magnitudes(p):
+        full = (p * (adp + total(dst, p * adp)[dst])).unsqueeze(-1) * abs(scale)
+        p = p.unsqueeze(-1)
+        return p * v[src].abs(), full * k[src].abs(), full * q[dst].abs(), p * o[dst].abs()
+
+    out, dq, dk, dv = magnitudes(p)
+    bounds = [c * E * total(dst, out), c * E * total(dst, dq)]
+    bounds += [E * (total(src, c[dst] * t) + 2 * out_of * total(src, t)) for t in (dk, dv)]
+    flushed = [total(at, t) for at, t in zip((dst, dst, src, src), magnitudes(torch.full_like(p, FLUSHED)))]
+    return [a + b for a, b in zip(bounds, flushed)]
+
+
+@pytest.mark.parametrize("kind", ["sparse", "classes", "hubs"])
+@pytest.mark.parametrize("h,d", [(1, 3), (8, 8), (4, 32), (3, 41), (2, 100)])
+def test_every_row_within_bounds_of_its_own(cuda, kind, h, d):
+    g = make_graph(kind)
+    q, k, v, o = case(g, h, d)
+    at = [values(t) for t in (q, k, v, o)]
+    want = reference(g, *at, 1 / math.sqrt(d))[0]
+    check(run(g, q, k, v, o), want, own_bounds(g, *at, 1 / math.sqrt(d)), torch.float32)
+
+
+def test_rows_without_a_schedule(cuda):
+    """The kernels without a plan of the rows, every row by a warp, as C callers may have them."""
+    from tango_b200 import _native
+    for kind in ("pair", "classes", "hubs"):
+        g = make_graph(kind)
+        handle = _native.graph(g)
+        assert not handle.has_edge_schedule("csc") and not handle.has_edge_schedule("csr")
+        for h, d in ((1, 3), (4, 32), (3, 41)):
+            q, k, v, o = case(g, h, d)
+            at = [values(t) for t in (q, k, v, o)]
+            want = reference(g, *at, 1 / math.sqrt(d))[0]
+            leaves = [t.requires_grad_() for t in (q, k, v)]
+            out = _native.ops.edge_attention(handle, *leaves, 1 / math.sqrt(d))
+            got = [out.detach(), *torch.autograd.grad(out, leaves, o)]
+            check(got, want, own_bounds(g, *at, 1 / math.sqrt(d), depth_of=lambda n: n), torch.float32)
+
+
+def test_no_piece_of_a_long_row_is_lost(cuda):
+    """A row of 100,000 edges asked for: cut into 64 pieces of 1563, a lane of the four warps takes at most a quarter of one, then 32
+    slots, four warps and 64 pieces meet.  The bound is narrow enough to tell a lost piece: planted in the 64-bit form."""
+    import tango_b200 as T
+    from tango_b200._lib import lib
+    from tango_b200.graph import Graph
+    n, e, long = 5000, 140_000, 100_000
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    src = torch.randint(0, n, (e,), device="cuda", generator=gen)
+    dst = torch.cat([torch.full((long,), 17, device="cuda"), torch.randint(0, n, (e - long,), device="cuda", generator=gen)])
+    g = T.graph_preprocess(Graph(src, dst, n), hub_block=0)
+    q, k, v, o = case(g, 2, 32)
+    at = [values(t) for t in (q, k, v, o)]
+    scale = 1 / math.sqrt(32)
+    want = reference(g, *at, scale)[0][0]
+    indptr, ids = g.adj_csc[0], g.adj_csc[1].long()
+    first, end = indptr[17:19].tolist()
+    pieces = lib.tango_edge_attention_rows_splits(3, end - first)
+    piece = -(-(end - first) // pieces)
+    assert pieces == 64 and end - first > 99_999
+
+    def depth(n):
+        return torch.where(n <= 256, n, piece // 4 + 32 + 4 + pieces)
+
+    bound = own_bounds(g, *at, scale, depth_of=depth)[0]
+    rows = torch.tensor([17, 5, 4999], device="cuda")
+    got = T.edge_attention_rows(g, rows, q[rows], T.pack8(k, 32), T.pack8(v, 32))
+    check([got], [want[rows]], [bound[rows]], torch.float32)
+    check([T.edge_attention(g, q, k, v)[17:18]], [want[17:18]], [bound[17:18]], torch.float32)
+    key, value, query = at[1][ids[first:end]].cpu(), at[2][ids[first:end]].cpu(), at[0][17].cpu()
+    p = torch.softmax((key * query).sum(-1) * scale, 0)
+    for lost in (0, 31, pieces - 1):
+        kept = torch.ones(end - first, 1)
+        kept[lost * piece:(lost + 1) * piece] = 0
+        wrong = (p * kept).unsqueeze(-1) * value
+        wrong = wrong.sum(0) / (p * kept).sum(0).unsqueeze(-1)
+        assert bool(((wrong - want[17].cpu()).abs() > bound[17].cpu()).any())
+
+
 # ------------------------------------------------------------------------------------------------ models that call them
 def test_transformer_layer_fused_against_the_chain_and_served(cuda):
     from tango_b200.gnn import HGT

@@ -362,3 +362,60 @@ def test_packing_on_another_stream_and_in_a_captured_graph(cuda):
         graph.replay()
         for a, b in zip(outs, step()):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("kind", ["groups", "pitch", "columns", "run"])
+def test_indices_beyond_32_bits(cuda, kind):
+    """More than 2^31 groups, rows further apart than 2^31 elements, more than 2^31 columns (the last a run of whole groups): the same
+    bits as of parts that stay below."""
+    import tango_b200 as T
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("needs 60 GB")
+    gen = torch.Generator(device="cuda").manual_seed(5)
+
+    def randn(n):
+        x = torch.empty(n, device="cuda", dtype=torch.bfloat16)
+        for part in x.split(1 << 28):
+            part.normal_(generator=gen)
+        return x
+
+    if kind == "groups":
+        x = randn(65537 * 32768).view(65537, 32768)
+        p = T.pack8(x, 1)
+        assert p.scales.numel() > 2 ** 31
+        y = p.unpack()
+        for at in (slice(0, 3), slice(32760, 32770), slice(65530, 65537)):
+            part = T.pack8(x[at], 1)
+            assert torch.equal(p.codes[at], part.codes) and torch.equal(p.scales[at], part.scales)
+            assert torch.equal(y[at], part.unpack())
+    elif kind == "pitch":
+        far = 2 ** 31 + 1
+        x, dy = (randn(far + 700) for _ in range(2))
+        x, dy = x.as_strided((2, 601), (far, 1), 3), dy.as_strided((2, 601), (far, 1), 2)
+        a, b = T.pack8(x, 64), T.pack8(x.contiguous(), 64)
+        assert torch.equal(a.codes, b.codes) and torch.equal(a.scales, b.scales)
+        res = []
+        for t, g in ((x, dy), (x.contiguous(), dy.contiguous())):
+            leaf = t.detach().requires_grad_()
+            y = T.activation8(leaf, "silu", 64)
+            res.append((y.detach(), *torch.autograd.grad(y, leaf, g)))
+        assert all(torch.equal(a, b) for a, b in zip(*res))
+    else:
+        whole = 2 ** 31
+        x = randn(whole + (128 if kind == "run" else 67))
+        rest = x[whole:]
+        p = T.pack8(x)
+        a, b = T.pack8(x[:whole].view(-1, 128)), T.pack8(rest)
+        assert torch.equal(p.codes[0, :whole].view(-1, 128), a.codes) and torch.equal(p.codes[0, whole:], b.codes[0])
+        assert torch.equal(p.scales[0, :-1], a.scales[:, 0]) and torch.equal(p.scales[0, -1:], b.scales[0])
+        y = p.unpack()
+        assert torch.equal(y[:whole].view(-1, 128), a.unpack()) and torch.equal(y[whole:], b.unpack())
+        del p, a, b, y
+        leaf = x.requires_grad_()
+        y = T.activation8(leaf, "elu")
+        tail = rest.detach().requires_grad_()
+        z = T.activation8(tail, "elu")
+        dy = torch.ones_like(y)
+        dx, = torch.autograd.grad(y, leaf, dy)
+        dz, = torch.autograd.grad(z, tail, dy[whole:])
+        assert torch.equal(y[whole:], z) and torch.equal(dx[whole:], dz)
