@@ -170,6 +170,8 @@ def _add_edge_schedules(g, handle, formats) -> None:
                 if indptr.is_cuda:          # the next call may come on another stream
                     torch.cuda.current_stream(indptr.device).synchronize()
                 handle.set_edge_schedule(fmt, sched)
+                if fmt == "csc":
+                    handle.set_longest(sched.longest)
 
 
 def edge_graph(g, backward: bool):
@@ -183,7 +185,7 @@ def edge_graph(g, backward: bool):
 
 
 def rows_graph(g):
-    """The same with the length of the longest row, which is found at the first call."""
+    """The same with the length of the longest row, which is found at the first call, or was when the schedules were made."""
     handle = graph(g)
     if not handle.knows_longest():
         indptr = g.adj_csc[0]

@@ -94,6 +94,7 @@ PYBIND11_MODULE(_torch_ops, m) {
             (fmt == "csr" ? g.csr : g.csc)->edge_sched = edge_schedule(s);
         })
         .def("knows_longest", [](const Graph &g) { return g.longest >= 0; })
+        .def("longest", [](const Graph &g) { return g.longest; })
         .def("set_longest", [](Graph &g, int64_t n) { g.longest = n; });
 
     m.def("set_rounding", [](int gemm, int quantize, uint64_t seed) {

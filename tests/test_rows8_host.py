@@ -293,3 +293,15 @@ def test_exact_rounding_of_the_smallest_scales():
             for side in (np.floor, np.ceil):             # whichever code the approximate quotient led to
                 got = rounded(x, s, side(x.astype(np.float64) / float(s)).astype(f32))
                 assert got.tolist() == exact, float(s)
+
+
+def test_longest_row_is_found_once():
+    """The row schedule of the incoming edges knows it; serving behind a training pass does not look for it again."""
+    from tango_b200 import _native
+    for first in (_native.edge_graph, _native.rows_graph):
+        g = _graph()
+        longest = int(torch.bincount(g.edges()[1].long()).max())
+        handle = first(g, True) if first is _native.edge_graph else first(g)
+        assert handle.knows_longest() and handle.longest() == longest
+        assert handle.has_edge_schedule("csc") == handle.has_edge_schedule("csr") == (first is _native.edge_graph)
+        assert _native.rows_graph(g) is handle
