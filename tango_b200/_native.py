@@ -166,7 +166,7 @@ def _add_edge_schedules(g, handle, formats) -> None:
             if not handle.has_edge_schedule(fmt):
                 plan = getattr(g, "_plans", {}).get(fmt)
                 indptr = (g.adj_csc if fmt == "csc" else g.adj_csr)[0]
-                sched = EdgeSchedule(indptr, g.num_edges(), getattr(plan, "row_order", None))
+                sched = EdgeSchedule(indptr, g.num_edges(), rows=getattr(plan, "row_info", None))
                 if indptr.is_cuda:          # the next call may come on another stream
                     torch.cuda.current_stream(indptr.device).synchronize()
                 handle.set_edge_schedule(fmt, sched)

@@ -348,13 +348,16 @@ class EdgeSchedule:
     48 (head of the row order first, so that the walk of the longest is hidden), on 1.2 M edges 160 to 200 us against 96 with
     up to 160.  Units keep the longest walk short on small graphs (128 edges) and their partial results few on large ones."""
 
-    def __init__(self, indptr: torch.Tensor, nnz: Optional[int] = None, order: Optional[torch.Tensor] = None):
-        """nnz and order (the rows by decreasing length, SpmmSchedule.row_order) where they are known already."""
-        length = indptr[1:] - indptr[:-1]
-        n, dev = length.numel(), indptr.device
-        if order is None:
-            order = torch.argsort(length, descending=True, stable=True)
-        order = order.to(torch.int32)
+    def __init__(self, indptr: torch.Tensor, nnz: Optional[int] = None, order: Optional[torch.Tensor] = None,
+                 rows: Optional[torch.Tensor] = None):
+        """nnz, order (the rows by decreasing length) or `rows` itself (SpmmSchedule.row_info) where they are known already."""
+        n, dev = indptr.numel() - 1, indptr.device
+        if rows is None:
+            if order is None:
+                order = torch.argsort(indptr[1:] - indptr[:-1], descending=True, stable=True)
+            order = order.to(torch.int32)
+            rows = torch.stack([order, indptr[:-1][order], indptr[1:][order], torch.zeros_like(order)], 1)
+        self.rows = rows
         if nnz is None:
             nnz = int(indptr[-1]) if n else 0
         team = min(512, max(48, nnz // 8192))
@@ -363,10 +366,9 @@ class EdgeSchedule:
             unit *= 2
         # a row below it is one warp's; on large graphs a longer walk is hidden, and fewer rows have parts to merge
         self.threshold = 2 * unit if unit < 1024 else 4 * unit
-        self.rows = torch.stack([order, indptr[:-1][order], indptr[1:][order], torch.zeros_like(order)], 1)
         self.n_long = self.n_heavy = self.longest = self.n_units = 0
         if n:
-            ranked = torch.neg(length[order])          # ascending
+            ranked = rows[:, 1] - rows[:, 2]           # lengths below 0: ascending
             n_long, n_heavy = torch.searchsorted(ranked, torch.tensor([-team, -self.threshold], device=dev, dtype=ranked.dtype)).tolist()
             self.longest, self.n_heavy, self.n_long = -int(ranked[0]), n_heavy, max(n_long, n_heavy)
         if self.n_heavy == 0:

@@ -305,3 +305,24 @@ def test_longest_row_is_found_once():
         assert handle.knows_longest() and handle.longest() == longest
         assert handle.has_edge_schedule("csc") == handle.has_edge_schedule("csr") == (first is _native.edge_graph)
         assert _native.rows_graph(g) is handle
+
+
+def test_rows_of_the_schedule_are_those_of_the_aggregations():
+    """One list of the rows by decreasing length serves both kinds of kernels, and the units that are cut from it are the same."""
+    from tango_b200 import _native
+    from tango_b200.graph import EdgeSchedule, SpmmSchedule
+    g = _graph(60, 20000)
+    for fmt, indptr in (("csc", g.adj_csc[0]), ("csr", g.adj_csr[0])):
+        plan = g._plans[fmt] = SpmmSchedule(indptr)
+        kept, own = EdgeSchedule(indptr, g.num_edges(), rows=plan.row_info), EdgeSchedule(indptr)
+        assert kept.rows is plan.row_info and torch.equal(kept.rows, own.rows) and torch.equal(kept.units, own.units)
+        assert kept.n_units == own.n_units > 0 and torch.equal(kept.heavy_first, own.heavy_first)
+        assert (kept.n_heavy, kept.n_long, kept.longest) == (own.n_heavy, own.n_long, own.longest)
+    made = []
+    init = EdgeSchedule.__init__
+    try:
+        EdgeSchedule.__init__ = lambda self, *a, **k: (init(self, *a, **k), made.append(self))[0]
+        _native.edge_graph(g, True)
+    finally:
+        EdgeSchedule.__init__ = init
+    assert [s.rows is g._plans[fmt].row_info for s, fmt in zip(made, ("csc", "csr"))] == [True, True]
