@@ -947,7 +947,8 @@ extern "C" int tango_edge_attention_rows(const int32_t *indptr, const int32_t *i
     if (!indptr || !indices || !rows || !q || !out || (n_rows > 1 && ldq < (int64_t)heads * d)) return TANGO_EINVAL;
     if (n_nodes > 0 && (!k || !v || !good_codes(k->q, d) || !good_codes(v->q, d) || !k->scales || !v->scales)) return TANGO_EINVAL;
     if (splits > 1 && (!ws || ws_bytes < tango_edge_attention_rows_workspace_bytes(n_rows, splits, heads, d))) return TANGO_EINVAL;
-    if (!aligned(q, type == TANGO_FP32 ? 4 : 2) || !aligned(ws, 16)) return TANGO_EALIGN;
+    const int element = type == TANGO_FP32 ? 4 : 2;
+    if (!aligned(q, element) || !aligned(out, element) || !aligned(ws, 16)) return TANGO_EALIGN;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     RowsArgs a{};
     a.indptr = indptr; a.indices = indices; a.rows = rows; a.n_nodes = n_nodes; a.q = q; a.ldq = ldq;

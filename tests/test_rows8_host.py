@@ -116,6 +116,16 @@ def test_attention_arguments_are_checked_before_any_launch():
     assert 1 < lib.tango_edge_attention_rows_splits(1, 10 ** 6) <= 65535
 
 
+def test_output_of_a_few_rows_starts_on_an_element():
+    r = _Rows(0x1000, 0x2000)
+
+    def rows(out, kind):
+        return _lib().tango_edge_attention_rows(0x100, 0x200, 4, 0x500, 2, 1, 2, 16, 0x1000, 32, kind, _ref(r), _ref(r), 1.0, out, None, 0,
+                                                1, 0, 0, None, None)
+
+    assert rows(0x3002, 0) == -2 and rows(0x3001, 1) == -2 and rows(0x3003, 2) == -2
+
+
 def _graph(n=20, e=60, seed=0):
     from tango_b200.graph import Graph
     gen = torch.Generator().manual_seed(seed)
