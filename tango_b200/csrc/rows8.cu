@@ -282,8 +282,10 @@ template <int ACCESS> constexpr bool kAhead = ACCESS != TURNED;
 constexpr int kAheadBlocks = 16;        // blocks an SM of the kernels that take several tiles
 
 // Five blocks an SM where registers hold that: 232965 x 602 fp32 162 -> 152 us, bf16 SiLU of 169343 x 601 177 -> 174 (six: 153, 219).
+// In the other rows the compiler is asked for one block with an activation, for nothing (0) without: one block means 106 registers in
+// place of 80.  Packing 100000 x 500 in groups of 100 61 us against 84, x 1024 in one 134 against 203; GELU of the second 250 against 226.
 template <class T, int ACCESS, int LPG, int R, bool ACT>
-__global__ void __launch_bounds__(kBlock, ACCESS == TURNED && R <= 4 ? 5 : 1) rows8_pack_kernel(const __grid_constant__ Rows8Args a) {
+__global__ void __launch_bounds__(kBlock, ACCESS == TURNED ? (R <= 4 ? 5 : 1) : ACT ? 1 : 0) rows8_pack_kernel(const __grid_constant__ Rows8Args a) {
     constexpr int U = Tile<LPG, R>::U, NG = Tile<LPG, R>::kGroups;
     const int job = blockIdx.x % a.jobs, lane = threadIdx.x % LPG;
     const T *x = static_cast<const T *>(a.x[job]);
@@ -300,7 +302,7 @@ __global__ void __launch_bounds__(kBlock, ACCESS == TURNED && R <= 4 ? 5 : 1) ro
         }
     };
     // Where registers allow, a block takes several tiles and has the next one's loads under way: 100000 x 500 in groups of 100
-    // 78 -> 67 us.  (In turned rows it lost: 232965 x 602 166 -> 203.)
+    // 78 -> 67 us (61 with the other blocks as they are now).  (In turned rows it lost: 232965 x 602 166 -> 203.)
     int64_t tile = blockIdx.x / a.jobs;
     const int64_t tiles = (a.items + NG * U - 1) / (NG * U), apart = gridDim.x / a.jobs;
     fetch(tile);
