@@ -501,7 +501,8 @@ int tango_act8_backward(int act, const int8_t *q, const float *scales, int64_t r
  * n_heavy of them are cut into the units (row, first slot, end slot, place in the row), those of the i-th being units
  * heavy_first[i] .. heavy_first[i + 1]; rows up to n_long get a warp, the rest a part of one.  `rows` and `units` 16-byte aligned.
  * Units need a workspace, 16-byte aligned, of tango_edge_attention_workspace_bytes (pass 0 forward, 1 bwd_dst, 2 bwd_src).
- * d <= 512.  Every sum has one order, which depends on the row's length and the schedule.
+ * d <= 512.  Every sum has one order, which depends on the row's length and the schedule.  A score above the range of
+ * fp32 makes its row NaN; one below it weighs nothing, and a row of no others is NaN.
  * Replaces sddmm_u_dot_v -> edge_softmax -> spmm_u_mul_e (evaluation/test_HGT.py:58-62) and their backward passes. */
 typedef struct tango_edge_plan {
     const int32_t *rows;
@@ -537,7 +538,9 @@ int tango_edge_attention_bwd_src(const int32_t *indptr, const int32_t *indices, 
 /* The same attention of n_rows nodes `rows` (int64, any order, repeats allowed; an id outside [0, n_nodes) gives a row of NaN)
  * whose queries q [n_rows, heads, d] just arrived in `type` (leading dimension ldq, elements), over keys and values kept as
  * 8-bit rows.  A row may be cut over `splits` blocks (1: none; tango_edge_attention_rows_splits gives a number for the
- * longest row of the graph), which needs a workspace of tango_edge_attention_rows_workspace_bytes, 16-byte aligned. */
+ * longest row of the graph, fewer the more rows are asked for), which needs a workspace of
+ * tango_edge_attention_rows_workspace_bytes, 16-byte aligned.  Sums have one order per row length and `splits`: the last bits of
+ * a node's result may differ between calls that differ in it.  Keys and values: tango_rows8_pack's, dense. */
 int tango_edge_attention_rows_splits(int64_t n_rows, int64_t longest);
 int64_t tango_edge_attention_rows_workspace_bytes(int64_t n_rows, int splits, int heads, int d);
 int tango_edge_attention_rows(const int32_t *indptr, const int32_t *indices, int64_t n_nodes, const int64_t *rows, int64_t n_rows,

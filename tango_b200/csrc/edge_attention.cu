@@ -10,14 +10,18 @@
 // are the same ones).  delta is not needed beforehand: dq = scale * (sum p dp k - delta sum p k), so one walk
 // gathers delta and both sums, and what the forward pass has to keep is the 8-bit rows and two floats per row and head.
 //
-// Sums are fp32, in one order per row length and schedule (no atomics).
+// Sums are fp32, in one order per row length and schedule (no atomics); where a few rows are asked for, per row length and number of
+// blocks a row, which follows the number of rows asked for.
+//
+// dq as a difference of two sums leaves rounding where the formula cancels: a node with one incoming edge, whose dq is 0, gets up to
+// 2^-23 |dp| |k| (dk, which knows delta beforehand, gets 0).
 //
 // What bounds these kernels is the gather through L1 and L2: an edge brings 2 F bytes of codes and 8 H bytes of scales (16 H by
-// source), 5.8 GB for 20 M edges of 4 x 32.  On 232,965 nodes they take 535 us forward, 669 by destination and 785 by source (10.8,
-// 8.6 and 8.2 TB/s of gathered bytes; 20 to 30 % of the sectors miss L2, whose near half holds no table of 60 MB), on 114.6 M edges
-// of 4 x 16 1361 us forward (13.5 TB/s, issue slots two thirds busy).  Without the weighted sums (leaving out the conversion and
-// addition of v) the forward passes would take 527 and 1254 us where they took 615 and 1537: their arithmetic is mostly hidden, and
-// matrix instructions for it would buy little.
+// source), 5.8 GB for 20 M edges of 4 x 32.  On 232,965 nodes they take 529 us forward, 659 by destination and 773 by source (11.0,
+// 8.8 and 8.3 TB/s of gathered bytes; 20 to 30 % of the sectors miss L2, whose near half holds no table of 60 MB), on 114.6 M edges
+// of 4 x 16 1347 us forward (13.6 TB/s; on 40 M edges of the same nodes the issue slots are 70 % busy).  Without the weighted sums
+// (leaving out the conversion and addition of v) the forward passes would take 527 and 1254 us where they took 615 and 1537: their
+// arithmetic is mostly hidden, and matrix instructions for it would buy little.
 //   * k and v (in the backward pass q and the gradient, which the pass by destination lays out for the one by source) lie in turns
 //     of one lane's codes, so that a 32-byte load brings both: 20 M edges 631 -> 603 us forward, by source 913 -> 861.
 //   * The loads of a lane's next edges are issued before the present ones are worked on (InFlight), and none depends on a
@@ -65,7 +69,7 @@ struct AttnArgs {
     float *ws;                                      // partial results of the units
 };
 
-// Results below the normal numbers become 0: a probability that small is lost beside the row's largest, which is 1.
+// Results below the normal numbers become 0: a weight that small is lost beside the row's largest, which lies between 1 and 2^kSlack.
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -291,7 +295,8 @@ __device__ __forceinline__ void softmax_step(Running<VB> &r, const float (&z)[U]
 
 // Edges of a slot in one trip and blocks an SM: what is loaded one trip ahead hides the way to L2, against the registers that it
 // takes.  Forward / by destination / by source, us, 20 M edges of 4 x 32: 2, 2, 2 edges with 6, 4, 4 blocks 605 / 755 / 849;
-// 3, 3, 3 with 5, 3, 3 572 / 788 / 886; 4, 4, 4 with 6, 4, 4 609 / 693 / 814; as here 544 / 681 / 790.
+// 3, 3, 3 with 5, 3, 3 572 / 788 / 886; 4, 4, 4 with 6, 4, 4 609 / 693 / 814; as here 544 / 681 / 790 (all four on one GPU, 2 to 3 %
+// slower than the one of the figures above).
 template <int MODE> struct InFlight { static constexpr int U = MODE == FORWARD ? 4 : 3, kBlocks = MODE == FORWARD ? 5 : 4; };
 
 template <int MODE, int VB, int P>
@@ -923,7 +928,8 @@ extern "C" int tango_edge_attention_rows_splits(int64_t n_rows, int64_t longest)
     if (n_rows < 0 || longest < 0) return TANGO_EINVAL;
     if (n_rows == 0 || longest <= kRowChunk) return 1;
     // Most of a row's blocks find nothing to do unless it is a long one, and take their turn all the same: 1024 rows of 20 M
-    // edges (62 in the middle, 2021 at most), 4 x 32, take 39 us with one block a row, 26 with 4, 28 with 8 (from HBM).
+    // edges (62 in the middle, 2021 at most), 4 x 32, take 39 us with one block a row, 26 with 4, 28 with 8 (from HBM).  From 2049
+    // rows on a row is one block's, however long it is.
     const int64_t want = ceil_div(longest, kRowChunk), most = 4096 / n_rows < 64 ? 4096 / n_rows : 64;
     return (int)(want < most ? want : most < 1 ? 1 : most);
 }

@@ -7,10 +7,11 @@
 // Bound by HBM in principle: pack 5 bytes an fp32 element (4 read, 1 written), unpack 5, activation forward 9, backward 9.  A group
 // is owned by a few lanes, each with R times four neighbouring elements LPG * 4 apart (a load and the store of four codes are
 // contiguous over the lanes), so that x is read once and stays in registers.  Measured, GB/s of those bytes:
-//   contiguous groups of 4, 8, .. 128 columns: GELU of 232965 x 256 forward 100 us (5.4 TB/s), backward 79 (6.8, dy partly in L2);
-//     three matrices of 23 M elements, one launch, 94 us (3.7): 25 instructions an element keep the issue slots three quarters busy
-//   602 columns, fp32: pack 152 us (4.6: 28 instructions an element), unpack 111 (6.3); pairs of elements, half a sector, 217 and 163
-//   601 columns, bf16, SiLU: forward 174 us (2.9), backward 146 (3.5): the arithmetic pipe is 70 % busy, with 40 instructions an element
+//   contiguous groups of 4, 8, .. 128 columns: GELU of 232965 x 256 forward 98 us (5.5 TB/s), backward 79 (6.8, dy partly in L2);
+//     three matrices of 29.8 M elements, one launch, 94 us (4.8): 26 instructions an element keep the issue slots three quarters busy
+//   602 columns, fp32: pack 151 us (4.7: 28 instructions an element, issue slots 76 % busy), unpack 110 (6.4); pairs of elements, half a
+//     sector, 217 and 163
+//   601 columns, bf16, SiLU: forward 176 us (2.9), backward 146 (3.5): 49 and 39 instructions an element, issue slots 81 and 78 % busy
 // An earlier form with four elements a lane and 32 lanes a group took 408, 215 and 406 us where the first of each pair stands.
 #include "rows8.cuh"
 
@@ -58,7 +59,9 @@ __device__ __forceinline__ float over(float x, float y) {
     return x * r;
 }
 // Upper tail of the normal distribution at |x| times two, erfc(|x| / sqrt(2)), with e = exp(-x^2 / 2): the rational formula 7.1.26
-// of Abramowitz and Stegun's handbook (|error| < 1.5e-7), which shares the exponential with the density.
+// of Abramowitz and Stegun's handbook (|error| < 1.5e-7), which shares the exponential with the density.  The error is of the
+// size of fp32's rounding of 1 + erf, but a choice all the same: GELU of 232965 x 256 normal numbers (1.5 wide) and its gradient are
+// 9.5e-8 of their norm from 64 bits, erf and exp in full 4.9e-8; for x below about -5, where 1 + erf cancels, the formula is closer.
 __device__ __forceinline__ float normal_tails(float x, float e) {
     const float t = over(1.f, fmaf(0.3275911f * 0.70710678118654752f, fabsf(x), 1.f));
     float p = fmaf(1.061405429f, t, -1.453152027f);

@@ -254,7 +254,8 @@ class QGATConv(nn.Module):
 
 class GAT(nn.Module):
     """evaluation/test_gat.py:172-224.  checkpoint="int8": the activations between the layers keep their input in 8 bits for the
-    backward pass instead of in fp32 (`rows8.activation8`); the outputs are the same."""
+    backward pass instead of in fp32 (`rows8.activation8`); the activations themselves are the same to fp32's rounding, which the
+    next layer's int8 codes may show."""
 
     def __init__(self, g, num_layers, in_dim, num_hidden, num_classes, heads, activation=F.elu, feat_drop=0.0,
                  attn_drop=0.0, negative_slope=0.2, residual=False, fused=True, checkpoint=None):

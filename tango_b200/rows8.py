@@ -59,8 +59,8 @@ _TORCH = {F.elu: "elu", torch.nn.functional.gelu: "gelu", F.silu: "silu"}
 
 def activation8(x: torch.Tensor, kind: str = "elu", group: int = GROUP) -> torch.Tensor:
     """ELU (alpha = 1), GELU (erf) or SiLU of x, which keeps an 8-bit copy of x for its backward pass in place of x itself: a
-    quarter of the memory in fp32, made in the same pass over x.  The output is that of the plain activation; the gradient is
-    dy * f'(copy of x).  The three are smooth, so that a copy off by half a step moves the slope by no more than that; a
+    quarter of the memory in fp32, made in the same pass over x.  The output is that of the plain activation to fp32's
+    rounding (GELU by a formula of the error function that is off by at most 1.5e-7); the gradient is dy * f'(copy of x).  The three are smooth, so that a copy off by half a step moves the slope by no more than that; a
     ReLU, whose slope hangs on the sign of small values, is not offered."""
     if kind not in _KINDS:
         raise ValueError(f"activation8: {kind!r} is not one of {', '.join(_KINDS)}")
