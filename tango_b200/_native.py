@@ -159,8 +159,15 @@ def graph(g):
 _edge_lock = threading.Lock()
 
 
+def _refuse_capture(what) -> None:
+    """What waits for the GPU would end a capture with a CUDA error."""
+    if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(f"{what} made at a graph's first call, which cannot be inside a captured CUDA graph: call it once before")
+
+
 def _add_edge_schedules(g, handle, formats) -> None:
     from .graph import EdgeSchedule
+    _refuse_capture("the row schedules of edge_attention (those of the backward pass at the first call with a gradient) are")
     with _edge_lock:
         for fmt in formats:
             if not handle.has_edge_schedule(fmt):
@@ -188,6 +195,7 @@ def rows_graph(g):
     """The same with the length of the longest row, which is found at the first call, or was when the schedules were made."""
     handle = graph(g)
     if not handle.knows_longest():
+        _refuse_capture("the look for the longest row of edge_attention_rows is")
         indptr = g.adj_csc[0]
         handle.set_longest(int((indptr[1:] - indptr[:-1]).max()) if g.num_nodes() else 0)
     return handle

@@ -436,6 +436,39 @@ def test_streams_and_captured_graphs(cuda):
                 assert torch.equal(a, b)
 
 
+def test_first_calls_inside_a_capture_are_refused(cuda):
+    """With an error that says so, before any work: the capture and the process go on."""
+    import tango_b200 as T
+    g = make_graph("hubs")
+    q, k, v, o = case(g, 4, 16)
+    k8, v8, ids = T.pack8(k, 16), T.pack8(v, 16), torch.arange(5, device="cuda")
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+
+    def refused(f):
+        x = torch.zeros(8, device="cuda")
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            x.add_(1)
+            with pytest.raises(RuntimeError, match="first call"):
+                f()
+            x.add_(1)
+        graph.replay()
+        assert x.eq(2).all()
+
+    refused(lambda: T.edge_attention_rows(g, ids, q[:5], k8, v8))
+    refused(lambda: T.edge_attention(g, q, k, v))
+    want = T.edge_attention(g, q, k, v)
+    refused(lambda: T.edge_attention(g, *leaves))           # the sources' schedule is still missing
+    assert torch.equal(run(g, q, k, v, o)[0], want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = run(g, q, k, v, o)
+        rows = T.edge_attention_rows(g, ids, q[:5], k8, v8)
+    graph.replay()
+    assert torch.equal(outs[0], want) and torch.equal(rows, T.edge_attention_rows(g, ids, q[:5], k8, v8))
+
+
 def test_captured_backward_beside_a_living_graph_of_the_same_leaves(cuda):
     import tango_b200 as T
     g = make_graph("hubs")
